@@ -288,6 +288,85 @@ mt_status mt_rope_attention(mt_ctx* ctx, void* stream, const float* qkv, int ldq
 mt_status mt_qwen_decode(mt_ctx* ctx, void* stream, const mt_qwen_weights* w, int requests, int rows, float* x,
                          float* kv, long long kv_stride, int capacity, const int32_t* positions, float* z);
 
+/* ---------------------------------------------------------------------------------------------
+ * 8-bit key/value caches: written, read back and attended to (no counterpart in the reference,
+ * whose caches are fp32, Qwen.swift:7-26)
+ *
+ * A cache holds the last `capacity` positions from `base` on of each request: 64 codes of one byte
+ * and one fp32 scale per (head, position), the value being code * scale. 136 bytes per position and
+ * head for keys and values against 512 in fp32.
+ *
+ * Rows: the calls take `requests` requests of `rows` rows each (row i of request r is row
+ * r * rows + i of the row-strided buffers). Row i of request r is at position positions[r] + i
+ * (device int32 [requests]). counts (device int32 [requests], or NULL: all rows) gives the rows of
+ * each request that are its own; the rows behind them are padding: nothing is read from them and
+ * what the outputs hold there stays. The same holds for every row of a request whose position is
+ * below the cache's base or with rows that would reach position 2^31 - 1 (an idle request: -1).
+ * Device memory of the call (tensors, positions, counts) is on ctx's device; the device current on
+ * the calling thread does not matter.
+ * ------------------------------------------------------------------------------------------- */
+enum { MT_KV_INT8 = 0, MT_KV_E4M3 = 1 };
+
+typedef struct {
+    int kind;                  /* MT_KV_INT8: signed integers, |code| <= 127. MT_KV_E4M3: 8-bit floats
+                                  (4 exponent, 3 mantissa bits, largest 448, no infinities) */
+    int kv_heads;
+    int capacity;              /* slots per request and head; position p is in slot (p - base) % capacity */
+    int base;                  /* first position the cache can hold: 0, or the length of a shared prefix */
+    long long request_stride;  /* slots from one request to the next: >= kv_heads * capacity */
+    uint8_t *k, *v;            /* codes [requests][kv_heads][capacity][64], 16-byte aligned */
+    float *k_scale, *v_scale;  /* [requests][kv_heads][capacity] */
+} mt_kv8_cache;
+
+/* NeoX RoPE (pairs i, i+32; angle = position * inv_freq[i] in 64 bits) of q and k, and the write to
+ * the cache: q_out[row, hq*64] (row stride ldqo) gets the rotated query heads, the rotated keys and
+ * the raw values of each row are quantised into its position's slot. qkv rows are [q | k | v]; q_out
+ * may be qkv itself (rotation in place), qkv is otherwise not modified.
+ * Of the 64 fp32 values x of a head (rotated keys are rounded to fp32 first): scale = max|x| / 127 (or
+ * 448), rounded to fp32, and each code is the nearest to x / scale, ties to even. A scale below
+ * 2^-126 is stored as 0 with codes 0; where a value is infinite or NaN, the scale is NaN and the
+ * codes are 0, so that every reader of that slot sees NaN. Requires rows <= capacity.
+ * The 8-bit form of mt_rope_cache, for a batch. */
+mt_status mt_rope_cache_kv8(mt_ctx* ctx, void* stream, const float* qkv, int ldq, int requests, int rows, int hq,
+                            const int32_t* positions, const int32_t* counts, const float* inv_freq,
+                            const mt_kv8_cache* cache, float* q_out, int ldqo);
+
+/* Reads positions back: row i of request r to k[r][head][i][64] and v[r][head][i][64] as fp32, code *
+ * scale, with out_capacity rows per head (>= rows): the layout of the fp32 caches, slot i holding
+ * position positions[r] + i. k or v may be NULL. Requires rows <= capacity. What is read from a
+ * position that was not written, or not held any more, is what its slot holds. */
+mt_status mt_kv8_read(mt_ctx* ctx, void* stream, const mt_kv8_cache* cache, int requests, int rows,
+                      const int32_t* positions, const int32_t* counts, float* k, float* v, int out_capacity);
+
+/* Causal GQA attention of every row over its request's cache, scale 1/8, which holds the rows' own
+ * positions too (mt_rope_cache_kv8 first): the row at position p sees the positions up to p that the
+ * cache holds, that is from max(base, last - capacity + 1) on, last being its request's last position;
+ * with window > 0 only those above p - window. One row per request (a decode step), a few or a whole
+ * prompt: any rows <= capacity, and window + rows - 1 <= capacity with a window.
+ * q[row, hq*64] is rotated already (row stride ldq); out[row, hq*64] (row stride ldo) must not
+ * overlap q. Slots that no row sees may hold anything, except that e4m3 codes of seen slots are
+ * never NaN (mt_rope_cache_kv8 writes none). workspace: device memory of at least
+ * mt_attention_kv8_workspace bytes, 16-byte aligned, its contents irrelevant before and after; calls
+ * that can overlap on the GPU need one each. NULL where that is 0.
+ * The 8-bit form of mt_attention, for a batch. */
+mt_status mt_attention_kv8(mt_ctx* ctx, void* stream, const float* q, int ldq, int requests, int rows, int hq,
+                           const int32_t* positions, const int32_t* counts, int window, const mt_kv8_cache* cache,
+                           float* out, int ldo, void* workspace, size_t workspace_bytes);
+/* Bytes of workspace that mt_attention_kv8 needs for these arguments on ctx (0: none). */
+size_t mt_attention_kv8_workspace(const mt_ctx* ctx, const mt_kv8_cache* cache, int requests, int rows, int hq, int window);
+
+/* Attention of a batch whose requests share a prefix (a voice prompt, a system prompt): every row sees
+ * all prefix_len positions of `prefix` (one request's cache with base 0, prefix_len <= capacity) and,
+ * causally, its own request's positions in `cache`, whose base is prefix_len. The prefix is read and
+ * multiplied once for the rows of all requests together. The two caches may differ in kind; prefix_len 0
+ * (prefix may be NULL) is mt_attention_kv8 without a window. The rest as there. */
+mt_status mt_attention_prefix_kv8(mt_ctx* ctx, void* stream, const float* q, int ldq, int requests, int rows, int hq,
+                                  const int32_t* positions, const int32_t* counts, const mt_kv8_cache* prefix,
+                                  int prefix_len, const mt_kv8_cache* cache, float* out, int ldo, void* workspace,
+                                  size_t workspace_bytes);
+size_t mt_attention_prefix_kv8_workspace(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int requests,
+                                         int rows, int hq);
+
 /* Full attention over `batch` sequences of `seq` <= 8 rows with interleaved RoPE (pairs 2l, 2l+1,
  * angle = row * inv_freq[l]). qkv rows are [q | k | v] of heads*64 each, row stride ld.
  * Replaces Encoder.ditAttention (Kernels.swift:210-220), dit_attention (Shaders.swift:613-648). */

@@ -109,7 +109,14 @@ class ConvDecWeights(ctypes.Structure):
                 ("out_w", c_void_p), ("out_b", c_void_p)]
 
 
+class KV8CacheStruct(ctypes.Structure):
+    _fields_ = [("kind", c_int), ("kv_heads", c_int), ("capacity", c_int), ("base", c_int),
+                ("request_stride", ctypes.c_longlong), ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p),
+                ("v_scale", c_void_p)]
+
+
 MT_DTYPE_BF16, MT_DTYPE_F32 = 0, 1
+MT_KV_INT8, MT_KV_E4M3 = 0, 1
 BUF_Z, BUF_STOP_LOGITS, BUF_LATENTS, BUF_AGG_OUT, BUF_VELOCITY0, BUF_VAE_HIDDEN, BUF_PCM = range(7)
 
 
@@ -141,6 +148,13 @@ PROTOTYPES = {
     "mt_qwen_decode": (c_int, [_P, _P, _P, c_int, c_int, _P, _P, ctypes.c_longlong, c_int, _P, _P]),
     "mt_rope_cache": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P, _P, c_int, _P]),
     "mt_attention": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, _P, _P, c_int, _P, c_int]),
+    "mt_rope_cache_kv8": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P, c_int]),
+    "mt_kv8_read": (c_int, [_P, _P, _P, c_int, c_int, _P, _P, _P, _P, c_int]),
+    "mt_attention_kv8": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, _P, _P, c_int, _P, _P, c_int, _P, c_size_t]),
+    "mt_attention_kv8_workspace": (c_size_t, [_P, _P, c_int, c_int, c_int, c_int]),
+    "mt_attention_prefix_kv8": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, _P, _P, _P, c_int, _P, _P, c_int, _P,
+                                        c_size_t]),
+    "mt_attention_prefix_kv8_workspace": (c_size_t, [_P, c_int, _P, c_int, c_int, c_int]),
     "mt_dit_attention": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, _P, _P, c_int]),
     "mt_flow_assemble": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, _P]),
     "mt_flow_euler": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_float, c_float, _P]),
@@ -303,8 +317,108 @@ class Context:
     def attention(self, q, ldq, m, hq, hkv, pos0, window, kc, vc, cap, out, ldo):
         self.call("attention", q, ldq, m, hq, hkv, pos0, window, kc, vc, cap, out, ldo)
 
+    # 8-bit caches: `cache` and `prefix` are KV8Cache objects, the rest as in mingcuda.h. The current
+    # stream is the one of the context's device.
+    def _kv8(self, st: int, what: str):
+        if st != MT_OK:
+            self._check(st, what)
+
+    def _stream(self, stream):
+        if stream is not None:
+            return stream
+        import torch
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _workspace(self, nbytes: int, given):
+        """(tensor, pointer, bytes): the caller's workspace, or a new one from torch's allocator."""
+        if given is not None:
+            return given, given.data_ptr(), given.numel() * given.element_size()
+        if nbytes == 0:
+            return None, None, 0
+        import torch
+        t = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{self.device}")
+        return t, t.data_ptr(), nbytes
+
+    def _requests(self, requests: int, *caches):
+        for c in caches:
+            if c.requests < requests:
+                raise MingError(MT_ERR_SHAPE, f"{requests} requests, but a cache of {c.requests}")
+
+    def rope_cache_kv8(self, qkv, ldq, requests, rows, hq, positions, counts, inv_freq, cache, q_out, ldqo, stream=None):
+        """mt_rope_cache_kv8: rotate q and k, quantise k and v into the cache."""
+        self._requests(requests, cache)
+        self._kv8(lib().mt_rope_cache_kv8(self._ctx, self._stream(stream), ptr(qkv), ldq, requests, rows, hq,
+                                          ptr(positions), ptr(counts), ptr(inv_freq), cache.ref, ptr(q_out), ldqo),
+                  "mt_rope_cache_kv8")
+
+    def kv8_read(self, cache, requests, rows, positions, counts, k, v, out_capacity, stream=None):
+        """mt_kv8_read: a range of positions back into fp32."""
+        self._requests(requests, cache)
+        self._kv8(lib().mt_kv8_read(self._ctx, self._stream(stream), cache.ref, requests, rows, ptr(positions),
+                                    ptr(counts), ptr(k), ptr(v), out_capacity), "mt_kv8_read")
+
+    def attention_kv8(self, q, ldq, requests, rows, hq, positions, counts, window, cache, out, ldo, workspace=None,
+                      stream=None):
+        """mt_attention_kv8: causal attention over the cache. Without a workspace (a CUDA tensor), one comes
+        from torch's allocator on the current stream: give one when `stream` is another."""
+        self._requests(requests, cache)
+        n = lib().mt_attention_kv8_workspace(self._ctx, cache.ref, requests, rows, hq, window)
+        keep, wp, wn = self._workspace(n, workspace)
+        self._kv8(lib().mt_attention_kv8(self._ctx, self._stream(stream), ptr(q), ldq, requests, rows, hq, ptr(positions),
+                                         ptr(counts), window, cache.ref, ptr(out), ldo, wp, wn), "mt_attention_kv8")
+
+    def attention_prefix_kv8(self, q, ldq, requests, rows, hq, positions, counts, prefix, prefix_len, cache, out, ldo,
+                             workspace=None, stream=None):
+        """mt_attention_prefix_kv8: attention over a prefix all requests share and each one's own cache."""
+        self._requests(requests, cache)
+        n = lib().mt_attention_prefix_kv8_workspace(self._ctx, prefix_len, cache.ref, requests, rows, hq)
+        keep, wp, wn = self._workspace(n, workspace)
+        self._kv8(lib().mt_attention_prefix_kv8(self._ctx, self._stream(stream), ptr(q), ldq, requests, rows, hq,
+                                                ptr(positions), ptr(counts), prefix.ref if prefix is not None else None,
+                                                prefix_len, cache.ref, ptr(out), ldo, wp, wn), "mt_attention_prefix_kv8")
+
     def dit_attention(self, qkv, ld, batch, seq, heads, inv_freq, out, ldo):
         self.call("dit_attention", qkv, ld, batch, seq, heads, inv_freq, out, ldo)
+
+
+class KV8Cache:
+    """mt_kv8_cache over torch tensors: codes k, v [requests, kv_heads, capacity, 64] (torch.int8 or
+    torch.float8_e4m3fn) and fp32 scales k_scale, v_scale [requests, kv_heads, capacity] on one CUDA
+    device. The last three (two) dimensions are dense; requests may be any multiple of a slot apart, the
+    same in all four (views of a slab with several layers). KV8Cache.allocate makes a zeroed one.
+    Position p is in slot (p - base) % capacity."""
+
+    def __init__(self, k, v, k_scale, v_scale, base: int = 0):
+        import torch
+        kinds = {torch.int8: MT_KV_INT8, torch.float8_e4m3fn: MT_KV_E4M3}
+        if k.dtype not in kinds or v.dtype != k.dtype:
+            raise TypeError(f"KV8Cache: codes of torch.int8 or torch.float8_e4m3fn, got {k.dtype} and {v.dtype}")
+        if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+            raise TypeError("KV8Cache: scales are torch.float32")
+        if k.dim() != 4 or k.shape[3] != 64 or v.shape != k.shape or not k_scale.shape == v_scale.shape == k.shape[:3]:
+            raise ValueError(f"KV8Cache: codes [requests, kv_heads, capacity, 64] and scales [requests, kv_heads, "
+                             f"capacity], got {[tuple(t.shape) for t in (k, v, k_scale, v_scale)]}")
+        if any(not t.is_cuda or t.device != k.device for t in (k, v, k_scale, v_scale)):
+            raise ValueError("KV8Cache: the four tensors are on one CUDA device")
+        requests, heads, capacity = k.shape[:3]
+        stride = k.stride(0) // 64 if requests > 1 else heads * capacity
+        for t, unit in ((k, 64), (v, 64), (k_scale, 1), (v_scale, 1)):
+            inner = (capacity * unit, unit, 1)[:t.dim() - 1]
+            if t.numel() and (tuple(t.stride()[1:]) != inner and not t[0].is_contiguous()
+                              or requests > 1 and t.stride(0) != stride * unit):
+                raise ValueError(f"KV8Cache: strides {t.stride()} of a tensor [{requests}, {heads}, {capacity}, ...]")
+        self.tensors = (k, v, k_scale, v_scale)  # kept alive
+        self.k, self.v, self.k_scale, self.v_scale = self.tensors
+        self.requests, self.base, self.device = requests, base, k.device
+        self.struct = KV8CacheStruct(kinds[k.dtype], heads, capacity, base, stride, *(t.data_ptr() for t in self.tensors))
+        self.ref = ctypes.byref(self.struct)
+
+    @classmethod
+    def allocate(cls, requests: int, kv_heads: int, capacity: int, dtype=None, base: int = 0, device="cuda") -> "KV8Cache":
+        import torch
+        k, v = (torch.zeros(requests, kv_heads, capacity, 64, dtype=dtype or torch.int8, device=device) for _ in range(2))
+        ks, vs = (torch.zeros(requests, kv_heads, capacity, device=device) for _ in range(2))
+        return cls(k, v, ks, vs, base)
 
 
 def version() -> str:
