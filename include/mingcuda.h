@@ -311,7 +311,8 @@ typedef struct {
     int kind;                  /* MT_KV_INT8: signed integers, |code| <= 127. MT_KV_E4M3: 8-bit floats
                                   (4 exponent, 3 mantissa bits, largest 448, no infinities) */
     int kv_heads;
-    int capacity;              /* slots per request and head; position p is in slot (p - base) % capacity */
+    int capacity;              /* slots per request and head, at most 2^30; position p is in slot
+                                  (p - base) % capacity */
     int base;                  /* first position the cache can hold: 0, or the length of a shared prefix */
     long long request_stride;  /* slots from one request to the next: >= kv_heads * capacity */
     uint8_t *k, *v;            /* codes [requests][kv_heads][capacity][64], 16-byte aligned */

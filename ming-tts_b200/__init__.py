@@ -317,65 +317,71 @@ class Context:
     def attention(self, q, ldq, m, hq, hkv, pos0, window, kc, vc, cap, out, ldo):
         self.call("attention", q, ldq, m, hq, hkv, pos0, window, kc, vc, cap, out, ldo)
 
-    # 8-bit caches: `cache` and `prefix` are KV8Cache objects, the rest as in mingcuda.h. The current
-    # stream is the one of the context's device.
-    def _kv8(self, st: int, what: str):
-        if st != MT_OK:
-            self._check(st, what)
-
-    def _stream(self, stream):
-        if stream is not None:
-            return stream
+    # 8-bit caches: `cache` and `prefix` are KV8Cache objects, the other tensors CUDA tensors, the rest as
+    # in mingcuda.h. The default stream is the current one of the context's device. A decode step is a
+    # few microseconds of GPU time, so these wrappers do little else than the call.
+    def _device_stream(self) -> int:
         import torch
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.device)
+
+    def _enough(self, cache, requests: int):
+        if cache.requests < requests:
+            raise MingError(MT_ERR_SHAPE, f"{requests} requests, but a cache of {cache.requests}")
 
     def _workspace(self, nbytes: int, given):
         """(tensor, pointer, bytes): the caller's workspace, or a new one from torch's allocator."""
-        if given is not None:
-            return given, given.data_ptr(), given.numel() * given.element_size()
-        if nbytes == 0:
-            return None, None, 0
-        import torch
-        t = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{self.device}")
-        return t, t.data_ptr(), nbytes
-
-    def _requests(self, requests: int, *caches):
-        for c in caches:
-            if c.requests < requests:
-                raise MingError(MT_ERR_SHAPE, f"{requests} requests, but a cache of {c.requests}")
+        if given is None:
+            import torch
+            given = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", self.device))
+        return given, given.data_ptr(), given.numel() * given.element_size()
 
     def rope_cache_kv8(self, qkv, ldq, requests, rows, hq, positions, counts, inv_freq, cache, q_out, ldqo, stream=None):
         """mt_rope_cache_kv8: rotate q and k, quantise k and v into the cache."""
-        self._requests(requests, cache)
-        self._kv8(lib().mt_rope_cache_kv8(self._ctx, self._stream(stream), ptr(qkv), ldq, requests, rows, hq,
-                                          ptr(positions), ptr(counts), ptr(inv_freq), cache.ref, ptr(q_out), ldqo),
-                  "mt_rope_cache_kv8")
+        self._enough(cache, requests)
+        st = lib().mt_rope_cache_kv8(self._ctx, self._device_stream() if stream is None else stream, qkv.data_ptr(), ldq,
+                                     requests, rows, hq, positions.data_ptr(),
+                                     None if counts is None else counts.data_ptr(), inv_freq.data_ptr(), cache.ref,
+                                     q_out.data_ptr(), ldqo)
+        if st != MT_OK:
+            self._check(st, "mt_rope_cache_kv8")
 
     def kv8_read(self, cache, requests, rows, positions, counts, k, v, out_capacity, stream=None):
         """mt_kv8_read: a range of positions back into fp32."""
-        self._requests(requests, cache)
-        self._kv8(lib().mt_kv8_read(self._ctx, self._stream(stream), cache.ref, requests, rows, ptr(positions),
-                                    ptr(counts), ptr(k), ptr(v), out_capacity), "mt_kv8_read")
+        self._enough(cache, requests)
+        st = lib().mt_kv8_read(self._ctx, self._device_stream() if stream is None else stream, cache.ref, requests, rows,
+                               positions.data_ptr(), None if counts is None else counts.data_ptr(), ptr(k), ptr(v),
+                               out_capacity)
+        if st != MT_OK:
+            self._check(st, "mt_kv8_read")
 
     def attention_kv8(self, q, ldq, requests, rows, hq, positions, counts, window, cache, out, ldo, workspace=None,
                       stream=None):
         """mt_attention_kv8: causal attention over the cache. Without a workspace (a CUDA tensor), one comes
         from torch's allocator on the current stream: give one when `stream` is another."""
-        self._requests(requests, cache)
-        n = lib().mt_attention_kv8_workspace(self._ctx, cache.ref, requests, rows, hq, window)
-        keep, wp, wn = self._workspace(n, workspace)
-        self._kv8(lib().mt_attention_kv8(self._ctx, self._stream(stream), ptr(q), ldq, requests, rows, hq, ptr(positions),
-                                         ptr(counts), window, cache.ref, ptr(out), ldo, wp, wn), "mt_attention_kv8")
+        self._enough(cache, requests)
+        need = lib().mt_attention_kv8_workspace(self._ctx, cache.ref, requests, rows, hq, window)
+        keep, wp, wn = self._workspace(need, workspace) if need else (None, None, 0)
+        st = lib().mt_attention_kv8(self._ctx, self._device_stream() if stream is None else stream, q.data_ptr(), ldq,
+                                    requests, rows, hq, positions.data_ptr(),
+                                    None if counts is None else counts.data_ptr(), window, cache.ref, out.data_ptr(), ldo,
+                                    wp, wn)
+        if st != MT_OK:
+            self._check(st, "mt_attention_kv8")
 
     def attention_prefix_kv8(self, q, ldq, requests, rows, hq, positions, counts, prefix, prefix_len, cache, out, ldo,
                              workspace=None, stream=None):
-        """mt_attention_prefix_kv8: attention over a prefix all requests share and each one's own cache."""
-        self._requests(requests, cache)
-        n = lib().mt_attention_prefix_kv8_workspace(self._ctx, prefix_len, cache.ref, requests, rows, hq)
-        keep, wp, wn = self._workspace(n, workspace)
-        self._kv8(lib().mt_attention_prefix_kv8(self._ctx, self._stream(stream), ptr(q), ldq, requests, rows, hq,
-                                                ptr(positions), ptr(counts), prefix.ref if prefix is not None else None,
-                                                prefix_len, cache.ref, ptr(out), ldo, wp, wn), "mt_attention_prefix_kv8")
+        """mt_attention_prefix_kv8: attention over a prefix all requests share and each one's own cache.
+        The workspace as in attention_kv8."""
+        self._enough(cache, requests)
+        need = lib().mt_attention_prefix_kv8_workspace(self._ctx, prefix_len, cache.ref, requests, rows, hq)
+        keep, wp, wn = self._workspace(need, workspace) if need else (None, None, 0)
+        st = lib().mt_attention_prefix_kv8(self._ctx, self._device_stream() if stream is None else stream, q.data_ptr(),
+                                           ldq, requests, rows, hq, positions.data_ptr(),
+                                           None if counts is None else counts.data_ptr(),
+                                           None if prefix is None else prefix.ref, prefix_len, cache.ref, out.data_ptr(),
+                                           ldo, wp, wn)
+        if st != MT_OK:
+            self._check(st, "mt_attention_prefix_kv8")
 
     def dit_attention(self, qkv, ld, batch, seq, heads, inv_freq, out, ldo):
         self.call("dit_attention", qkv, ld, batch, seq, heads, inv_freq, out, ldo)

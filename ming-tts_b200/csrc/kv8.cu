@@ -12,7 +12,7 @@ namespace mt {
 mt_status kv8_check_cache(mt_ctx* ctx, const char* what, const mt_kv8_cache* c, int requests) {
     MT_REQUIRE(ctx, c && c->k && c->v && c->k_scale && c->v_scale, MT_ERR_ARG, "%s: null cache", what);
     MT_REQUIRE(ctx, c->kind == MT_KV_INT8 || c->kind == MT_KV_E4M3, MT_ERR_ARG, "%s: cache kind %d", what, c->kind);
-    MT_REQUIRE(ctx, c->kv_heads > 0 && c->capacity > 0 && c->base >= 0 &&
+    MT_REQUIRE(ctx, c->kv_heads > 0 && c->capacity > 0 && c->capacity <= (1 << 30) && c->base >= 0 &&
                         (long long)c->kv_heads * c->capacity <= c->request_stride,
                MT_ERR_SHAPE, "%s: cache of %d heads x %d positions from %d on, request stride %lld", what, c->kv_heads,
                c->capacity, c->base, c->request_stride);

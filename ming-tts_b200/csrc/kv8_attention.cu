@@ -1,8 +1,27 @@
 // kv8_attention.cu -- attention over 8-bit key/value caches, alone (mt_attention_kv8) and behind a
 // prefix that all requests share (mt_attention_prefix_kv8).
 //
-// out = sum_j w_j v_j / sum_j w_j with w_j = exp(q.k_j / 8 - m), one pass with a running maximum m.
+// out = sum_j w_j v_j / sum_j w_j with w_j = exp(q.k_j / 8 - m), one pass with a running reference m.
 // The reference's attention_cache (Shaders.swift:500-591) reads fp32 caches of one request.
+//
+// Arithmetic. A code (an integer up to 128, or an e4m3 value) is exact in fp16. A query value and a
+// weight (times its value row's scale) are carried as two fp16 planes, x = hi + lo with
+// |x - hi - lo| <= 2^-22 |x|, so two 16-bit matrix products with fp32 sums give both contractions at
+// fp32 accuracy: q.k_j = scale_j (hi.c_j + lo.c_j), and the same for the values. Queries are scaled by
+// a power of two per row, weights by one per row that follows the largest weight times scale, so that
+// the planes use fp16's range whatever the units.
+//
+// A warp owns a tile of query rows (8, 16 or 32: rows x grouped heads, flattened) and walks its keys 16
+// at a time. Its lanes load codes straight from the cache into the layout of the matrix instruction
+// (m16n8k16): which key or dimension a fragment's row or column stands for is free as long as both
+// operands agree, so a lane takes 16 consecutive bytes of one key row for the scores, 8 consecutive
+// bytes of four key rows for the values, and the conversion to fp16 pairs the bytes of two keys. No
+// shared memory and no barrier until the partial results of the block's warps are joined.
+//   Lane (g, t) = (lane / 4, lane % 4), in a tile of keys 0..15:
+//     scores, column g of half j is key 4 (g / 2) + 2 j + g % 2, so lane t's scores are keys 4t .. 4t+3
+//     values, contraction index 2t, 2t+1, 2t+8, 2t+9 is key 4t .. 4t+3; column g of block i is dimension
+//     8 g + i, so lane t's outputs are dimensions 16 t .. 16 t + 15.
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -17,105 +36,608 @@ struct Kv8View {
     const float *ks, *vs;
     long long request_stride;
     int capacity, kind;
+    bool quads;  // four scales from a slot that is a multiple of four are one aligned 16-byte load
 };
 
-struct Kv8AttnArgs {
-    const float* q; int ldq;
-    float* out; int ldo;
+// One pass over one set of keys: a request's own cache (units: request x kv head, causal), or the
+// shared prefix (units: kv heads, the rows of all requests in one tile space, every key seen).
+struct PassArgs {
+    const float* q; int ldq; bool qvec;
+    float* out; int ldo; bool ovec;  // written when the pass has one part
     Kv8Rows rows;
-    int requests, hq, hkv, window;
-    Kv8View own, prefix;
-    int prefix_len;
+    int requests, hq, hkv, group, window;
+    Kv8View c;
+    int prefix_len;                  // > 0: the prefix pass
+    int units, row_blocks, splits;   // grid: units x row_blocks x splits
+    int key_warps;                   // warps of a block that share a row tile and interleave its keys
+    float *part_o, *part_ml;         // parts: [row * hq + head][parts][64] and [..][parts][2] (reference, sum)
+    int parts, part0;                // parts of the whole call, and this pass's first
 };
 
-constexpr int AT_WARPS = 4;
-
-__device__ __forceinline__ float2 decode2(uint32_t c, int kind) {
-    if (kind == MT_KV_INT8) return make_float2((float)(int8_t)c, (float)(int8_t)(c >> 8));
-    return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c & 0xFFFFu), __NV_E4M3)));
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// One warp a (row, query head): 32 keys at a time, a lane a key for the scores and a lane two
-// dimensions for the values.
-__global__ void __launch_bounds__(AT_WARPS * 32) kv8_attention_kernel(Kv8AttnArgs a) {
-    __shared__ float qs[AT_WARPS][64];
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Codes of bytes 0, 1 and of bytes 2, 3 as two fp16 pairs. Integers: the byte with its sign bit
+// flipped, put under fp16's 1024 (0x64), is 1024 + 128 + code.
+template <int KIND>
+__device__ __forceinline__ void to_half(uint32_t w, uint32_t& h01, uint32_t& h23) {
+    if (KIND == MT_KV_INT8) {
+        w ^= 0x80808080u;
+        const uint32_t bias = 0x64806480u;  // 1152, 1152
+        uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(h01) : "r"(a), "r"(bias));
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(h23) : "r"(b), "r"(bias));
+    } else {
+        asm("{.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;}"
+            : "=r"(h01), "=r"(h23)
+            : "r"(w));
+    }
+}
+
+// Two values as fp16 pairs hi + lo.
+__device__ __forceinline__ void split_half2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// 2^(target - e) for x in [2^e, 2^(e+1)), within 2^+-126.
+__device__ __forceinline__ float power_to(float x, int target) {
+    const int e = (int)(__float_as_uint(x) >> 23) - 127;
+    return __uint_as_float((uint32_t)(min(126, max(-126, target - e)) + 127) << 23);
+}
+
+// Codes and scales of a warp's 16 keys, in a lane's share.
+struct KeyTile {
+    uint4 k[2];
+    uint2 v[4];
+    float ks[4], vs[4];
+};
+
+// Where a warp's keys are. Index u counts positions from a multiple of the capacity, so that slot(u) is
+// u or u - capacity; the rows of the tile see [lo, hi] at most, and all of [in_lo, in_hi].
+struct KeyRange {
+    size_t row;  // first slot of the request and head
+    int lo, hi, in_lo, in_hi, capacity;
+};
+
+__device__ __forceinline__ void load_keys(KeyTile& x, const Kv8View& c, const KeyRange& r, int u0, int g, int t) {
+    const bool whole = u0 >= r.lo && u0 + 15 <= r.hi && (u0 + 16 <= r.capacity || u0 >= r.capacity);
+    const int s0 = u0 >= r.capacity ? u0 - r.capacity : u0;
+    if (whole && c.quads) {
+        const size_t at = r.row + s0;
+        const uint8_t* kp = c.k + (at + 4 * (g >> 1) + (g & 1)) * 64 + 16 * t;
+        x.k[0] = *reinterpret_cast<const uint4*>(kp);
+        x.k[1] = *reinterpret_cast<const uint4*>(kp + 128);
+        const uint8_t* vp = c.v + (at + 4 * t) * 64 + 8 * g;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x.v[i] = *reinterpret_cast<const uint2*>(vp + 64 * i);
+        const float4 a = *reinterpret_cast<const float4*>(c.ks + at + 4 * t);
+        const float4 b = *reinterpret_cast<const float4*>(c.vs + at + 4 * t);
+        x.ks[0] = a.x; x.ks[1] = a.y; x.ks[2] = a.z; x.ks[3] = a.w;
+        x.vs[0] = b.x; x.vs[1] = b.y; x.vs[2] = b.z; x.vs[3] = b.w;
+        return;
+    }
+    // Keys outside the range stand in as the nearest inside it: the slot of a key that no row sees may
+    // hold codes that are NaN, which a weight of zero would not silence.
+    auto slot = [&](int key) {
+        const int u = min(max(u0 + key, r.lo), r.hi);
+        return r.row + (u >= r.capacity ? u - r.capacity : u);
+    };
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+        x.k[j] = *reinterpret_cast<const uint4*>(c.k + slot(4 * (g >> 1) + 2 * j + (g & 1)) * 64 + 16 * t);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const size_t at = slot(4 * t + i);
+        x.v[i] = *reinterpret_cast<const uint2*>(c.v + at * 64 + 8 * g);
+        x.ks[i] = c.ks[at];
+        x.vs[i] = c.vs[at];
+    }
+}
+
+// NT 0: 8 rows, whose hi planes are rows 0-7 and lo planes rows 8-15 of one 16-row operand (a decode
+// step's group of heads); NT 1, 2: 16 or 32 rows, the planes as two operands.
+template <int NT>
+struct Rows {
+    static constexpr int SETS = NT == 0 ? 1 : NT;         // 16-row operands
+    static constexpr int PLANES = NT == 0 ? 1 : 2;        // of each
+    static constexpr int LANE = NT == 0 ? 1 : 2 * NT;     // rows of which a lane holds a part
+    static constexpr int COUNT = NT == 0 ? 8 : 16 * NT;   // rows of a warp
+    static constexpr int WARPS = NT == 0 ? 8 : 4;
+    static constexpr int BLOCKS = NT == 2 ? 2 : NT == 1 ? 3 : 2;  // resident blocks the registers allow
+};
+
+constexpr float REF_NONE = -1.7e38f;  // reference of a row that has seen no key
+constexpr int FOLD = 8;               // key tiles summed in the matrix unit's accumulators at a time
+
+template <int KIND, int NT>
+__global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pass_kernel(const PassArgs a) {
+    using R = Rows<NT>;
+    constexpr int LR = R::LANE;
+    extern __shared__ float smem[];  // [warp][row][64] sums, [warp][row][2] reference and sum, [row] owner
     pdl_wait();
     pdl_launch();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * AT_WARPS + warp;
-    const int head = (int)(unit % a.hq);
-    const long long row = unit / a.hq;
-    if (row >= (long long)a.requests * a.rows.rows) return;
-    const int request = (int)(row / a.rows.rows), i = (int)(row % a.rows.rows);
-    const Kv8Span s = kv8_span(a.rows, request);
-    if (i >= s.count) return;
-    const float* q = a.q + (size_t)row * a.ldq + (size_t)head * 64;
-    qs[warp][lane] = q[lane] * 0.125f;
-    qs[warp][lane + 32] = q[lane + 32] * 0.125f;
-    __syncwarp();
-    const int p = s.pos + i;
-    int first = max(a.rows.base, s.pos + s.count - a.own.capacity);
-    if (a.window > 0) first = max(first, p - a.window + 1);
-    const int kh = head / (a.hq / a.hkv);
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int part = 0; part < 2; part++) {
-        const Kv8View& c = part == 0 ? a.prefix : a.own;
-        const int from = part == 0 ? 0 : first, to = part == 0 ? a.prefix_len : p + 1;
-        const size_t base = (part == 0 ? 0 : (size_t)request * c.request_stride) + (size_t)kh * c.capacity;
-        for (int j0 = from; j0 < to; j0 += 32) {
-            const int j = j0 + lane;
-            const bool on = j < to;
-            const int slot = on ? (part == 0 ? j : (j - a.rows.base) % c.capacity) : 0;
-            float score = -INFINITY, vs = 0.f;
-            if (on) {
-                const uint4* kr = reinterpret_cast<const uint4*>(c.k + (base + slot) * 64);
-                float d = 0.f;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    // Blocks with the most keys (the last rows) first.
+    const int split = blockIdx.x % a.splits;
+    const int unit = (blockIdx.x / a.splits) % a.units;
+    const int row_block = a.row_blocks - 1 - blockIdx.x / (a.splits * a.units);
+    const int phase = warp % a.key_warps;
+    const int tile = row_block * (R::WARPS / a.key_warps) + warp / a.key_warps;
+    const bool shared_keys = a.prefix_len > 0;
+    const int request = shared_keys ? 0 : unit / a.hkv, kvh = shared_keys ? unit : unit % a.hkv;
+
+    // This lane's rows: where they are, and what they see.
+    int row_of[LR];  // row * hq + head, or -1
+    int hi[LR], lo[LR];
+    KeyRange r;
+    r.capacity = a.c.capacity;
+    r.row = (size_t)request * a.c.request_stride + (size_t)kvh * a.c.capacity;
+    int u_shift = 0;
+    bool any_row;
+    if (shared_keys) {
+        r.lo = 0; r.hi = a.prefix_len - 1; r.in_lo = 0; r.in_hi = r.hi;
+        const long long total = (long long)a.requests * a.rows.rows * a.group;
+        any_row = (long long)tile * R::COUNT < total;
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const uint4 w = kr[t];
-                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        for (int i = 0; i < LR; i++) {
+            const long long e = (long long)tile * R::COUNT + 8 * i + g;
+            const int row = (int)(e / a.group), req = row / a.rows.rows;
+            const bool live = e < total && row - req * a.rows.rows < kv8_span(a.rows, req).count;
+            row_of[i] = live ? row * a.hq + kvh * a.group + (int)(e - (long long)row * a.group) : -1;
+            lo[i] = 0; hi[i] = r.hi;
+        }
+    } else {
+        const Kv8Span s = kv8_span(a.rows, request);
+        const int i0 = tile * R::COUNT / a.group, i1 = min((tile * R::COUNT + R::COUNT - 1) / a.group, s.count - 1);
+        any_row = i0 < s.count;
+        const int first = max(a.rows.base, s.pos + s.count - a.c.capacity);
+        const int from = a.window > 0 ? max(first, s.pos + i0 - a.window + 1) : first;
+        const int rel = any_row ? from - a.rows.base : 0;
+        u_shift = any_row ? from - rel % a.c.capacity : 0;  // position of u = 0
+        r.lo = from - u_shift; r.hi = s.pos + i1 - u_shift;
+        r.in_lo = (a.window > 0 ? max(first, s.pos + i1 - a.window + 1) : first) - u_shift;
+        r.in_hi = s.pos + i0 - u_shift;
 #pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        const float2 f = decode2(ws[u], c.kind), g = decode2(ws[u] >> 16, c.kind);
-                        const float* qq = &qs[warp][t * 16 + u * 4];
-                        d = fmaf(f.x, qq[0], fmaf(f.y, qq[1], fmaf(g.x, qq[2], fmaf(g.y, qq[3], d))));
+        for (int i = 0; i < LR; i++) {
+            const int e = tile * R::COUNT + 8 * i + g, at = e / a.group;
+            const bool live = at < s.count;
+            row_of[i] = live ? (request * a.rows.rows + at) * a.hq + kvh * a.group + (e - at * a.group) : -1;
+            hi[i] = live ? s.pos + at - u_shift : r.hi;
+            lo[i] = live && a.window > 0 ? max(first, s.pos + at - a.window + 1) - u_shift : r.lo;
+        }
+    }
+
+    // Sums of the rows in shared memory, in units of 2^at_ref: the matrix unit drops the bits of a sum
+    // that its 24 do not hold (it does not round them), so a long chain of products drifts towards
+    // zero: 256 key tiles in one chain were 4e-6 off. Every FOLD tiles the registers are added here.
+    float* const acc = smem + (warp * R::COUNT + g) * 64 + 16 * t;  // row i of the lane: + 512 i
+    float ref[LR], at_ref[LR], sum[LR], unit_w[LR];
+    float o[R::SETS][8][4];
+#pragma unroll
+    for (int i = 0; i < LR; i++) { ref[i] = REF_NONE; at_ref[i] = REF_NONE; sum[i] = 0.f; unit_w[i] = 0x1p126f; }
+    auto clear = [&]() {
+#pragma unroll
+        for (int n = 0; n < R::SETS; n++)
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[n][i][j] = 0.f;
+    };
+    clear();
+    auto fold = [&](bool first) {
+#pragma unroll
+        for (int i = 0; i < LR; i++) {
+            const float f = first ? 0.f : ex2(at_ref[i] - ref[i]), n = 1.f / unit_w[i];
+            at_ref[i] = ref[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float4* at = reinterpret_cast<float4*>(acc + 512 * i) + j;
+                float4 y = first ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
+                auto add = [&](float& x, int d) {
+                    const int m = 4 * (j & 1) + d, col = j >> 1;
+                    const float v = NT == 0 ? o[0][m][col] + o[0][m][2 + col] : o[i / 2][m][2 * (i & 1) + col];
+                    x = first ? v * n : fmaf(v, n, x * f);
+                };
+                add(y.x, 0); add(y.y, 1); add(y.z, 2); add(y.w, 3);
+                *at = y;
+            }
+        }
+    };
+
+    const int t0 = r.lo >> 4, tiles = any_row ? (r.hi >> 4) - t0 + 1 : 0;
+    const int per = (tiles + a.splits - 1) / a.splits;
+    const int end = min(tiles, (split + 1) * per);
+    int at = split * per + phase;
+    bool folded = false;
+    if (at < end) {
+        KeyTile next;
+        load_keys(next, a.c, r, (t0 + at) * 16, g, t);
+        // Queries: 16 dimensions of each of the lane's rows, as fp16 planes of a power-of-two multiple.
+        uint32_t qa[R::SETS][R::PLANES][4][4];
+        float q_scale[LR];
+#pragma unroll
+        for (int i = 0; i < LR; i++) {
+            float x[16];
+            float top = 0.f;
+            if (row_of[i] >= 0) {
+                const int row = row_of[i] / a.hq, head = row_of[i] - row * a.hq;
+                const float* src = a.q + (size_t)row * a.ldq + (size_t)head * 64 + 16 * t;
+                if (a.qvec) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float4 f = reinterpret_cast<const float4*>(src)[j];
+                        x[4 * j] = f.x; x[4 * j + 1] = f.y; x[4 * j + 2] = f.z; x[4 * j + 3] = f.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; j++) x[j] = src[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; j++) x[j] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; j++) top = fmaxf(top, fabsf(x[j]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float up = power_to(top, 13);
+            q_scale[i] = 0.125f * 1.4426950408889634f / up;  // scores in powers of two
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                uint32_t h0, l0, h1, l1;
+                split_half2(x[4 * s] * up, x[4 * s + 1] * up, h0, l0);
+                split_half2(x[4 * s + 2] * up, x[4 * s + 3] * up, h1, l1);
+                if (NT == 0) {
+                    qa[0][0][s][0] = h0; qa[0][0][s][1] = l0; qa[0][0][s][2] = h1; qa[0][0][s][3] = l1;
+                } else {
+                    qa[i / 2][0][s][i & 1] = h0; qa[i / 2][0][s][2 + (i & 1)] = h1;
+                    qa[i / 2][R::PLANES - 1][s][i & 1] = l0; qa[i / 2][R::PLANES - 1][s][2 + (i & 1)] = l1;
+                }
+            }
+        }
+
+        int chain = 0;
+        for (; at < end; at += a.key_warps) {
+            if (++chain == FOLD + 1) {
+                fold(!folded);
+                clear();
+                folded = true;
+                chain = 1;
+            }
+            const KeyTile x = next;
+            const int u0 = (t0 + at) * 16;
+            if (at + a.key_warps < end) load_keys(next, a.c, r, u0 + 16 * a.key_warps, g, t);
+
+            // Scores (before scaling): 4 keys of each of the lane's rows.
+            float s[LR][4];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const uint32_t kw[4] = {x.k[j].x, x.k[j].y, x.k[j].z, x.k[j].w};
+                float c[R::SETS][4];
+#pragma unroll
+                for (int n = 0; n < R::SETS; n++) { c[n][0] = 0.f; c[n][1] = 0.f; c[n][2] = 0.f; c[n][3] = 0.f; }
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    uint32_t b0, b1;
+                    to_half<KIND>(kw[w], b0, b1);
+#pragma unroll
+                    for (int n = 0; n < R::SETS; n++)
+#pragma unroll
+                        for (int p = 0; p < R::PLANES; p++) mma16816(c[n], qa[n][p][w], b0, b1);
+                }
+                if (NT == 0) {
+                    s[0][2 * j] = c[0][0] + c[0][2];
+                    s[0][2 * j + 1] = c[0][1] + c[0][3];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < LR; i++) {
+                        s[i][2 * j] = c[i / 2][2 * (i & 1)];
+                        s[i][2 * j + 1] = c[i / 2][2 * (i & 1) + 1];
                     }
                 }
-                score = d * c.ks[base + slot];
-                vs = c.vs[base + slot];
             }
-            float top = warp_max(score);
-            const float mn = fmaxf(m, top);
-            const float fix = mn == -INFINITY ? 1.f : expf(m - mn);
-            const float w = on ? expf(score - (mn == -INFINITY ? 0.f : mn)) : 0.f;
-            m = mn;
-            l = l * fix + w;
-            o0 *= fix;
-            o1 *= fix;
-            const float wv = on ? w * vs : 0.f;
-            const int n = min(32, to - j0);
-            for (int t = 0; t < n; t++) {
-                const float x = __shfl_sync(0xffffffffu, wv, t);
-                const int sl = __shfl_sync(0xffffffffu, slot, t);
-                const float2 f = decode2(reinterpret_cast<const uint16_t*>(c.v + (base + sl) * 64)[lane], c.kind);
-                o0 = fmaf(x, f.x, o0);
-                o1 = fmaf(x, f.y, o1);
+            const bool whole = u0 >= r.in_lo && u0 + 15 <= r.in_hi;
+            // Weights exp2(score - reference). The reference moves only when a score is 8 above it (a
+            // factor of 256, which fp32 sums and the planes' range have room for).
+            float w[LR][4];
+            bool raise = false;
+#pragma unroll
+            for (int i = 0; i < LR; i++) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    s[i][k] *= x.ks[k];
+                    w[i][k] = fmaf(s[i][k], q_scale[i], -ref[i]);
+                    if (!whole) {
+                        const int u = u0 + 4 * t + k;
+                        if (u < lo[i] || u > hi[i]) w[i][k] = -INFINITY;
+                    }
+                }
+                raise |= fmaxf(fmaxf(w[i][0], w[i][1]), fmaxf(w[i][2], w[i][3])) > 8.f;
+            }
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int i = 0; i < LR; i++) {
+                    float top = REF_NONE;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (w[i][k] != -INFINITY) top = fmaxf(top, s[i][k] * q_scale[i]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    if (top - ref[i] > 8.f) {
+                        const float before = ref[i];
+                        ref[i] = top;
+                        const float f = ex2(before - ref[i]);
+                        sum[i] *= f;
+#pragma unroll
+                        for (int n = 0; n < 8; n++) {
+                            if (NT == 0) {
+                                o[0][n][0] *= f; o[0][n][1] *= f; o[0][n][2] *= f; o[0][n][3] *= f;
+                            } else {
+                                o[i / 2][n][2 * (i & 1)] *= f;
+                                o[i / 2][n][2 * (i & 1) + 1] *= f;
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (w[i][k] != -INFINITY) w[i][k] = fmaf(s[i][k], q_scale[i], -ref[i]);
+                    }
+                }
+            }
+            // Weights times the value rows' scales, as planes.
+            uint32_t pa[R::SETS][R::PLANES][4];
+            bool over = false;
+#pragma unroll
+            for (int i = 0; i < LR; i++) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float p = ex2(w[i][k]);
+                    sum[i] += p;
+                    // a scale of a key that this row does not see may be NaN
+                    w[i][k] = whole || w[i][k] != -INFINITY ? p * x.vs[k] : 0.f;
+                }
+                over |= fmaxf(fmaxf(fabsf(w[i][0]), fabsf(w[i][1])), fmaxf(fabsf(w[i][2]), fabsf(w[i][3]))) * unit_w[i] > 16384.f;
+            }
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int i = 0; i < LR; i++) {
+                    float top = fmaxf(fmaxf(fabsf(w[i][0]), fabsf(w[i][1])), fmaxf(fabsf(w[i][2]), fabsf(w[i][3])));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    if (top * unit_w[i] > 16384.f) {
+                        const float now = power_to(top, 10), f = now * (1.f / unit_w[i]);
+                        unit_w[i] = now;
+#pragma unroll
+                        for (int n = 0; n < 8; n++) {
+                            if (NT == 0) {
+                                o[0][n][0] *= f; o[0][n][1] *= f; o[0][n][2] *= f; o[0][n][3] *= f;
+                            } else {
+                                o[i / 2][n][2 * (i & 1)] *= f;
+                                o[i / 2][n][2 * (i & 1) + 1] *= f;
+                            }
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < LR; i++) {
+                uint32_t h0, l0, h1, l1;
+                split_half2(w[i][0] * unit_w[i], w[i][1] * unit_w[i], h0, l0);
+                split_half2(w[i][2] * unit_w[i], w[i][3] * unit_w[i], h1, l1);
+                if (NT == 0) {
+                    pa[0][0][0] = h0; pa[0][0][1] = l0; pa[0][0][2] = h1; pa[0][0][3] = l1;
+                } else {
+                    pa[i / 2][0][i & 1] = h0; pa[i / 2][0][2 + (i & 1)] = h1;
+                    pa[i / 2][R::PLANES - 1][i & 1] = l0; pa[i / 2][R::PLANES - 1][2 + (i & 1)] = l1;
+                }
+            }
+            // Values: dimensions 8g .. 8g+7 of keys 4t .. 4t+3, the two keys of a pair side by side.
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint32_t v0 = h ? x.v[0].y : x.v[0].x, v1 = h ? x.v[1].y : x.v[1].x;
+                const uint32_t v2 = h ? x.v[2].y : x.v[2].x, v3 = h ? x.v[3].y : x.v[3].x;
+                uint32_t b0[4], b1[4];
+                to_half<KIND>(__byte_perm(v0, v1, 0x5140), b0[0], b0[1]);
+                to_half<KIND>(__byte_perm(v0, v1, 0x7362), b0[2], b0[3]);
+                to_half<KIND>(__byte_perm(v2, v3, 0x5140), b1[0], b1[1]);
+                to_half<KIND>(__byte_perm(v2, v3, 0x7362), b1[2], b1[3]);
+#pragma unroll
+                for (int d = 0; d < 4; d++)
+#pragma unroll
+                    for (int n = 0; n < R::SETS; n++)
+#pragma unroll
+                        for (int p = 0; p < R::PLANES; p++) mma16816(o[n][4 * h + d], pa[n][p], b0[d], b1[d]);
             }
         }
     }
-    l = warp_sum(l);
-    float* out = a.out + (size_t)row * a.ldo + (size_t)head * 64;
-    out[2 * lane] = o0 / l;
-    out[2 * lane + 1] = o1 / l;
+
+    // Join the key_warps warps of each row tile.
+    fold(!folded);
+    float2* sml = reinterpret_cast<float2*>(smem + R::WARPS * R::COUNT * 64);
+#pragma unroll
+    for (int i = 0; i < LR; i++) {
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+        if (t == 0) sml[warp * R::COUNT + 8 * i + g] = make_float2(ref[i], sum[i]);
+    }
+    int* owner = reinterpret_cast<int*>(sml + R::WARPS * R::COUNT);
+    if (phase == 0 && t == 0) {
+#pragma unroll
+        for (int i = 0; i < LR; i++) owner[(warp / a.key_warps) * R::COUNT + 8 * i + g] = row_of[i];
+    }
+    __syncthreads();
+    const int rows_here = R::WARPS / a.key_warps * R::COUNT;
+    for (int e = threadIdx.x; e < rows_here * 16; e += R::WARPS * 32) {
+        const int row = e >> 4, d4 = e & 15, target = owner[row];
+        if (target < 0) continue;
+        const int base = (row / R::COUNT) * a.key_warps * R::COUNT + row % R::COUNT;
+        float top = REF_NONE, l = 0.f;
+        for (int k = 0; k < a.key_warps; k++) top = fmaxf(top, sml[base + k * R::COUNT].x);
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < a.key_warps; k++) {
+            const float2 ml = sml[base + k * R::COUNT];
+            const float f = ex2(ml.x - top);
+            const float4 v = reinterpret_cast<const float4*>(smem + (base + k * R::COUNT) * 64)[d4];
+            l += f * ml.y;
+            y.x += f * v.x; y.y += f * v.y; y.z += f * v.z; y.w += f * v.w;
+        }
+        if (a.parts == 1) {
+            const int qrow = target / a.hq, head = target - qrow * a.hq;
+            float* dst = a.out + (size_t)qrow * a.ldo + (size_t)head * 64 + 4 * d4;
+            const float n = 1.f / l;
+            y.x *= n; y.y *= n; y.z *= n; y.w *= n;
+            if (a.ovec) {
+                *reinterpret_cast<float4*>(dst) = y;
+            } else {
+                dst[0] = y.x; dst[1] = y.y; dst[2] = y.z; dst[3] = y.w;
+            }
+        } else {
+            const size_t part = (size_t)target * a.parts + a.part0 + split;
+            if (d4 == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(top, l);
+            reinterpret_cast<float4*>(a.part_o + part * 64)[d4] = y;
+        }
+    }
+}
+
+// Joins the parts of each (row, head): out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. A warp a
+// (row, head): 16 lanes cover the 64 dimensions, the two halves take alternate parts.
+struct JoinArgs {
+    Kv8Rows rows;
+    int total, hq, parts;  // total: requests * rows
+    const float *part_o, *part_ml;
+    float* out; int ldo; bool ovec;
+};
+constexpr int JOIN_THREADS = 128;
+
+__global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const JoinArgs a) {
+    pdl_wait();
+    pdl_launch();
+    const int lane = threadIdx.x & 31, half = lane >> 4, d4 = lane & 15;
+    const long long e = (long long)blockIdx.x * (JOIN_THREADS / 32) + (threadIdx.x >> 5);
+    if (e >= (long long)a.total * a.hq) return;
+    const int row = (int)(e / a.hq), head = (int)(e - (long long)row * a.hq);
+    const int request = row / a.rows.rows;
+    if (row - request * a.rows.rows >= kv8_span(a.rows, request).count) return;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + e * a.parts;
+    const float4* po = reinterpret_cast<const float4*>(a.part_o + e * a.parts * 64);
+    float top = REF_NONE;
+    for (int s = lane; s < a.parts; s += 32) top = fmaxf(top, ml[s].x);
+    top = warp_max(top);
+    float l = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = half; s < a.parts; s += 2) {
+        const float2 p = ml[s];
+        const float4 v = po[(size_t)s * 16 + d4];
+        const float f = ex2(p.x - top);
+        l += f * p.y;
+        y.x += f * v.x; y.y += f * v.y; y.z += f * v.z; y.w += f * v.w;
+    }
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
+    y.x += __shfl_xor_sync(0xffffffffu, y.x, 16);
+    y.y += __shfl_xor_sync(0xffffffffu, y.y, 16);
+    y.z += __shfl_xor_sync(0xffffffffu, y.z, 16);
+    y.w += __shfl_xor_sync(0xffffffffu, y.w, 16);
+    if (half) return;
+    const float n = 1.f / l;
+    float* dst = a.out + (size_t)row * a.ldo + (size_t)head * 64 + 4 * d4;
+    y.x *= n; y.y *= n; y.z *= n; y.w *= n;
+    if (a.ovec) {
+        *reinterpret_cast<float4*>(dst) = y;
+    } else {
+        dst[0] = y.x; dst[1] = y.y; dst[2] = y.z; dst[3] = y.w;
+    }
 }
 
 Kv8View view(const mt_kv8_cache* c) {
-    return Kv8View{c->k, c->v, c->k_scale, c->v_scale, c->request_stride, c->capacity, c->kind};
+    const bool quads = (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 15u) == 0 && c->capacity % 4 == 0 &&
+                       c->request_stride % 4 == 0;
+    return Kv8View{c->k, c->v, c->k_scale, c->v_scale, c->request_stride, c->capacity, c->kind, quads};
 }
 
-size_t workspace_bytes(const mt_ctx*, int prefix_len, const mt_kv8_cache* cache, int requests, int rows, int hq, int window) {
-    (void)prefix_len; (void)cache; (void)requests; (void)rows; (void)hq; (void)window;
-    return 0;
+// How a pass is laid out over the GPU.
+struct PassPlan {
+    int nt, units, row_blocks, key_warps, splits;
+};
+
+// `units` row spaces of `qrows` (row, head) rows each over at most `keys` keys.
+PassPlan plan_pass(int sm_count, long long units, long long qrows, int keys) {
+    PassPlan p{};
+    if (units < 1) return p;
+    const int key_tiles = (keys + 15) / 16 + 1;
+    const long long warps_fit = 16ll * sm_count;
+    // Tiles of 8 rows while that leaves every SM room: a warp's chain of dependent steps is shortest.
+    // 16 or 32 rows convert each key's codes once for more rows.
+    const long long tiles8 = (qrows + 7) / 8;
+    p.nt = qrows <= 8 || units * tiles8 * ((key_tiles + 3) / 4) <= warps_fit ? 0 : qrows <= 16 ? 1 : 2;
+    const int count = p.nt == 0 ? 8 : 16 * p.nt, warps = p.nt == 0 ? 8 : 4;
+    const long long row_tiles = (qrows + count - 1) / count;
+    // Warps of a block: over the keys of one row tile, unless that makes more blocks than are resident
+    // at once or there are not that many key tiles; then over row tiles.
+    auto blocks_at = [&](int kw) { return units * ((row_tiles + warps / kw - 1) / (warps / kw)); };
+    p.key_warps = warps;
+    while (p.key_warps > 1 && (blocks_at(p.key_warps) > 2ll * sm_count || p.key_warps > key_tiles)) p.key_warps /= 2;
+    p.units = (int)units;
+    const long long blocks = blocks_at(p.key_warps);
+    p.row_blocks = (int)(blocks / units);
+    // Split the keys over blocks while there are SMs without one and every warp keeps 4 tiles.
+    long long s = (2ll * sm_count + blocks - 1) / blocks;
+    const long long most = key_tiles / (4 * p.key_warps);
+    if (s > most) s = most;
+    p.splits = s < 1 ? 1 : (int)s;
+    return p;
+}
+
+struct Plan {
+    PassPlan own, prefix;
+    int parts;
+    size_t o_bytes, bytes;
+};
+
+Plan make_plan(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int requests, int rows, int hq, int window) {
+    Plan p{};
+    const int hkv = cache->kv_heads > 0 ? cache->kv_heads : 1;
+    const long long group = hq / hkv;
+    const long long seen = window > 0 ? (long long)window + rows - 1 : cache->capacity;
+    p.own = plan_pass(ctx->sm_count, (long long)requests * hkv, rows * group, (int)(seen < cache->capacity ? seen : cache->capacity));
+    p.parts = p.own.splits;
+    if (prefix_len > 0) {
+        p.prefix = plan_pass(ctx->sm_count, hkv, (long long)requests * rows * group, prefix_len);
+        p.parts += p.prefix.splits;
+    }
+    if (p.parts > 1) {
+        const size_t n = (size_t)requests * rows * hq * p.parts;
+        p.o_bytes = n * 64 * sizeof(float);
+        p.bytes = p.o_bytes + n * 2 * sizeof(float);
+    }
+    return p;
+}
+
+template <int KIND, int NT>
+void launch_pass_as(const PassArgs& a, cudaStream_t s) {
+    using R = Rows<NT>;
+    const size_t smem = (size_t)R::WARPS * R::COUNT * (64 + 2 + 1) * sizeof(float);
+    launch_k(kv8_pass_kernel<KIND, NT>, dim3((unsigned)(a.units * a.row_blocks * a.splits)), R::WARPS * 32, smem, s, a);
+}
+
+void launch_pass(const PassArgs& a, int nt, cudaStream_t s) {
+    if (a.c.kind == MT_KV_INT8)
+        nt == 0 ? launch_pass_as<MT_KV_INT8, 0>(a, s) : nt == 1 ? launch_pass_as<MT_KV_INT8, 1>(a, s) : launch_pass_as<MT_KV_INT8, 2>(a, s);
+    else
+        nt == 0 ? launch_pass_as<MT_KV_E4M3, 0>(a, s) : nt == 1 ? launch_pass_as<MT_KV_E4M3, 1>(a, s) : launch_pass_as<MT_KV_E4M3, 2>(a, s);
 }
 
 mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q, int ldq, int requests, int rows, int hq,
@@ -132,22 +654,38 @@ mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q,
     MT_REQUIRE(ctx, rows <= cache->capacity && (window == 0 || (long long)window + rows - 1 <= cache->capacity), MT_ERR_CAPACITY,
                "%s: %d rows, window %d, capacity %d", what, rows, window, cache->capacity);
     MT_REQUIRE(ctx, ctx, MT_ERR_ARG, "%s: null context", what);
-    const size_t need = workspace_bytes(ctx, prefix_len, cache, requests, rows, hq, window);
-    MT_REQUIRE(ctx, need == 0 || (workspace && have >= need && ((uintptr_t)workspace & 15u) == 0), MT_ERR_CAPACITY,
-               "%s: workspace of %zu bytes (16-byte aligned), needs %zu", what, workspace ? have : (size_t)0, need);
+    MT_REQUIRE(ctx, (long long)requests * rows * hq <= 0x7FFFFFFFll, MT_ERR_SHAPE, "%s: %d requests of %d rows of %d heads",
+               what, requests, rows, hq);
     if (requests == 0 || rows == 0) return MT_OK;
+    const Plan plan = make_plan(ctx, prefix_len, cache, requests, rows, hq, window);
+    MT_REQUIRE(ctx, plan.bytes == 0 || (workspace && have >= plan.bytes && ((uintptr_t)workspace & 15u) == 0), MT_ERR_CAPACITY,
+               "%s: workspace of %zu bytes (16-byte aligned), needs %zu", what, workspace ? have : (size_t)0, plan.bytes);
     DeviceGuard guard(ctx->device);
     MT_REQUIRE(ctx, guard.err == cudaSuccess, MT_ERR_CUDA, "%s: %s", what, cudaGetErrorString(guard.err));
-    Kv8AttnArgs a{};
-    a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo;
+    cudaStream_t s = as_stream(stream);
+    PassArgs a{};
+    a.q = q; a.ldq = ldq; a.qvec = ((uintptr_t)q & 15u) == 0 && ldq % 4 == 0;
+    a.out = out; a.ldo = ldo; a.ovec = ((uintptr_t)out & 15u) == 0 && ldo % 4 == 0;
     a.rows = Kv8Rows{positions, counts, rows, cache->base};
-    a.requests = requests; a.hq = hq; a.hkv = hkv; a.window = window;
-    a.own = view(cache);
-    a.prefix = prefix_len > 0 ? view(prefix) : a.own;
-    a.prefix_len = prefix_len;
-    const long long blocks = ((long long)requests * rows * hq + AT_WARPS - 1) / AT_WARPS;
-    MT_REQUIRE(ctx, blocks <= 0x7FFFFFFFll, MT_ERR_SHAPE, "%s: %d requests of %d rows", what, requests, rows);
-    launch_k(kv8_attention_kernel, (unsigned)blocks, AT_WARPS * 32, 0, as_stream(stream), a);
+    a.requests = requests; a.hq = hq; a.hkv = hkv; a.group = hq / hkv;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + plan.o_bytes / sizeof(float);
+    a.parts = plan.parts;
+    auto run = [&](const PassPlan& p) {
+        a.units = p.units; a.row_blocks = p.row_blocks; a.splits = p.splits; a.key_warps = p.key_warps;
+        launch_pass(a, p.nt, s);
+    };
+    if (prefix_len > 0) {
+        a.c = view(prefix); a.prefix_len = prefix_len; a.part0 = 0;
+        run(plan.prefix);
+    }
+    a.c = view(cache); a.prefix_len = 0; a.part0 = plan.parts - plan.own.splits; a.window = window;
+    run(plan.own);
+    if (plan.parts > 1) {
+        JoinArgs j{a.rows, requests * rows, hq, plan.parts, a.part_o, a.part_ml, out, ldo, a.ovec};
+        const long long n = (long long)requests * rows * hq;
+        launch_k(kv8_join_kernel, dim3((unsigned)((n + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32))), JOIN_THREADS, 0, s, j);
+    }
     return check_launch(ctx, what);
 }
 
@@ -160,12 +698,13 @@ using namespace mt;
 extern "C" {
 
 size_t mt_attention_kv8_workspace(const mt_ctx* ctx, const mt_kv8_cache* cache, int requests, int rows, int hq, int window) {
-    return ctx && cache ? workspace_bytes(ctx, 0, cache, requests, rows, hq, window) : 0;
+    return ctx && cache && requests > 0 && rows > 0 && hq > 0 ? make_plan(ctx, 0, cache, requests, rows, hq, window).bytes : 0;
 }
 
 size_t mt_attention_prefix_kv8_workspace(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int requests,
                                          int rows, int hq) {
-    return ctx && cache ? workspace_bytes(ctx, prefix_len, cache, requests, rows, hq, 0) : 0;
+    return ctx && cache && requests > 0 && rows > 0 && hq > 0 ? make_plan(ctx, prefix_len, cache, requests, rows, hq, 0).bytes
+                                                             : 0;
 }
 
 mt_status mt_attention_kv8(mt_ctx* ctx, void* stream, const float* q, int ldq, int requests, int rows, int hq,
