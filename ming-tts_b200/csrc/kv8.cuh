@@ -1,6 +1,8 @@
 // kv8.cuh -- shared by the 8-bit key/value cache kernels (kv8.cu, kv8_attention.cu).
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 
 namespace mt {
@@ -26,6 +28,151 @@ __device__ __forceinline__ Kv8Span kv8_span(const Kv8Rows& a, int request) {
 // Host-side checks that the entry points share. `what` names the entry point.
 mt_status kv8_check_cache(mt_ctx* ctx, const char* what, const mt_kv8_cache* c, int requests);
 mt_status kv8_check_rows(mt_ctx* ctx, const char* what, int requests, int rows, int hq, int hkv);
+
+// ------------------------------------------------------------------------------------------------
+// Attention (kv8_attention.cu, kv8_attention_wide.cu)
+// ------------------------------------------------------------------------------------------------
+struct Kv8View {
+    const uint8_t *k, *v;
+    const float *ks, *vs;
+    long long request_stride;
+    int capacity, kind;
+    bool quads;  // four scales from a slot that is a multiple of four are one aligned 16-byte load
+};
+
+// One pass over one set of keys: a request's own cache (units: request x kv head, causal), or the
+// shared prefix (units: kv heads, the rows of all requests in one tile space, every key seen).
+struct PassArgs {
+    const float* q; int ldq; bool qvec;
+    float* out; int ldo; bool ovec;  // written when the pass has one part
+    Kv8Rows rows;
+    int requests, hq, hkv, group, window;
+    Kv8View c;
+    int prefix_len;                  // > 0: the prefix pass
+    int units, row_blocks, splits;   // grid: units x row_blocks x splits
+    int key_warps;                   // warps of a block that share a row tile and interleave its keys
+    float *part_o, *part_ml;         // parts: [row * hq + head][parts][64] and [..][parts][2] (reference, sum)
+    int parts, part0;                // parts of the whole call, and this pass's first
+};
+
+// Where the keys of a tile of rows are. Index u counts positions from a multiple of the capacity, so that
+// slot(u) is u or u - capacity; the tile's rows see [lo, hi] at most, and all of [in_lo, in_hi].
+struct KeyRange {
+    size_t row;  // first slot of the request and head
+    int lo, hi, in_lo, in_hi, capacity;
+    __device__ __forceinline__ size_t slot(int u) const {  // u outside the range: the nearest inside it
+        u = min(max(u, lo), hi);
+        return row + (u >= capacity ? u - capacity : u);
+    }
+    // Slots u0 .. u0 + n - 1 are in the range and side by side.
+    __device__ __forceinline__ bool whole(int u0, int n) const {
+        return u0 >= lo && u0 + n - 1 <= hi && (u0 + n <= capacity || u0 >= capacity);
+    }
+};
+
+// A unit's row space: rows x group (row, head) pairs, row-major. In a pass over a request's own cache a
+// unit is (request, kv head), in a prefix pass a kv head and the rows are those of all requests.
+struct UnitRows {
+    const PassArgs& a;
+    int request, kvh;
+    Kv8Span span;  // of the request
+    int first;     // oldest position that the cache holds
+    int shift;     // position of u = 0
+    KeyRange keys;
+
+    __device__ __forceinline__ UnitRows(const PassArgs& args, int unit) : a(args) {
+        const bool prefix = a.prefix_len > 0;
+        request = prefix ? 0 : unit / a.hkv;
+        kvh = prefix ? unit : unit % a.hkv;
+        keys.capacity = a.c.capacity;
+        keys.row = (size_t)request * a.c.request_stride + (size_t)kvh * a.c.capacity;
+        shift = 0;
+        if (!prefix) {
+            span = kv8_span(a.rows, request);
+            first = max(a.rows.base, span.pos + span.count - a.c.capacity);
+        }
+    }
+    // (row, head) pairs of the unit.
+    __device__ __forceinline__ int size() const {
+        return (a.prefix_len > 0 ? a.requests * a.rows.rows : span.count) * a.group;
+    }
+    // Sets `keys` for the pairs e0 .. e0 + n - 1 (e0 < size()).
+    __device__ __forceinline__ void tile(int e0, int n) {
+        if (a.prefix_len > 0) {
+            keys.lo = 0; keys.hi = a.prefix_len - 1; keys.in_lo = 0; keys.in_hi = keys.hi;
+            return;
+        }
+        const int i0 = e0 / a.group, i1 = min((e0 + n - 1) / a.group, span.count - 1);
+        const int from = oldest(i0);
+        shift = from - (from - a.rows.base) % a.c.capacity;
+        keys.lo = from - shift;
+        keys.hi = span.pos + i1 - shift;
+        keys.in_lo = oldest(i1) - shift;
+        keys.in_hi = span.pos + i0 - shift;
+    }
+    // Oldest position that row i sees.
+    __device__ __forceinline__ int oldest(int i) const {
+        return a.window > 0 ? max(first, span.pos + i - a.window + 1) : first;
+    }
+    // Pair e: row * hq + head, or -1 where it is not one of a request's own, and the keys [lo, hi] it sees.
+    __device__ __forceinline__ int pair(int e, int& lo, int& hi) const {
+        lo = keys.lo; hi = keys.hi;
+        if (e >= size()) return -1;
+        const int i = e / a.group, head = kvh * a.group + e - i * a.group;
+        if (a.prefix_len > 0) {
+            const int req = i / a.rows.rows;
+            return i - req * a.rows.rows < kv8_span(a.rows, req).count ? i * a.hq + head : -1;
+        }
+        hi = span.pos + i - shift;
+        lo = oldest(i) - shift;
+        return (request * a.rows.rows + i) * a.hq + head;
+    }
+};
+
+constexpr float KV8_REF_NONE = -1.7e38f;  // reference of a row that has seen no key
+
+// The kernel for many rows (kv8_attention_wide.cu): blocks of KV8_WIDE_ROWS rows, `splits` parts of
+// `chunk` tiles of KV8_WIDE_KEYS keys each.
+constexpr int KV8_WIDE_ROWS = 256, KV8_WIDE_KEYS = 64;
+void launch_kv8_wide(const PassArgs& a, int chunk, unsigned int* status, cudaStream_t s);
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Codes of bytes 0, 1 and of bytes 2, 3 as two fp16 pairs. Integers: the byte with its sign bit
+// flipped, put under fp16's 1024 (0x64), is 1024 + 128 + code.
+template <int KIND>
+__device__ __forceinline__ void to_half(uint32_t w, uint32_t& h01, uint32_t& h23) {
+    if (KIND == MT_KV_INT8) {
+        w ^= 0x80808080u;
+        const uint32_t bias = 0x64806480u;  // 1152, 1152
+        uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(h01) : "r"(a), "r"(bias));
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(h23) : "r"(b), "r"(bias));
+    } else {
+        asm("{.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;}"
+            : "=r"(h01), "=r"(h23)
+            : "r"(w));
+    }
+}
+
+// Two values as fp16 pairs hi + lo.
+__device__ __forceinline__ void split_half2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// 2^(target - e) for x in [2^e, 2^(e+1)), within 2^+-126.
+__device__ __forceinline__ float power_to(float x, int target) {
+    const int e = (int)(__float_as_uint(x) >> 23) - 127;
+    return __uint_as_float((uint32_t)(min(126, max(-126, target - e)) + 127) << 23);
+}
 
 // Makes a device current for a call and puts the caller's back.
 struct DeviceGuard {

@@ -21,8 +21,6 @@
 //     scores, column g of half j is key 4 (g / 2) + 2 j + g % 2, so lane t's scores are keys 4t .. 4t+3
 //     values, contraction index 2t, 2t+1, 2t+8, 2t+9 is key 4t .. 4t+3; column g of block i is dimension
 //     8 g + i, so lane t's outputs are dimensions 16 t .. 16 t + 15.
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <math.h>
 
 #include "kv8.cuh"
@@ -31,72 +29,11 @@ namespace mt {
 
 namespace {
 
-struct Kv8View {
-    const uint8_t *k, *v;
-    const float *ks, *vs;
-    long long request_stride;
-    int capacity, kind;
-    bool quads;  // four scales from a slot that is a multiple of four are one aligned 16-byte load
-};
-
-// One pass over one set of keys: a request's own cache (units: request x kv head, causal), or the
-// shared prefix (units: kv heads, the rows of all requests in one tile space, every key seen).
-struct PassArgs {
-    const float* q; int ldq; bool qvec;
-    float* out; int ldo; bool ovec;  // written when the pass has one part
-    Kv8Rows rows;
-    int requests, hq, hkv, group, window;
-    Kv8View c;
-    int prefix_len;                  // > 0: the prefix pass
-    int units, row_blocks, splits;   // grid: units x row_blocks x splits
-    int key_warps;                   // warps of a block that share a row tile and interleave its keys
-    float *part_o, *part_ml;         // parts: [row * hq + head][parts][64] and [..][parts][2] (reference, sum)
-    int parts, part0;                // parts of the whole call, and this pass's first
-};
-
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Codes of bytes 0, 1 and of bytes 2, 3 as two fp16 pairs. Integers: the byte with its sign bit
-// flipped, put under fp16's 1024 (0x64), is 1024 + 128 + code.
-template <int KIND>
-__device__ __forceinline__ void to_half(uint32_t w, uint32_t& h01, uint32_t& h23) {
-    if (KIND == MT_KV_INT8) {
-        w ^= 0x80808080u;
-        const uint32_t bias = 0x64806480u;  // 1152, 1152
-        uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(h01) : "r"(a), "r"(bias));
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(h23) : "r"(b), "r"(bias));
-    } else {
-        asm("{.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;}"
-            : "=r"(h01), "=r"(h23)
-            : "r"(w));
-    }
-}
-
-// Two values as fp16 pairs hi + lo.
-__device__ __forceinline__ void split_half2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x0, x1);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-}
-
-// 2^(target - e) for x in [2^e, 2^(e+1)), within 2^+-126.
-__device__ __forceinline__ float power_to(float x, int target) {
-    const int e = (int)(__float_as_uint(x) >> 23) - 127;
-    return __uint_as_float((uint32_t)(min(126, max(-126, target - e)) + 127) << 23);
 }
 
 // Codes and scales of a warp's 16 keys, in a lane's share.
@@ -106,17 +43,9 @@ struct KeyTile {
     float ks[4], vs[4];
 };
 
-// Where a warp's keys are. Index u counts positions from a multiple of the capacity, so that slot(u) is
-// u or u - capacity; the rows of the tile see [lo, hi] at most, and all of [in_lo, in_hi].
-struct KeyRange {
-    size_t row;  // first slot of the request and head
-    int lo, hi, in_lo, in_hi, capacity;
-};
-
 __device__ __forceinline__ void load_keys(KeyTile& x, const Kv8View& c, const KeyRange& r, int u0, int g, int t) {
-    const bool whole = u0 >= r.lo && u0 + 15 <= r.hi && (u0 + 16 <= r.capacity || u0 >= r.capacity);
     const int s0 = u0 >= r.capacity ? u0 - r.capacity : u0;
-    if (whole && c.quads) {
+    if (c.quads && r.whole(u0, 16)) {
         const size_t at = r.row + s0;
         const uint8_t* kp = c.k + (at + 4 * (g >> 1) + (g & 1)) * 64 + 16 * t;
         x.k[0] = *reinterpret_cast<const uint4*>(kp);
@@ -132,16 +61,12 @@ __device__ __forceinline__ void load_keys(KeyTile& x, const Kv8View& c, const Ke
     }
     // Keys outside the range stand in as the nearest inside it: the slot of a key that no row sees may
     // hold codes that are NaN, which a weight of zero would not silence.
-    auto slot = [&](int key) {
-        const int u = min(max(u0 + key, r.lo), r.hi);
-        return r.row + (u >= r.capacity ? u - r.capacity : u);
-    };
 #pragma unroll
     for (int j = 0; j < 2; j++)
-        x.k[j] = *reinterpret_cast<const uint4*>(c.k + slot(4 * (g >> 1) + 2 * j + (g & 1)) * 64 + 16 * t);
+        x.k[j] = *reinterpret_cast<const uint4*>(c.k + r.slot(u0 + 4 * (g >> 1) + 2 * j + (g & 1)) * 64 + 16 * t);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const size_t at = slot(4 * t + i);
+        const size_t at = r.slot(u0 + 4 * t + i);
         x.v[i] = *reinterpret_cast<const uint2*>(c.v + at * 64 + 8 * g);
         x.ks[i] = c.ks[at];
         x.vs[i] = c.vs[at];
@@ -160,7 +85,6 @@ struct Rows {
     static constexpr int BLOCKS = NT == 2 ? 2 : NT == 1 ? 3 : 2;  // resident blocks the registers allow
 };
 
-constexpr float REF_NONE = -1.7e38f;  // reference of a row that has seen no key
 constexpr int FOLD = 8;               // key tiles summed in the matrix unit's accumulators at a time
 
 template <int KIND, int NT>
@@ -177,49 +101,14 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
     const int row_block = a.row_blocks - 1 - blockIdx.x / (a.splits * a.units);
     const int phase = warp % a.key_warps;
     const int tile = row_block * (R::WARPS / a.key_warps) + warp / a.key_warps;
-    const bool shared_keys = a.prefix_len > 0;
-    const int request = shared_keys ? 0 : unit / a.hkv, kvh = shared_keys ? unit : unit % a.hkv;
-
-    // This lane's rows: where they are, and what they see.
-    int row_of[LR];  // row * hq + head, or -1
-    int hi[LR], lo[LR];
-    KeyRange r;
-    r.capacity = a.c.capacity;
-    r.row = (size_t)request * a.c.request_stride + (size_t)kvh * a.c.capacity;
-    int u_shift = 0;
-    bool any_row;
-    if (shared_keys) {
-        r.lo = 0; r.hi = a.prefix_len - 1; r.in_lo = 0; r.in_hi = r.hi;
-        const long long total = (long long)a.requests * a.rows.rows * a.group;
-        any_row = (long long)tile * R::COUNT < total;
+    UnitRows rows(a, unit);
+    const int e0 = tile * R::COUNT;
+    const bool any_row = e0 < rows.size();
+    if (any_row) rows.tile(e0, R::COUNT);
+    const KeyRange& r = rows.keys;
+    int row_of[LR], hi[LR], lo[LR];
 #pragma unroll
-        for (int i = 0; i < LR; i++) {
-            const long long e = (long long)tile * R::COUNT + 8 * i + g;
-            const int row = (int)(e / a.group), req = row / a.rows.rows;
-            const bool live = e < total && row - req * a.rows.rows < kv8_span(a.rows, req).count;
-            row_of[i] = live ? row * a.hq + kvh * a.group + (int)(e - (long long)row * a.group) : -1;
-            lo[i] = 0; hi[i] = r.hi;
-        }
-    } else {
-        const Kv8Span s = kv8_span(a.rows, request);
-        const int i0 = tile * R::COUNT / a.group, i1 = min((tile * R::COUNT + R::COUNT - 1) / a.group, s.count - 1);
-        any_row = i0 < s.count;
-        const int first = max(a.rows.base, s.pos + s.count - a.c.capacity);
-        const int from = a.window > 0 ? max(first, s.pos + i0 - a.window + 1) : first;
-        const int rel = any_row ? from - a.rows.base : 0;
-        u_shift = any_row ? from - rel % a.c.capacity : 0;  // position of u = 0
-        r.lo = from - u_shift; r.hi = s.pos + i1 - u_shift;
-        r.in_lo = (a.window > 0 ? max(first, s.pos + i1 - a.window + 1) : first) - u_shift;
-        r.in_hi = s.pos + i0 - u_shift;
-#pragma unroll
-        for (int i = 0; i < LR; i++) {
-            const int e = tile * R::COUNT + 8 * i + g, at = e / a.group;
-            const bool live = at < s.count;
-            row_of[i] = live ? (request * a.rows.rows + at) * a.hq + kvh * a.group + (e - at * a.group) : -1;
-            hi[i] = live ? s.pos + at - u_shift : r.hi;
-            lo[i] = live && a.window > 0 ? max(first, s.pos + at - a.window + 1) - u_shift : r.lo;
-        }
-    }
+    for (int i = 0; i < LR; i++) row_of[i] = any_row ? rows.pair(e0 + 8 * i + g, lo[i], hi[i]) : -1;
 
     // Sums of the rows in shared memory, in units of 2^at_ref: the matrix unit drops the bits of a sum
     // that its 24 do not hold (it does not round them), so a long chain of products drifts towards
@@ -228,7 +117,7 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
     float ref[LR], at_ref[LR], sum[LR], unit_w[LR];
     float o[R::SETS][8][4];
 #pragma unroll
-    for (int i = 0; i < LR; i++) { ref[i] = REF_NONE; at_ref[i] = REF_NONE; sum[i] = 0.f; unit_w[i] = 0x1p126f; }
+    for (int i = 0; i < LR; i++) { ref[i] = KV8_REF_NONE; at_ref[i] = KV8_REF_NONE; sum[i] = 0.f; unit_w[i] = 0x1p126f; }
     auto clear = [&]() {
 #pragma unroll
         for (int n = 0; n < R::SETS; n++)
@@ -371,7 +260,7 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int i = 0; i < LR; i++) {
-                    float top = REF_NONE;
+                    float top = KV8_REF_NONE;
 #pragma unroll
                     for (int k = 0; k < 4; k++)
                         if (w[i][k] != -INFINITY) top = fmaxf(top, s[i][k] * q_scale[i]);
@@ -484,7 +373,7 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
         const int row = e >> 4, d4 = e & 15, target = owner[row];
         if (target < 0) continue;
         const int base = (row / R::COUNT) * a.key_warps * R::COUNT + row % R::COUNT;
-        float top = REF_NONE, l = 0.f;
+        float top = KV8_REF_NONE, l = 0.f;
         for (int k = 0; k < a.key_warps; k++) top = fmaxf(top, sml[base + k * R::COUNT].x);
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int k = 0; k < a.key_warps; k++) {
@@ -533,7 +422,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const JoinArgs a
     if (row - request * a.rows.rows >= kv8_span(a.rows, request).count) return;
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + e * a.parts;
     const float4* po = reinterpret_cast<const float4*>(a.part_o + e * a.parts * 64);
-    float top = REF_NONE;
+    float top = KV8_REF_NONE;
     for (int s = lane; s < a.parts; s += 32) top = fmaxf(top, ml[s].x);
     top = warp_max(top);
     float l = 0.f;
@@ -570,13 +459,29 @@ Kv8View view(const mt_kv8_cache* c) {
 
 // How a pass is laid out over the GPU.
 struct PassPlan {
-    int nt, units, row_blocks, key_warps, splits;
+    bool wide;
+    int nt, units, row_blocks, key_warps, splits, chunk;
 };
 
+constexpr int WIDE_FROM = 97;
+
 // `units` row spaces of `qrows` (row, head) rows each over at most `keys` keys.
-PassPlan plan_pass(int sm_count, long long units, long long qrows, int keys) {
+PassPlan plan_pass(int sm_count, long long units, long long qrows, int keys, bool causal) {
     PassPlan p{};
     if (units < 1) return p;
+    if (qrows >= WIDE_FROM) {
+        p.wide = true;
+        p.units = (int)units;
+        p.row_blocks = (int)((qrows + KV8_WIDE_ROWS - 1) / KV8_WIDE_ROWS);
+        const int tiles = (keys + 15 + KV8_WIDE_KEYS - 1) / KV8_WIDE_KEYS;
+        const long long blocks = units * p.row_blocks;
+        long long s = causal ? (2ll * sm_count + blocks - 1) / blocks : sm_count / blocks;
+        if (s > tiles / 4) s = tiles / 4;
+        if (s < 1) s = 1;
+        p.chunk = (int)((tiles + s - 1) / s);
+        p.splits = (tiles + p.chunk - 1) / p.chunk;
+        return p;
+    }
     const int key_tiles = (keys + 15) / 16 + 1;
     const long long warps_fit = 16ll * sm_count;
     // Tiles of 8 rows while that leaves every SM room: a warp's chain of dependent steps is shortest.
@@ -612,10 +517,10 @@ Plan make_plan(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int
     const int hkv = cache->kv_heads > 0 ? cache->kv_heads : 1;
     const long long group = hq / hkv;
     const long long seen = window > 0 ? (long long)window + rows - 1 : cache->capacity;
-    p.own = plan_pass(ctx->sm_count, (long long)requests * hkv, rows * group, (int)(seen < cache->capacity ? seen : cache->capacity));
+    p.own = plan_pass(ctx->sm_count, (long long)requests * hkv, rows * group, (int)(seen < cache->capacity ? seen : cache->capacity), true);
     p.parts = p.own.splits;
     if (prefix_len > 0) {
-        p.prefix = plan_pass(ctx->sm_count, hkv, (long long)requests * rows * group, prefix_len);
+        p.prefix = plan_pass(ctx->sm_count, hkv, (long long)requests * rows * group, prefix_len, false);
         p.parts += p.prefix.splits;
     }
     if (p.parts > 1) {
@@ -654,7 +559,7 @@ mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q,
     MT_REQUIRE(ctx, rows <= cache->capacity && (window == 0 || (long long)window + rows - 1 <= cache->capacity), MT_ERR_CAPACITY,
                "%s: %d rows, window %d, capacity %d", what, rows, window, cache->capacity);
     MT_REQUIRE(ctx, ctx, MT_ERR_ARG, "%s: null context", what);
-    MT_REQUIRE(ctx, (long long)requests * rows * hq <= 0x7FFFFFFFll, MT_ERR_SHAPE, "%s: %d requests of %d rows of %d heads",
+    MT_REQUIRE(ctx, (long long)requests * rows * hq <= 0x7FFFFF00ll, MT_ERR_SHAPE, "%s: %d requests of %d rows of %d heads",
                what, requests, rows, hq);
     if (requests == 0 || rows == 0) return MT_OK;
     const Plan plan = make_plan(ctx, prefix_len, cache, requests, rows, hq, window);
@@ -673,7 +578,8 @@ mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q,
     a.parts = plan.parts;
     auto run = [&](const PassPlan& p) {
         a.units = p.units; a.row_blocks = p.row_blocks; a.splits = p.splits; a.key_warps = p.key_warps;
-        launch_pass(a, p.nt, s);
+        if (p.wide) launch_kv8_wide(a, p.chunk, ctx->d_status, s);
+        else launch_pass(a, p.nt, s);
     };
     if (prefix_len > 0) {
         a.c = view(prefix); a.prefix_len = prefix_len; a.part0 = 0;
