@@ -4,21 +4,28 @@
 //
 // A block takes 256 (row, head) pairs of one kv head, as two tiles of 128, and walks its keys 64 at a
 // time. Its warps:
-//   0-3, 4-7  the rows of tile 0, 1: a thread a row. It reads the row's scores from TMEM, keeps the
-//             reference and the sum, writes the weights (times the value rows' scales) back as two fp16
-//             planes over the scores, and adds each key tile's output, read from TMEM, to 64 registers.
-//   8-11      convert codes to fp16 in shared memory (four stages), K and V alike: a key a 128-byte row
-//   12 (of the last four) issues the matrix instructions: S = Q K^T (128 x 64, both planes of Q from TMEM)
-//             and O = P V (128 x 64, both planes of P from TMEM; V is the [key][dimension] tile as it is)
-// The scores of the next key tile are in a second buffer while a tile's weights are made, so neither the
-// row threads nor the tensor cores wait for the other in turn.
+//   0-7, 8-15 the rows of tile 0, 1 (16 a warp): they read scores from TMEM, keep each row's reference and
+//             sum, write the weights (times the value rows' scales) back as two fp16 planes over the
+//             scores, and add each key tile's output, read from TMEM, to registers
+//   16-18     convert codes to fp16 in shared memory (four stages), K and V alike: a key a 128-byte row
+//   19        issues the matrix instructions: S = Q K^T (128 x 64, both planes of Q in shared memory) and
+//             O = P V (128 x 64, both planes of P in TMEM; V is the [key][dimension] tile as it is)
+// Scores and outputs have two buffers each: the scores of the next key tile are there while a tile's
+// weights are made, and an output is read two tiles later, so neither the row warps nor the tensor cores
+// wait for the other in turn. (With one output buffer and the query planes in TMEM, a tile had to wait
+// for the product of the one before: 2800 cycles a key tile even with no arithmetic on the weights.)
 //
 // Every key tile's O starts from zero: the accumulators drop the bits that 24 do not hold, and a chain of
 // 64 keys keeps that near fp32's own rounding; it also leaves nothing in TMEM to rescale.
 //
 // TMEM, 256 columns a row tile: 0-63 and 64-127 scores of even and odd key tiles (fp32), overwritten 16
-// columns at a time by 8 columns of hi and 8 of lo planes of the same 16 keys' weights; 128-191 the
-// query planes in the same way; 192-255 O.
+// columns at a time by 8 columns of hi and 8 of lo planes of the same 16 keys' weights; 128-191 and
+// 192-255 their outputs.
+//
+// A row warp has 16 of the 32 lanes that its place in the block lets it read, in the layout of 16 rows x 8
+// columns to 4 registers: lane (g, t) = (lane / 4, lane % 4) has columns 2t, 2t+1 of every 8, of rows g
+// and g + 8 (its slots 0 and 1). Four such warps a scheduler hide one another's latencies: with 8 warps of
+// 32 rows a key tile took 3400 cycles, of which 2200 were these warps' own.
 #include <math.h>
 
 #include "kv8.cuh"
@@ -27,77 +34,67 @@ namespace mt {
 
 namespace {
 
-constexpr int WD_ROW_WARPS = 8, WD_CONVERT_WARPS = 4;
-constexpr int WD_THREADS = 32 * (WD_ROW_WARPS + WD_CONVERT_WARPS + 4);
-// Registers of a thread, by warpgroup: the block starts with 512 x 128 = 65,536 of them, and
-// 256 x 168 + 128 x 96 + 128 x 80 is as many.
-constexpr int WD_ROW_REGS = 168, WD_CONVERT_REGS = 96, WD_ISSUE_REGS = 80;
+constexpr int WD_ROW_WARPS = 16, WD_CONVERT_WARPS = 3;
+constexpr int WD_THREADS = 32 * (WD_ROW_WARPS + WD_CONVERT_WARPS + 1);
+// Registers of a thread, by warpgroup: the block starts with 640 x 96 = 61,440 of them, and
+// 512 x 104 + 128 x 64 is as many.
+constexpr int WD_ROW_REGS = 104, WD_OTHER_REGS = 64;
 constexpr int WD_KEYS = KV8_WIDE_KEYS;
 constexpr int WD_STAGE = WD_KEYS * 128;  // bytes of a K or V tile in fp16
 constexpr int WD_STAGES = 4;
-constexpr int WD_PLANE = 128 * 128;      // bytes of a plane of a tile's queries
+constexpr int WD_PLANE = 128 * 128;      // bytes of a plane of a row tile's queries
 constexpr size_t WD_SMEM = 2 * WD_STAGES * WD_STAGE + 4 * WD_PLANE + 1024;
-constexpr uint32_t T_Q = 128, T_O = 192, T_TILE = 256;
-constexpr float WD_LIFT_MAX = 118.f;  // largest power that the weights are scaled by
+constexpr uint32_t T_O = 128, T_TILE = 256;
 constexpr int WD_LIFT_TO = 8;         // exponent that a row's largest scaled product is brought to ..
 constexpr float WD_PRODUCT_MAX = 32768.f;  // .. once one is above this (fp16 ends at 65504)
-constexpr float WD_WEIGHT_MAX = 0x1p100f;
+constexpr float WD_WEIGHT_MAX = 0x1p100f;  // what a sum of four weights may be in units of 2^off
 
-// 16 columns of this thread's lane: issue, and wait for every load issued so far (the registers are
-// operands of the wait, so nothing uses them before it).
-__device__ __forceinline__ void tmem_ld16(uint32_t at, float (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
-        : "r"(at));
+// 16 lanes x 16 columns of TMEM to and from 8 registers: fp32 (register 4 n + 2 slot + i is column 8 n + 2 t
+// + i of row g + 8 slot) or fp16 pairs (register 2 n + slot is column 4 n + t). A load's registers are
+// operands of the wait for it, so that nothing uses them before.
+#define TM_OUT8(r) "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
+__device__ __forceinline__ void tmem_ld_tile(uint32_t at, float (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : TM_OUT8(r) : "r"(at));
 }
-__device__ __forceinline__ void tmem_ld_wait(float (&r)[16]) {
+__device__ __forceinline__ void tmem_ld_planes(uint32_t at, float (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x128b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : TM_OUT8(r) : "r"(at));
+}
+__device__ __forceinline__ void tmem_ld_wait(float (&r)[8]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
-                   "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7])
                  :
                  : "memory");
 }
-
-__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&u)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
-        "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
-        "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
-        : "memory");
+__device__ __forceinline__ void tmem_st_planes(uint32_t at, const uint32_t (&u)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(u[0]), "r"(u[1]),
+                 "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                 : "memory");
 }
-
-// Calls f(c, columns 16 c ..) for c = 0 .. N-1 with the next columns' load in flight.
-template <int N, typename F>
-__device__ __forceinline__ void tmem_walk(uint32_t at, F&& f) {
-    float x[16], y[16];
-    tmem_ld16(at, x);
-#pragma unroll 1
-    for (int c = 0; c < N; c += 2) {
-        tmem_ld_wait(x);
-        tmem_ld16(at + 16 * c + 16, y);
-        f(c, x);
-        tmem_ld_wait(y);
-        if (c + 2 < N) tmem_ld16(at + 16 * c + 32, x);
-        f(c + 1, y);
-    }
-}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // TMEM stores of this thread done and ordered before what another thread does after a barrier.
 __device__ __forceinline__ void tmem_publish() {
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    tmem_st_wait();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_acquire() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// D[tmem] (+)= A[tmem] B[shared], fp16 operands, fp32 accumulator, M = 128.
+// D[tmem] (+)= A B, A in TMEM or in shared memory, B in shared memory; fp16 operands, fp32 accumulator,
+// M = 128.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
 // One thread of the warp, in a form that the compiler knows to be one: its matrix instructions then take
@@ -125,169 +122,180 @@ constexpr uint32_t IDESC_O = 1u << 4 | 1u << 16 | (64 / 8) << 17 | (128 / 16) <<
 
 struct Shared {
     alignas(16) float ks[WD_STAGES][WD_KEYS], vs[WD_STAGES][WD_KEYS];  // scales of the stages' keys (values': / unit)
-    float k_top[WD_STAGES][WD_CONVERT_WARPS];                          // largest norm of a key, by converting warp
     float first[WD_CONVERT_WARPS];
     float unit;                                                        // power of two near the first value scales
     uint64_t k_full[WD_STAGES], k_free[WD_STAGES], v_full[WD_STAGES], v_free[WD_STAGES];
-    uint64_t q_ready[2], s_ready[2][2], p_ready[2], o_ready[2];        // by row tile (and key tile parity)
+    uint64_t q_ready[2], s_ready[2][2], p_ready[2][2], o_ready[2][2];     // by row tile (and key tile parity)
     uint32_t tmem;
     int abort;
 };
 
-// Two fp32 values in one register pair and the instructions that work on both.
-struct F2 {
-    uint64_t v;
-};
-__device__ __forceinline__ F2 f2(float x, float y) {
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ void f2_parts(F2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
-__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-
-// A row's state. Weights are 2^(score - off), off = reference - lift: the reference is near a score that
-// was the row's largest, the lift brings the largest weight times value scale to 2^8, where the planes
-// have 22 bits for weights down to 2^-20 of it.
+// The state of a lane's two rows. Weights are 2^(score - off), off = reference - lift: the reference is
+// near a score that was the row's largest, the lift brings the largest weight times value scale to 2^8,
+// where the planes have 22 bits for weights down to 2^-20 of it. The sums and outputs are in units of
+// 2^off; a sum is the lane's own part of the row.
+constexpr float WD_UNSET = 1000.f;  // the lift of a row that has no unit yet (its off is 0)
 struct RowState {
-    float off, lift;
-    F2 sum;
-    float o[64];
-    float carry;  // by which the output not yet added is to be scaled
+    float off[2], lift[2], rs[2];  // rs: scores in powers of two are TMEM value x key scale x rs
+    int lo[2], hi[2];              // keys that the row sees
+    float sum[2];
+    float o[4][8];  // 16 columns each, as tmem_ld_tile
+    bool fresh;     // the unit of one of the warp's rows is not set yet
 
-    __device__ __forceinline__ void scale(float f) {
-        sum = f2_mul(sum, f2(f, f));
-        carry *= f;
+    __device__ __forceinline__ void scale(int slot, float f) {
+        sum[slot] *= f;
 #pragma unroll
-        for (int j = 0; j < 64; j++) o[j] *= f;
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                o[c][4 * n + 2 * slot] *= f;
+                o[c][4 * n + 2 * slot + 1] *= f;
+            }
     }
 };
 
-// The keys of a tile as a row's thread sees them.
+// The keys of a tile: the lane's first scales in shared memory (its columns are 8 n + 0, 1 from there),
+// and their index.
 struct TileKeys {
     const float *ks, *vs;
-    int u0, lo, hi;  // of the first key; the row sees [lo, hi]
+    int u;
 };
 
-template <bool MASK>
-__device__ __forceinline__ bool sees(const TileKeys& t, int key) {
-    return !MASK || (t.u0 + key >= t.lo && t.u0 + key <= t.hi);
-}
-
-// First tile, and where the weights could pass fp32's range: sets the reference to the row's largest
-// score of this tile, and the lift.
-__device__ __noinline__ float2 row_reference(uint32_t tm, const TileKeys& t, float rs, float off, float lift) {
-    float top = -INFINITY;
-    tmem_walk<4>(tm, [&](int c, const float(&s)[16]) {
-#pragma unroll
-        for (int j = 0; j < 16; j++)
-            if (sees<true>(t, 16 * c + j)) top = fmaxf(top, s[j] * t.ks[16 * c + j] * rs);
-    });
-    float ref = off + lift;
-    if (top > ref) ref = top;
-    float product = 0.f;
-    tmem_walk<4>(tm, [&](int c, const float(&s)[16]) {
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const float w = ex2(fmaf(s[j] * t.ks[16 * c + j], rs, -ref)) * fabsf(t.vs[16 * c + j]);
-            if (sees<true>(t, 16 * c + j)) product = fmaxf(product, w);
-        }
-    });
-    if (product * ex2(lift) > WD_PRODUCT_MAX)
-        lift = fminf((float)(WD_LIFT_TO + 127 - (int)(__float_as_uint(product) >> 23)), WD_LIFT_MAX);
-    return make_float2(ref, lift);
-}
-
-// Products of the tile so far (planes of `chunks` times 16 keys) scaled by f.
-__device__ __noinline__ void row_rescale(uint32_t tm, int chunks, float f) {
+// The planes of `chunks` times 16 keys, scaled by the rows' factors.
+__device__ __forceinline__ void row_rescale(uint32_t tm, int chunks, float f0, float f1) {
+    tmem_st_wait();
+#pragma unroll 1
     for (int c = 0; c < chunks; c++) {
-        float x[16];
-        uint32_t planes[16];
-        tmem_ld16(tm + 16 * c, x);
+        float x[8];
+        uint32_t planes[8];
+        tmem_ld_planes(tm + 16 * c, x);
         tmem_ld_wait(x);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
+        for (int j = 0; j < 4; j++) {
+            const float f = j & 1 ? f1 : f0;
             const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&x[j]));
-            const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&x[8 + j]));
-            split_half2((hi.x + lo.x) * f, (hi.y + lo.y) * f, planes[j], planes[8 + j]);
+            const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&x[4 + j]));
+            split_half2((hi.x + lo.x) * f, (hi.y + lo.y) * f, planes[j], planes[4 + j]);
         }
-        tmem_st16(tm + 16 * c, planes);
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tmem_st_planes(tm + 16 * c, planes);
+        tmem_st_wait();
     }
 }
 
-// Weights of the row in this tile: 2^(score - off), summed, and times the value scales into the planes.
+// Weights of 16 keys (s: scores, k and v: the keys' scales): 2^(score - off), their sums, and times the
+// value scales as planes. Returns the largest product.
 template <bool MASK>
-__device__ __forceinline__ void row_weights(uint32_t tm, const TileKeys& t, float rs, RowState& row) {
-    const F2 rs2 = f2(rs, rs), minus = f2(-1.f, -1.f);
-    tmem_walk<4>(tm, [&](int c, const float(&s)[16]) {
-        const F2 off2 = f2(-row.off, -row.off);
-        F2 w[8];
-        float top = 0.f;
+__device__ __forceinline__ float row_products(const TileKeys& t, const RowState& row, int c, const float (&s)[8], uint32_t (&planes)[8],
+                                              float (&add)[2]) {
+    const float2 k[2] = {*reinterpret_cast<const float2*>(t.ks + 16 * c), *reinterpret_cast<const float2*>(t.ks + 16 * c + 8)};
+    const float2 v[2] = {*reinterpret_cast<const float2*>(t.vs + 16 * c), *reinterpret_cast<const float2*>(t.vs + 16 * c + 8)};
+    float top = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-            const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(t.ks + 16 * c + j);
-            const ulonglong2 v4 = *reinterpret_cast<const ulonglong2*>(t.vs + 16 * c + j);
+    for (int i = 0; i < 2; i++) {
+        float sum[2];
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-                const F2 k{i ? k4.y : k4.x}, v{i ? v4.y : v4.x};
-                const bool on0 = sees<MASK>(t, 16 * c + j + i), on1 = sees<MASK>(t, 16 * c + j + i + 1);
-                float x0, x1;
-                f2_parts(f2_fma(f2_mul(f2(s[j + i], s[j + i + 1]), k), rs2, off2), x0, x1);
-                const F2 p = f2(on0 ? ex2(x0) : 0.f, on1 ? ex2(x1) : 0.f);
-                row.sum = f2_add(row.sum, p);
-                w[(j + i) / 2] = f2_mul(p, v);
-                f2_parts(w[(j + i) / 2], x0, x1);
-                if (MASK) {  // a scale of a key that this row does not see may be NaN
-                    x0 = on0 ? x0 : 0.f;
-                    x1 = on1 ? x1 : 0.f;
-                    w[(j + i) / 2] = f2(x0, x1);
+        for (int n = 0; n < 2; n++) {
+            const int u = t.u + 16 * c + 8 * n;
+            const bool on0 = !MASK || (u >= row.lo[i] && u <= row.hi[i]), on1 = !MASK || (u + 1 >= row.lo[i] && u + 1 <= row.hi[i]);
+            float p0 = ex2(fmaf(s[4 * n + 2 * i] * k[n].x, row.rs[i], -row.off[i]));
+            float p1 = ex2(fmaf(s[4 * n + 2 * i + 1] * k[n].y, row.rs[i], -row.off[i]));
+            if (MASK) {
+                p0 = on0 ? p0 : 0.f;
+                p1 = on1 ? p1 : 0.f;
+            }
+            sum[n] = p0 + p1;
+            p0 *= v[n].x;
+            p1 *= v[n].y;
+            if (MASK) {  // a scale of a key that this row does not see may be NaN
+                p0 = on0 ? p0 : 0.f;
+                p1 = on1 ? p1 : 0.f;
+            }
+            top = fmaxf(top, fmaxf(fabsf(p0), fabsf(p1)));
+            split_half2(p0, p1, planes[2 * n + i], planes[4 + 2 * n + i]);
+        }
+        add[i] = sum[0] + sum[1];
+    }
+    return top;
+}
+
+// A tile whose keys all rows see and whose products stay in range: nothing here changes a row's unit,
+// which is what keeps the loop at 9.4 instructions a weight (with that code in it, 12). Returns the first
+// 16 keys whose products do not stay in range, or 4.
+__device__ __forceinline__ int row_weights(uint32_t tm, const TileKeys& t, RowState& row) {
+    int c;
+#pragma unroll 1
+    for (c = 0; c < 4; c++) {
+        float s[8], add[2];
+        uint32_t planes[8];
+        tmem_ld_tile(tm + 16 * c, s);
+        tmem_ld_wait(s);
+        const float top = row_products<false>(t, row, c, s, planes, add);
+        if (__any_sync(0xffffffffu, !(top <= WD_PRODUCT_MAX && add[0] <= WD_WEIGHT_MAX && add[1] <= WD_WEIGHT_MAX))) break;
+        row.sum[0] += add[0];
+        row.sum[1] += add[1];
+        tmem_st_planes(tm + 16 * c, planes);
+    }
+    return c;
+}
+
+// The rest of a tile from `c` on, whatever its rows see: sets the units of rows that have none, and moves
+// them where products leave the range. `settle` adds the outputs that are still in TMEM, which are in the
+// units before.
+template <typename F>
+__device__ __forceinline__ void row_weights_slowly(uint32_t tm, const TileKeys& t, RowState& row, int c, F&& settle) {
+#pragma unroll 1
+    for (; c < 4; c++) {
+        float s[8], add[2];
+        uint32_t planes[8];
+        tmem_ld_tile(tm + 16 * c, s);
+        tmem_ld_wait(s);
+#pragma unroll 1
+        for (int tries = 0; tries < 2; tries++) {
+            const float top = row_products<true>(t, row, c, s, planes, add);
+            if (!row.fresh && !__any_sync(0xffffffffu, !(top <= WD_PRODUCT_MAX && add[0] <= WD_WEIGHT_MAX && add[1] <= WD_WEIGHT_MAX))) break;
+            settle(1);
+            float f[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float z[4], v[4], most = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int key = 16 * c + 8 * (j >> 1) + (j & 1);
+                    const bool on = t.u + key >= row.lo[i] && t.u + key <= row.hi[i];
+                    z[j] = on ? s[4 * (j >> 1) + 2 * i + (j & 1)] * t.ks[key] * row.rs[i] : -INFINITY;
+                    v[j] = on ? fabsf(t.vs[key]) : 0.f;
+                    most = fmaxf(most, z[j]);
                 }
-                top = fmaxf(top, fmaxf(fabsf(x0), fabsf(x1)));
-            }
-        }
-        if (__any_sync(0xffffffffu, top > WD_PRODUCT_MAX)) {  // rare: the row's scale moves within the tile
-            float f = 1.f;
-            if (top > WD_PRODUCT_MAX && top <= 3.4e38f) {
-                const int down = (int)(__float_as_uint(top) >> 23) - 127 - WD_LIFT_TO;
-                f = __uint_as_float((uint32_t)(127 - min(down, 126)) << 23);
-                row.off += (float)min(down, 126);
-                row.lift -= (float)min(down, 126);
-                row.scale(f);
-            }
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            row_rescale(tm, c, f);
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                auto product = [&](float from) {  // the row's largest in these keys, in units of 2^from
+                    float x = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; j++) w[j] = f2_mul(w[j], f2(f, f));
+                    for (int j = 0; j < 4; j++) x = fmaxf(x, ex2(z[j] - from) * v[j]);
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                    return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                };
+                float off = row.off[i], lift = row.lift[i];
+                const bool unset = lift == WD_UNSET;
+                const float now = product(off);
+                if (most > -INFINITY && (unset || most - off > 90.f || now > WD_PRODUCT_MAX)) off = unset ? most : fmaxf(off + lift, most);
+                const float then = product(off);
+                if (off != row.off[i] || now > WD_PRODUCT_MAX || (unset && most > -INFINITY)) {
+                    lift = then > 0.f ? fminf(80.f, fmaxf(-100.f, (float)(WD_LIFT_TO + 127 - (int)(__float_as_uint(then) >> 23)))) : 0.f;
+                    off -= lift;
+                }
+                f[i] = row.lift[i] == WD_UNSET ? 1.f : ex2(row.off[i] - off);
+                if (off != row.off[i]) row.scale(i, f[i]);
+                row.off[i] = off;
+                row.lift[i] = lift;
+            }
+            row.fresh = __any_sync(0xffffffffu, row.lift[0] == WD_UNSET || row.lift[1] == WD_UNSET);
+            row_rescale(tm, c, f[0], f[1]);
         }
-        uint32_t planes[16];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            float x0, x1;
-            f2_parts(w[j], x0, x1);
-            const __half2 hi = __floats2half2_rn(x0, x1);
-            const float2 back = __half22float2(hi);
-            f2_parts(f2_fma(f2(back.x, back.y), minus, w[j]), x0, x1);
-            const __half2 lo = __floats2half2_rn(x0, x1);
-            planes[j] = *reinterpret_cast<const uint32_t*>(&hi);
-            planes[8 + j] = *reinterpret_cast<const uint32_t*>(&lo);
-        }
-        tmem_st16(tm + 16 * c, planes);
-    });
+        row.sum[0] += add[0];
+        row.sum[1] += add[1];
+        tmem_st_planes(tm + 16 * c, planes);
+    }
 }
 
 template <int N>
@@ -316,7 +324,7 @@ __global__ void __launch_bounds__(WD_THREADS, 1) kv8_wide_kernel(const PassArgs 
     if (u_first > r.hi) {
         if (warp < WD_ROW_WARPS) {
             int lo, hi;
-            const int target = rows.pair(e0 + threadIdx.x, lo, hi);
+            const int target = threadIdx.x < KV8_WIDE_ROWS ? rows.pair(e0 + threadIdx.x, lo, hi) : -1;
             if (target >= 0)
                 reinterpret_cast<float2*>(a.part_ml)[(size_t)target * a.parts + a.part0 + split] = make_float2(KV8_REF_NONE, 0.f);
         }
@@ -333,11 +341,13 @@ __global__ void __launch_bounds__(WD_THREADS, 1) kv8_wide_kernel(const PassArgs 
             mbar_init(&sh.v_free[i], 1);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sh.q_ready[i], 4);
+            mbar_init(&sh.q_ready[i], WD_ROW_WARPS / 2);
             mbar_init(&sh.s_ready[i][0], 1);
             mbar_init(&sh.s_ready[i][1], 1);
-            mbar_init(&sh.p_ready[i], 4);
-            mbar_init(&sh.o_ready[i], 1);
+            mbar_init(&sh.p_ready[i][0], WD_ROW_WARPS / 2);
+            mbar_init(&sh.p_ready[i][1], WD_ROW_WARPS / 2);
+            mbar_init(&sh.o_ready[i][0], 1);
+            mbar_init(&sh.o_ready[i][1], 1);
         }
         sh.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -352,207 +362,183 @@ __global__ void __launch_bounds__(WD_THREADS, 1) kv8_wide_kernel(const PassArgs 
     const uint32_t tmem = sh.tmem;
     volatile int* const abort = &sh.abort;
 
+    if (warp >= WD_ROW_WARPS) fewer_registers<WD_OTHER_REGS>();
     if (warp < WD_ROW_WARPS) {
         more_registers<WD_ROW_REGS>();
-        const int tile = warp >> 2;
+        const int tile = warp >> 3;
         if (tile < row_tiles) {
-            int lo, hi;
-            const int target = rows.pair(e0 + threadIdx.x, lo, hi);
-            const uint32_t tm = tmem + tile * T_TILE + ((uint32_t)(warp & 3) << 21);  // lanes 32 (warp % 4) ..
-            float rs = 0.f;     // scores in powers of two: TMEM value x key scale x rs
-            float reach = 0.f;  // no score is above reach x the key's norm
+            const int first_row = 32 * (warp & 3) + 16 * ((warp >> 2) & 1);  // of the tile's 128: a lane of TMEM each
+            const uint32_t tm = tmem + tile * T_TILE + ((uint32_t)first_row << 16);
+            const int col = 2 * (lane & 3);
+            int target[2];
+            RowState row;
             {
-                // Queries: four lanes a row, 16 dimensions each, 8 rows a pass.
-                long long src = -1;
-                if (target >= 0) {
-                    const int row = target / a.hq;
-                    src = (long long)row * a.ldq + (long long)(target - row * a.hq) * 64;
+                // Queries: a lane has dimensions 8 n + 2 t, + 1 of its two rows.
+                int lo, hi;
+                const int mine = rows.pair(e0 + 128 * tile + first_row + (lane & 15), lo, hi), at = mine / a.hq;
+                long long from = (long long)at * a.ldq + (long long)(mine - at * a.hq) * 64;
+                if (mine < 0) from = -1;
+                const float* src[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int owner = 8 * i + (lane >> 2);
+                    target[i] = __shfl_sync(0xffffffffu, mine, owner);
+                    row.lo[i] = __shfl_sync(0xffffffffu, lo, owner);
+                    row.hi[i] = __shfl_sync(0xffffffffu, hi, owner);
+                    src[i] = a.q + __shfl_sync(0xffffffffu, from, owner) + col;
                 }
-                const int part = lane & 3;
-                float x[4][16];
+                float2 x[2][8];
+                if (a.qvec) {  // all of them issued before the first is used
 #pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    const long long from = __shfl_sync(0xffffffffu, src, 8 * n + (lane >> 2));
-                    const float* f = a.q + from + 16 * part;
-                    if (from < 0) {
+                    for (int j = 0; j < 16; j++)
+                        x[j >> 3][j & 7] = target[j >> 3] < 0 ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(src[j >> 3] + 8 * (j & 7));
+                } else {
 #pragma unroll
-                        for (int j = 0; j < 16; j++) x[n][j] = 0.f;
-                    } else if (a.qvec) {
+                    for (int j = 0; j < 16; j++)
+                        x[j >> 3][j & 7] = target[j >> 3] < 0 ? make_float2(0.f, 0.f) : make_float2(src[j >> 3][8 * (j & 7)], src[j >> 3][8 * (j & 7) + 1]);
+                }
+                float top[2] = {0.f, 0.f}, up[2];
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const float4 y = reinterpret_cast<const float4*>(f)[j];
-                            x[n][4 * j] = y.x; x[n][4 * j + 1] = y.y; x[n][4 * j + 2] = y.z; x[n][4 * j + 3] = y.w;
-                        }
-                    } else {
+                for (int i = 0; i < 2; i++) {
 #pragma unroll
-                        for (int j = 0; j < 16; j++) x[n][j] = f[j];
+                    for (int n = 0; n < 8; n++) top[i] = fmaxf(top[i], fmaxf(fabsf(x[i][n].x), fabsf(x[i][n].y)));
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+                    up[i] = power_to(top[i], 13);
+                    const int at = first_row + 8 * i + (lane >> 2);
+                    uint8_t* to = stages + 2 * WD_STAGES * WD_STAGE + 2 * tile * WD_PLANE + at * 128 + 2 * col;
+#pragma unroll
+                    for (int n = 0; n < 8; n++) {
+                        const float x0 = x[i][n].x * up[i], x1 = x[i][n].y * up[i];
+                        uint8_t* const here = to + ((n ^ (at & 7)) << 4);
+                        split_half2(x0, x1, *reinterpret_cast<uint32_t*>(here), *reinterpret_cast<uint32_t*>(here + WD_PLANE));
                     }
                 }
-                uint8_t* const planes = stages + 2 * WD_STAGES * WD_STAGE + 2 * tile * WD_PLANE;
 #pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    float top = 0.f, norm = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 16; j++) top = fmaxf(top, fabsf(x[n][j]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const float up = power_to(top, 13);
-                    const int row = 32 * (warp & 3) + 8 * n + (lane >> 2);
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint32_t qh[4], ql[4];
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const float y0 = x[n][8 * h + 2 * j] * up, y1 = x[n][8 * h + 2 * j + 1] * up;
-                            norm = fmaf(y0, y0, fmaf(y1, y1, norm));
-                            split_half2(y0, y1, qh[j], ql[j]);
-                        }
-                        const int at = row * 128 + (((2 * part + h) ^ (row & 7)) << 4);
-                        *reinterpret_cast<uint4*>(planes + at) = make_uint4(qh[0], qh[1], qh[2], qh[3]);
-                        *reinterpret_cast<uint4*>(planes + WD_PLANE + at) = make_uint4(ql[0], ql[1], ql[2], ql[3]);
-                    }
-                    norm += __shfl_xor_sync(0xffffffffu, norm, 1);
-                    norm += __shfl_xor_sync(0xffffffffu, norm, 2);
-                    const float r0 = __shfl_sync(0xffffffffu, 0.125f * 1.4426950408889634f / up, 4 * (lane & 7));
-                    const float n0 = __shfl_sync(0xffffffffu, norm, 4 * (lane & 7));
-                    if (lane >> 3 == n) {
-                        rs = r0;
-                        reach = 1.001f * sqrtf(n0) * r0;
-                    }
+                for (int i = 0; i < 2; i++) {
+                    // up is a power of two within 2^+-126: so is its reciprocal
+                    row.rs[i] = 0.125f * 1.4426950408889634f * __uint_as_float(0x7F000000u - __float_as_uint(up[i]));
+                    row.off[i] = 0.f;
+                    row.lift[i] = WD_UNSET;
+                    row.sum[i] = 0.f;
                 }
+                row.fresh = true;
             }
-            __syncwarp();
-            {
-                const int row = threadIdx.x & 127;
-                const uint8_t* const planes = stages + 2 * WD_STAGES * WD_STAGE + 2 * tile * WD_PLANE + row * 128;
-#pragma unroll
-                for (int c = 0; c < 4; c++) {  // 16 dimensions: 8 columns of hi and 8 of lo
-                    uint32_t x[16];
-#pragma unroll
-                    for (int h = 0; h < 4; h++) {
-                        const uint4 y = *reinterpret_cast<const uint4*>(planes + (h >> 1) * WD_PLANE + (((2 * c + (h & 1)) ^ (row & 7)) << 4));
-                        x[4 * h] = y.x; x[4 * h + 1] = y.y; x[4 * h + 2] = y.z; x[4 * h + 3] = y.w;
-                    }
-                    tmem_st16(tm + T_Q + 16 * c, x);
-                }
-            }
-            tmem_publish();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.q_ready[tile]);
 
-            RowState row;
-            row.off = KV8_REF_NONE; row.lift = WD_LIFT_MAX; row.carry = 1.f;
-            row.sum = f2(0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < 64; j++) row.o[j] = 0.f;
-            auto add_output = [&]() {
-                const F2 carry = f2(row.carry, row.carry);
-                float y[2][16];
-                tmem_ld16(tm + T_O, y[0]);
+            for (int c = 0; c < 4; c++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    tmem_ld_wait(y[c & 1]);
-                    if (c < 3) tmem_ld16(tm + T_O + 16 * (c + 1), y[(c + 1) & 1]);
+                for (int j = 0; j < 8; j++) row.o[c][j] = 0.f;
+            bool ok = true;
+            int n = 0, added = 0;  // key tiles begun, and those whose output is in row.o
+            auto settle = [&](int back) {
+#pragma unroll 1
+                for (; added <= n - back && ok; added++) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_ready[tile][added & 1], (added >> 1) & 1, status, 22, abort));
+                    if (!ok) return;
+                    tmem_acquire();
+                    const uint32_t from = tm + T_O + (added & 1) * 64;
+                    float y[2][8];
+                    tmem_ld_tile(from, y[0]);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        float* o = row.o + 16 * c + j;
-                        f2_parts(f2_fma(f2(y[c & 1][j], y[c & 1][j + 1]), carry, f2(o[0], o[1])), o[0], o[1]);
+                    for (int c = 0; c < 4; c++) {
+                        tmem_ld_wait(y[c & 1]);
+                        if (c < 3) tmem_ld_tile(from + 16 * c + 16, y[(c + 1) & 1]);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) row.o[c][j] += y[c & 1][j];
                     }
                 }
             };
-            bool ok = true;
-            for (int n = 0; n < tiles; n++) {
+            for (; ok && n < tiles; n++) {
                 const int st = n & (WD_STAGES - 1), u0 = u_first + n * WD_KEYS;
                 ok = mbar_wait(&sh.v_full[st], (n / WD_STAGES) & 1, status, 21, abort) &&  // the scales come with the values
                      mbar_wait(&sh.s_ready[tile][n & 1], (n >> 1) & 1, status, 20, abort);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 tmem_acquire();
-                const TileKeys keys{sh.ks[st], sh.vs[st], u0, lo, hi};
+                const TileKeys keys{sh.ks[st] + col, sh.vs[st] + col, u0 + col};
                 const uint32_t tp = tm + (n & 1) * WD_KEYS;
-                const float k_top = fmaxf(fmaxf(sh.k_top[st][0], sh.k_top[st][1]), fmaxf(sh.k_top[st][2], sh.k_top[st][3]));
-                // |q.k| <= |q| |k|: no weight passes 2^100.
-                if (__any_sync(0xffffffffu, !(ex2(reach * k_top - row.off) <= WD_WEIGHT_MAX))) {
-                    const float2 rl = row_reference(tp, keys, rs, row.off, row.lift);
-                    const float to = rl.x - rl.y;
-                    if (to != row.off) row.scale(ex2(row.off - to));
-                    row.off = to;
-                    row.lift = rl.y;
-                }
-                if (u0 >= r.in_lo && u0 + WD_KEYS - 1 <= r.in_hi) row_weights<false>(tp, keys, rs, row);
-                else row_weights<true>(tp, keys, rs, row);
-                if (n > 0) {  // the last tile's output, before the next is written over it
-                    ok = mbar_wait(&sh.o_ready[tile], (n - 1) & 1, status, 22, abort);
-                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                    tmem_acquire();
-                    add_output();
-                }
-                row.carry = 1.f;
+                settle(2);
+                int c = 0;
+                if (!row.fresh && u0 >= r.in_lo && u0 + WD_KEYS - 1 <= r.in_hi) c = row_weights(tp, keys, row);
+                if (c < 4) row_weights_slowly(tp, keys, row, c, settle);
                 tmem_publish();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_ready[tile]);
+                if (lane == 0) mbar_arrive(&sh.p_ready[tile][n & 1]);  // by parity: a warp can be a tile ahead of another
             }
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_ready[tile], (tiles - 1) & 1, status, 22, abort));
+            if (ok) settle(1);
             if (ok) {
-                tmem_acquire();
-                add_output();
-                if (target >= 0) {
-                    float s0, s1;
-                    f2_parts(row.sum, s0, s1);
-                    const float down = ex2(-row.lift), total = (s0 + s1) * down;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    float s0 = row.sum[i];
+                    s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
+                    s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
+                    if (target[i] < 0) continue;
+                    const float lift = row.lift[i] == WD_UNSET ? 0.f : row.lift[i], down = ex2(-lift), total = s0 * down;
                     float f = sh.unit * down;
                     float* dst;
                     bool vec = true;
                     if (a.parts == 1) {
-                        const int at = target / a.hq, head = target - at * a.hq;
-                        dst = a.out + (size_t)at * a.ldo + (size_t)head * 64;
+                        const int at = target[i] / a.hq;
+                        dst = a.out + (size_t)at * a.ldo + (size_t)(target[i] - at * a.hq) * 64;
                         vec = a.ovec;
                         f /= total;
                     } else {
-                        const size_t part = (size_t)target * a.parts + a.part0 + split;
-                        reinterpret_cast<float2*>(a.part_ml)[part] = make_float2(row.off + row.lift, total);
-                        dst = a.part_o + part * 64;
+                        const size_t at = (size_t)target[i] * a.parts + a.part0 + split;
+                        if (col == 0) reinterpret_cast<float2*>(a.part_ml)[at] = make_float2(s0 == 0.f ? KV8_REF_NONE : row.off[i] + lift, total);
+                        dst = a.part_o + at * 64;
                     }
-                    if (vec) {
+                    dst += col;
 #pragma unroll
-                        for (int j = 0; j < 16; j++)
-                            reinterpret_cast<float4*>(dst)[j] =
-                                make_float4(row.o[4 * j] * f, row.o[4 * j + 1] * f, row.o[4 * j + 2] * f, row.o[4 * j + 3] * f);
-                    } else {
+                    for (int c = 0; c < 4; c++)
 #pragma unroll
-                        for (int j = 0; j < 64; j++) dst[j] = row.o[j] * f;
-                    }
+                        for (int j = 0; j < 2; j++) {
+                            const float* o = row.o[c] + 4 * j + 2 * i;
+                            if (vec) {
+                                *reinterpret_cast<float2*>(dst + 16 * c + 8 * j) = make_float2(o[0] * f, o[1] * f);
+                            } else {
+                                dst[16 * c + 8 * j] = o[0] * f;
+                                dst[16 * c + 8 * j + 1] = o[1] * f;
+                            }
+                        }
                 }
             }
         }
     } else if (warp < WD_ROW_WARPS + WD_CONVERT_WARPS) {
-        fewer_registers<WD_CONVERT_REGS>();
-        // Four lanes a key, 16 codes each: 32 keys a pass. The next tile's codes are in registers while
-        // this one's stage is waited for.
-        const int i = threadIdx.x - 32 * WD_ROW_WARPS, part = i & 3, w = warp - WD_ROW_WARPS;
-        uint4 k[2], v[2];
-        float kn[2], ks = 0.f, vs = 0.f;  // scales of the keys whose codes this lane has; of key i
+        // Four lanes a key, 16 codes each: 8 keys a warp at a time, the three warps in turn. The stages let
+        // them run ahead of the tensor cores, which hides the loads' latency.
+        const int w = warp - WD_ROW_WARPS, part = lane & 3;
+        constexpr int TURNS = (WD_KEYS / 8 + WD_CONVERT_WARPS - 1) / WD_CONVERT_WARPS;
+        uint4 k[TURNS], v[TURNS];
+        float ks[TURNS], vs[TURNS];
+        auto key_of = [&](int j) { return 8 * (w + WD_CONVERT_WARPS * j) + (lane >> 2); };
+        const uint8_t *k0 = a.c.k + r.row * 64 + 16 * part, *v0 = a.c.v + r.row * 64 + 16 * part;
+        const float *ks0 = a.c.ks + r.row, *vs0 = a.c.vs + r.row;
         auto load = [&](int u0) {
             const bool whole = r.whole(u0, WD_KEYS);
-            const size_t at = r.row + (u0 >= r.capacity ? u0 - r.capacity : u0);
+            const int first = u0 >= r.capacity ? u0 - r.capacity : u0;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int j = 0; j < TURNS; j++) {
                 // Keys outside the range stand in as the nearest inside it: see kv8_attention.cu.
-                const int key = 32 * j + (i >> 2);
-                const size_t slot = whole ? at + key : r.slot(u0 + key), byte = slot * 64 + 16 * part;
-                k[j] = *reinterpret_cast<const uint4*>(a.c.k + byte);
-                v[j] = *reinterpret_cast<const uint4*>(a.c.v + byte);
-                kn[j] = a.c.ks[slot];
-            }
-            if (i < WD_KEYS) {
-                const size_t slot = whole ? at + i : r.slot(u0 + i);
-                ks = a.c.ks[slot];
-                vs = a.c.vs[slot];
+                const int key = min(key_of(j), WD_KEYS - 1);
+                int slot = first + key;
+                if (!whole) {
+                    slot = min(max(u0 + key, r.lo), r.hi);
+                    slot = slot >= r.capacity ? slot - r.capacity : slot;
+                }
+                k[j] = *reinterpret_cast<const uint4*>(k0 + (size_t)slot * 64);
+                v[j] = *reinterpret_cast<const uint4*>(v0 + (size_t)slot * 64);
+                ks[j] = ks0[slot];
+                vs[j] = vs0[slot];
             }
         };
-        auto store = [&](uint8_t* stage, const uint4 (&x)[2]) {
+        auto store = [&](uint8_t* stage, const uint4 (&x)[TURNS]) {
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int key = 32 * j + (i >> 2);
+            for (int j = 0; j < TURNS; j++) {
+                const int key = key_of(j);
+                if (key >= WD_KEYS) break;
                 const uint32_t c[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
                 uint32_t h[8];
 #pragma unroll
@@ -564,74 +550,53 @@ __global__ void __launch_bounds__(WD_THREADS, 1) kv8_wide_kernel(const PassArgs 
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
-        // Norms of the lanes' keys (scale not included), to 2%.
-        auto norm = [&](const uint4& x) {
-            const uint32_t c[4] = {x.x, x.y, x.z, x.w};
-            float sq;
-            if (KIND == MT_KV_INT8) {
-                int n = 0;
-#pragma unroll
-                for (int j = 0; j < 4; j++) n = __dp4a((int)c[j], (int)c[j], n);
-                sq = (float)n;
-            } else {
-                __half2 n = __float2half2_rn(0.f);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    uint32_t h[2];
-                    to_half<KIND>(c[j], h[0], h[1]);
-#pragma unroll
-                    for (int m = 0; m < 2; m++) {  // / 256: 16 squares stay below fp16's range
-                        const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h[m]), __float2half2_rn(0x1p-8f));
-                        n = __hfma2(y, y, n);
-                    }
-                }
-                const float2 f = __half22float2(n);
-                sq = (f.x + f.y + 0x1p-10f) * 65536.f;
-            }
-            sq += __shfl_xor_sync(0xffffffffu, sq, 1);
-            sq += __shfl_xor_sync(0xffffffffu, sq, 2);
-            return 1.02f * sqrtf(sq);
-        };
         load(u_first);
         // The value scales' unit, from the first tile: a power of two, divided out of all of them.
-        const float mine = warp_max(fabsf(vs));
-        if (lane == 0) sh.first[w] = mine;
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const float per_unit = power_to(fmaxf(fmaxf(sh.first[0], sh.first[1]), fmaxf(sh.first[2], sh.first[3])), 0);
-        if (i == 0) sh.unit = 1.f / per_unit;
+        float most = 0.f;
+#pragma unroll
+        for (int j = 0; j < TURNS; j++) most = fmaxf(most, fabsf(vs[j]));
+        most = warp_max(most);
+        if (lane == 0) sh.first[w] = most;
+        asm volatile("bar.sync 1, 96;" ::: "memory");
+        const float per_unit = power_to(fmaxf(sh.first[0], fmaxf(sh.first[1], sh.first[2])), 0);
+        if (w == 0 && lane == 0) sh.unit = 1.f / per_unit;
         for (int n = 0; n < tiles; n++) {
+            if (n > 0) load(u_first + n * WD_KEYS);
             const int st = n & (WD_STAGES - 1);
             const uint32_t reuse = ((n / WD_STAGES) & 1) ^ 1;
-            const float k_top = warp_max(fmaxf(norm(k[0]) * fabsf(kn[0]), norm(k[1]) * fabsf(kn[1])));
             if (n >= WD_STAGES && !mbar_wait(&sh.k_free[st], reuse, status, 23, abort)) break;
             store(stages + st * WD_STAGE, k);
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.k_full[st]);
             if (n >= WD_STAGES && !mbar_wait(&sh.v_free[st], reuse, status, 24, abort)) break;
             store(stages + (WD_STAGES + st) * WD_STAGE, v);
-            if (i < WD_KEYS) {
-                sh.ks[st][i] = ks;
-                sh.vs[st][i] = vs * per_unit;
+            if (part == 0) {
+#pragma unroll
+                for (int j = 0; j < TURNS; j++) {
+                    const int key = key_of(j);
+                    if (key >= WD_KEYS) break;
+                    sh.ks[st][key] = ks[j];
+                    sh.vs[st][key] = vs[j] * per_unit;
+                }
             }
-            if (lane == 0) sh.k_top[st][w] = k_top;
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.v_full[st]);
-            if (n + 1 < tiles) load(u_first + (n + 1) * WD_KEYS);
         }
     } else {
-        fewer_registers<WD_ISSUE_REGS>();
         if (warp == WD_ROW_WARPS + WD_CONVERT_WARPS && elect_one()) {
         const uint64_t k_desc = tile_desc(smem_u32(stages)), v_desc = tile_desc(smem_u32(stages) + WD_STAGES * WD_STAGE);
+        const uint64_t q_desc = tile_desc(smem_u32(stages) + 2 * WD_STAGES * WD_STAGE);
         // Scores of a row tile: 4 steps of 16 dimensions (32 bytes of a row) for each plane of Q. The lo
         // planes go first, here and below: their sums are small, and so is what the accumulator drops.
         auto scores = [&](int tile, int n) {
             const uint32_t at = tmem + tile * T_TILE;
             const uint64_t b = k_desc + (uint64_t)((n & (WD_STAGES - 1)) * (WD_STAGE >> 4));
+            const uint64_t q = q_desc + (uint64_t)(tile * (2 * WD_PLANE >> 4));
 #pragma unroll
             for (int p = 1; p >= 0; p--)
 #pragma unroll
                 for (int s = 0; s < 4; s++)
-                    mma_ts(at + (n & 1) * WD_KEYS, at + T_Q + 16 * s + 8 * p, b + 2 * s, IDESC_S, p == 0 || s > 0);
+                    mma_ss(at + (n & 1) * WD_KEYS, q + p * (WD_PLANE >> 4) + 2 * s, b + 2 * s, IDESC_S, p == 0 || s > 0);
         };
         // Outputs: 4 steps of 16 keys (16 rows of V, 2048 bytes) for each plane of P.
         auto outputs = [&](int tile, int n) {
@@ -641,38 +606,34 @@ __global__ void __launch_bounds__(WD_THREADS, 1) kv8_wide_kernel(const PassArgs 
             for (int p = 1; p >= 0; p--)
 #pragma unroll
                 for (int s = 0; s < 4; s++)
-                    mma_ts(at + T_O, at + (n & 1) * WD_KEYS + 16 * s + 8 * p, b + 128 * s, IDESC_O, p == 0 || s > 0);
+                    mma_ts(at + T_O + (n & 1) * 64, at + (n & 1) * WD_KEYS + 16 * s + 8 * p, b + 128 * s, IDESC_O, p == 0 || s > 0);
         };
         auto keys_ready = [&](int n) { return mbar_wait(&sh.k_full[n & (WD_STAGES - 1)], (n / WD_STAGES) & 1, status, 25, abort); };
         bool ok = true;
-        for (int n = 0; ok && n < 2 && n < tiles; n++) {
-            ok = keys_ready(n);
-            for (int t = 0; ok && t < row_tiles; t++) {
-                ok = n > 0 || mbar_wait(&sh.q_ready[t], 0, status, 26, abort);
-                if (!ok) break;
-                tmem_acquire();
-                scores(t, n);
-                mma_done(&sh.s_ready[t][n & 1]);
+        for (int t = 0; ok && t < row_tiles; t++) ok = mbar_wait(&sh.q_ready[t], 0, status, 26, abort);
+        for (int n = -1; ok && n < tiles; n++) {
+            // The next tile's scores, into the buffer of the last one's weights: its product has read them.
+            if (n + 1 < tiles) {
+                ok = keys_ready(n + 1);
+                for (int t = 0; ok && t < row_tiles; t++) {
+                    ok = n < 1 || mbar_wait(&sh.o_ready[t][(n - 1) & 1], ((n - 1) >> 1) & 1, status, 30, abort);
+                    if (!ok) break;
+                    tmem_acquire();
+                    scores(t, n + 1);
+                    mma_done(&sh.s_ready[t][(n + 1) & 1]);
+                }
+                if (ok) mma_done(&sh.k_free[(n + 1) & (WD_STAGES - 1)]);
             }
-            if (ok) mma_done(&sh.k_free[n]);
-        }
-        for (int n = 0; ok && n < tiles; n++) {
-            const bool more = n + 2 < tiles;
+            if (n < 0 || !ok) continue;
+            ok = mbar_wait(&sh.v_full[n & (WD_STAGES - 1)], (n / WD_STAGES) & 1, status, 28, abort);
             for (int t = 0; ok && t < row_tiles; t++) {
-                ok = mbar_wait(&sh.p_ready[t], n & 1, status, 27, abort) &&
-                     (t > 0 || mbar_wait(&sh.v_full[n & (WD_STAGES - 1)], (n / WD_STAGES) & 1, status, 28, abort));
+                ok = mbar_wait(&sh.p_ready[t][n & 1], (n >> 1) & 1, status, 27, abort);
                 if (!ok) break;
                 tmem_acquire();
                 outputs(t, n);
-                mma_done(&sh.o_ready[t]);
-                if (t == row_tiles - 1) mma_done(&sh.v_free[n & (WD_STAGES - 1)]);
-                if (!more) continue;
-                ok = t > 0 || keys_ready(n + 2);
-                if (!ok) break;
-                scores(t, n + 2);
-                mma_done(&sh.s_ready[t][n & 1]);
-                if (t == row_tiles - 1) mma_done(&sh.k_free[(n + 2) & (WD_STAGES - 1)]);
+                mma_done(&sh.o_ready[t][n & 1]);
             }
+            if (ok) mma_done(&sh.v_free[n & (WD_STAGES - 1)]);
         }
         }
     }
