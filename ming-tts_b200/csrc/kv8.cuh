@@ -53,6 +53,10 @@ struct PassArgs {
     int key_warps;                   // warps of a block that share a row tile and interleave its keys
     float *part_o, *part_ml;         // parts: [row * hq + head][parts][64] and [..][parts][2] (reference, sum)
     int parts, part0;                // parts of the whole call, and this pass's first
+    // The pass before this one in the stream is the same call's other pass: they write different parts, so
+    // this one runs beside it and waits for it at its end (every block of that pass has waited for what
+    // came before the call, or this one would not have been launched).
+    bool beside;
 };
 
 // Where the keys of a tile of rows are. Index u counts positions from a multiple of the capacity, so that

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
     using R = Rows<NT>;
     constexpr int LR = R::LANE;
     extern __shared__ float smem[];  // [warp][row][64] sums, [warp][row][2] reference and sum, [row] owner
-    pdl_wait();
+    if (!a.beside) pdl_wait();
     pdl_launch();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     // Blocks with the most keys (the last rows) first.
@@ -399,6 +399,7 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
             reinterpret_cast<float4*>(a.part_o + part * 64)[d4] = y;
         }
     }
+    if (a.beside) pdl_wait();
 }
 
 // Joins the parts of each (row, head): out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. A warp a
@@ -466,7 +467,7 @@ struct PassPlan {
 constexpr int WIDE_FROM = 97;
 
 // `units` row spaces of `qrows` (row, head) rows each over at most `keys` keys.
-PassPlan plan_pass(int sm_count, long long units, long long qrows, int keys, bool causal) {
+PassPlan plan_pass(int sm_count, long long units, long long qrows, int keys) {
     PassPlan p{};
     if (units < 1) return p;
     if (qrows >= WIDE_FROM) {
@@ -475,7 +476,7 @@ PassPlan plan_pass(int sm_count, long long units, long long qrows, int keys, boo
         p.row_blocks = (int)((qrows + KV8_WIDE_ROWS - 1) / KV8_WIDE_ROWS);
         const int tiles = (keys + 15 + KV8_WIDE_KEYS - 1) / KV8_WIDE_KEYS;
         const long long blocks = units * p.row_blocks;
-        long long s = causal ? (2ll * sm_count + blocks - 1) / blocks : sm_count / blocks;
+        long long s = sm_count / blocks;
         if (s > tiles / 4) s = tiles / 4;
         if (s < 1) s = 1;
         p.chunk = (int)((tiles + s - 1) / s);
@@ -517,10 +518,10 @@ Plan make_plan(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int
     const int hkv = cache->kv_heads > 0 ? cache->kv_heads : 1;
     const long long group = hq / hkv;
     const long long seen = window > 0 ? (long long)window + rows - 1 : cache->capacity;
-    p.own = plan_pass(ctx->sm_count, (long long)requests * hkv, rows * group, (int)(seen < cache->capacity ? seen : cache->capacity), true);
+    p.own = plan_pass(ctx->sm_count, (long long)requests * hkv, rows * group, (int)(seen < cache->capacity ? seen : cache->capacity));
     p.parts = p.own.splits;
     if (prefix_len > 0) {
-        p.prefix = plan_pass(ctx->sm_count, hkv, (long long)requests * rows * group, prefix_len, false);
+        p.prefix = plan_pass(ctx->sm_count, hkv, (long long)requests * rows * group, prefix_len);
         p.parts += p.prefix.splits;
     }
     if (p.parts > 1) {
@@ -586,6 +587,7 @@ mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q,
         run(plan.prefix);
     }
     a.c = view(cache); a.prefix_len = 0; a.part0 = plan.parts - plan.own.splits; a.window = window;
+    a.beside = prefix_len > 0;
     run(plan.own);
     if (plan.parts > 1) {
         JoinArgs j{a.rows, requests * rows, hq, plan.parts, a.part_o, a.part_ml, out, ldo, a.ovec};

@@ -45,7 +45,7 @@ constexpr int WD_STAGES = 4;
 constexpr int WD_PLANE = 128 * 128;      // bytes of a plane of a row tile's queries
 constexpr size_t WD_SMEM = 2 * WD_STAGES * WD_STAGE + 4 * WD_PLANE + 1024;
 constexpr uint32_t T_O = 128, T_TILE = 256;
-constexpr int WD_LIFT_TO = 8;         // exponent that a row's largest scaled product is brought to ..
+constexpr int WD_LIFT_TO = 0;         // exponent that a row's largest scaled product is brought to ..
 constexpr float WD_PRODUCT_MAX = 32768.f;  // .. once one is above this (fp16 ends at 65504)
 constexpr float WD_WEIGHT_MAX = 0x1p100f;  // what a sum of four weights may be in units of 2^off
 
@@ -304,12 +304,10 @@ template <int N>
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <int KIND>
-__global__ void __launch_bounds__(WD_THREADS, 1) kv8_wide_kernel(const PassArgs a, int chunk, unsigned int* status) {
+__device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigned int* status) {
     extern __shared__ uint8_t dynamic[];
     __shared__ Shared sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    pdl_wait();
-    pdl_launch();
     // Blocks with the most keys (the last rows) first.
     const int split = blockIdx.x % a.splits;
     const int unit = (blockIdx.x / a.splits) % a.units;
@@ -644,6 +642,14 @@ __global__ void __launch_bounds__(WD_THREADS, 1) kv8_wide_kernel(const PassArgs 
         tmem_acquire();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(WD_THREADS, 1) kv8_wide_kernel(const PassArgs a, int chunk, unsigned int* status) {
+    if (!a.beside) pdl_wait();
+    pdl_launch();
+    wide_block<KIND>(a, chunk, status);
+    if (a.beside) pdl_wait();
 }
 
 }  // namespace
