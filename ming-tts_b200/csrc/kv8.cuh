@@ -37,7 +37,6 @@ struct Kv8View {
     const float *ks, *vs;
     long long request_stride;
     int capacity, kind;
-    bool quads;  // four scales from a slot that is a multiple of four are one aligned 16-byte load
 };
 
 // One pass over one set of keys: a request's own cache (units: request x kv head, causal), or the
@@ -176,6 +175,39 @@ __device__ __forceinline__ void split_half2(float x0, float x1, uint32_t& hi, ui
 __device__ __forceinline__ float power_to(float x, int target) {
     const int e = (int)(__float_as_uint(x) >> 23) - 127;
     return __uint_as_float((uint32_t)(min(126, max(-126, target - e)) + 127) << 23);
+}
+
+// The unit of a row's weights. They are 2^(score - off), off = reference - lift: the reference is near a
+// score that was the row's largest, the lift brings the largest weight times value scale to 1 when it is
+// set: the two planes hold 22 bits of products down to 2^-3 of it, 2^-25 of it below, and have room for
+// 2^15 above. A row moves its unit only when a product leaves that room (or a weight fp32's): keeping
+// the products near 2^8 instead moved it ten times as often, and cost 10% of the wide kernel's time.
+constexpr float KV8_UNSET = 1000.f;           // the lift of a row that has no unit yet (its off is 0)
+constexpr float KV8_PRODUCT_MAX = 32768.f;    // fp16 ends at 65504
+constexpr float KV8_WEIGHT_MAX = 0x1p100f;    // what a sum of four weights may be
+
+// (off, lift) of a row after four of a lane's keys (scores z in powers of two, -infinity where not seen,
+// value scales v): all four lanes of the row get the same.
+__device__ __forceinline__ float2 kv8_unit(const float (&z)[4], const float (&v)[4], float off, float lift) {
+    auto row_max = [](float x) {
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+    };
+    auto product = [&](float from) {  // the largest, in units of 2^from
+        float x = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) x = fmaxf(x, ex2(z[j] - from) * v[j]);
+        return row_max(x);
+    };
+    const float most = row_max(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
+    const bool unset = lift == KV8_UNSET;
+    const float now = product(off);
+    const bool move = most > -INFINITY && (unset || most - off > 90.f || now > KV8_PRODUCT_MAX);
+    const float ref = unset ? most : fmaxf(off + lift, most);
+    const float then = product(ref);
+    if (!move) return make_float2(off, lift);
+    lift = then > 0.f ? fminf(80.f, fmaxf(-100.f, (float)(127 - (int)(__float_as_uint(then) >> 23)))) : 0.f;
+    return make_float2(ref - lift, lift);
 }
 
 // Makes a device current for a call and puts the caller's back.

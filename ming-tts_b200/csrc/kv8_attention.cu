@@ -23,6 +23,8 @@
 //     8 g + i, so lane t's outputs are dimensions 16 t .. 16 t + 15.
 #include <math.h>
 
+#include <type_traits>
+
 #include "kv8.cuh"
 
 namespace mt {
@@ -36,41 +38,46 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Codes and scales of a warp's 16 keys, in a lane's share.
-struct KeyTile {
-    uint4 k[2];
-    uint2 v[4];
-    float ks[4], vs[4];
-};
+// A warp's ring of key tiles in shared memory, filled by asynchronous copies RING - 1 tiles ahead: codes of
+// 16 keys (64 bytes a key) and their scales. 16 warps an SM have some 100 KB in flight, where one tile
+// ahead in registers had 33 and was bound by DRAM's latency (8 long requests 28 us).
+constexpr int RING = 4;
+constexpr int TILE_BYTES = 2 * 16 * 64 + 2 * 16 * 4;
 
-__device__ __forceinline__ void load_keys(KeyTile& x, const Kv8View& c, const KeyRange& r, int u0, int g, int t) {
-    const int s0 = u0 >= r.capacity ? u0 - r.capacity : u0;
-    if (c.quads && r.whole(u0, 16)) {
-        const size_t at = r.row + s0;
-        const uint8_t* kp = c.k + (at + 4 * (g >> 1) + (g & 1)) * 64 + 16 * t;
-        x.k[0] = *reinterpret_cast<const uint4*>(kp);
-        x.k[1] = *reinterpret_cast<const uint4*>(kp + 128);
-        const uint8_t* vp = c.v + (at + 4 * t) * 64 + 8 * g;
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool l1) {
+    if (l1) asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
+// Keys outside the range stand in as the nearest inside it: the slot of a key that no row sees may hold
+// codes that are NaN, which a weight of zero would not silence. Value rows are placed so that the reads
+// below (4 rows 256 bytes apart, 8 bytes each of 4 places) touch every bank once: odd groups of four rows
+// have their rows swapped in pairs, the last eight rows their halves.
+__device__ __forceinline__ void copy_keys(uint32_t to, const Kv8View& c, const KeyRange& r, int u0, int lane, bool l1) {
+    const int part = lane & 3, key = lane & 15;
+    const float* const scales = lane < 16 ? c.ks : c.vs;
+    const bool whole = r.whole(u0, 16);
+    const size_t first = r.row + (u0 >= r.capacity ? u0 - r.capacity : u0);
 #pragma unroll
-        for (int i = 0; i < 4; i++) x.v[i] = *reinterpret_cast<const uint2*>(vp + 64 * i);
-        const float4 a = *reinterpret_cast<const float4*>(c.ks + at + 4 * t);
-        const float4 b = *reinterpret_cast<const float4*>(c.vs + at + 4 * t);
-        x.ks[0] = a.x; x.ks[1] = a.y; x.ks[2] = a.z; x.ks[3] = a.w;
-        x.vs[0] = b.x; x.vs[1] = b.y; x.vs[2] = b.z; x.vs[3] = b.w;
-        return;
+    for (int j = 0; j < 2; j++) {
+        const int row = 8 * j + (lane >> 2);
+        const size_t from = (whole ? first + row : r.slot(u0 + row)) * 64 + 16 * part;
+        copy16(to + row * 64 + 16 * part, c.k + from, l1);
+        copy16(to + 1024 + (row ^ ((row >> 2) & 1)) * 64 + 16 * (part ^ (2 * j)), c.v + from, l1);
     }
-    // Keys outside the range stand in as the nearest inside it: the slot of a key that no row sees may
-    // hold codes that are NaN, which a weight of zero would not silence.
-#pragma unroll
-    for (int j = 0; j < 2; j++)
-        x.k[j] = *reinterpret_cast<const uint4*>(c.k + r.slot(u0 + 4 * (g >> 1) + 2 * j + (g & 1)) * 64 + 16 * t);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const size_t at = r.slot(u0 + 4 * t + i);
-        x.v[i] = *reinterpret_cast<const uint2*>(c.v + at * 64 + 8 * g);
-        x.ks[i] = c.ks[at];
-        x.vs[i] = c.vs[at];
-    }
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 2048 + 4 * lane), "l"(scales + (whole ? first + key : r.slot(u0 + key)))
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Power of two that brings the largest of a tile's value scales near 1 (all zero: 1).
+__device__ __forceinline__ float value_unit(const float (&vs)[4]) {
+    float x = fmaxf(fmaxf(fabsf(vs[0]), fabsf(vs[1])), fmaxf(fabsf(vs[2]), fabsf(vs[3])));
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+    return x > 0.f ? power_to(x, 0) : 1.f;
 }
 
 // NT 0: 8 rows, whose hi planes are rows 0-7 and lo planes rows 8-15 of one 16-row operand (a decode
@@ -83,6 +90,8 @@ struct Rows {
     static constexpr int COUNT = NT == 0 ? 8 : 16 * NT;   // rows of a warp
     static constexpr int WARPS = NT == 0 ? 8 : 4;
     static constexpr int BLOCKS = NT == 2 ? 2 : NT == 1 ? 3 : 2;  // resident blocks the registers allow
+    static constexpr int SUM_BYTES = WARPS * COUNT * (64 + 2 + 1) * 4;   // sums, references, owners
+    static constexpr int SMEM = SUM_BYTES + WARPS * RING * TILE_BYTES;
 };
 
 constexpr int FOLD = 8;               // key tiles summed in the matrix unit's accumulators at a time
@@ -91,7 +100,8 @@ template <int KIND, int NT>
 __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pass_kernel(const PassArgs a) {
     using R = Rows<NT>;
     constexpr int LR = R::LANE;
-    extern __shared__ float smem[];  // [warp][row][64] sums, [warp][row][2] reference and sum, [row] owner
+    // [warp][row][64] sums, [warp][row][2] reference and sum, [row] owner, [warp] ring
+    extern __shared__ __align__(16) float smem[];
     if (!a.beside) pdl_wait();
     pdl_launch();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -110,14 +120,15 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
 #pragma unroll
     for (int i = 0; i < LR; i++) row_of[i] = any_row ? rows.pair(e0 + 8 * i + g, lo[i], hi[i]) : -1;
 
-    // Sums of the rows in shared memory, in units of 2^at_ref: the matrix unit drops the bits of a sum
+    // Sums of the rows in shared memory, in units of 2^at_off: the matrix unit drops the bits of a sum
     // that its 24 do not hold (it does not round them), so a long chain of products drifts towards
     // zero: 256 key tiles in one chain were 4e-6 off. Every FOLD tiles the registers are added here.
     float* const acc = smem + (warp * R::COUNT + g) * 64 + 16 * t;  // row i of the lane: + 512 i
-    float ref[LR], at_ref[LR], sum[LR], unit_w[LR];
+    float off[LR], at_off[LR], lift[LR], sum[LR], v_unit = 0.f;  // see kv8_unit; v_unit divides the value scales
+    bool fresh = true;
     float o[R::SETS][8][4];
 #pragma unroll
-    for (int i = 0; i < LR; i++) { ref[i] = KV8_REF_NONE; at_ref[i] = KV8_REF_NONE; sum[i] = 0.f; unit_w[i] = 0x1p126f; }
+    for (int i = 0; i < LR; i++) { off[i] = 0.f; at_off[i] = 0.f; lift[i] = KV8_UNSET; sum[i] = 0.f; }
     auto clear = [&]() {
 #pragma unroll
         for (int n = 0; n < R::SETS; n++)
@@ -127,11 +138,12 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
                 for (int j = 0; j < 4; j++) o[n][i][j] = 0.f;
     };
     clear();
-    auto fold = [&](bool first) {
+    auto fold = [&](bool first, bool last) {
+        const float n = v_unit > 0.f ? 1.f / v_unit : 0.f;
 #pragma unroll
         for (int i = 0; i < LR; i++) {
-            const float f = first ? 0.f : ex2(at_ref[i] - ref[i]), n = 1.f / unit_w[i];
-            at_ref[i] = ref[i];
+            const float f = first ? 0.f : ex2(at_off[i] - off[i]), down = last && lift[i] != KV8_UNSET ? ex2(-lift[i]) : 1.f;
+            at_off[i] = off[i];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 float4* at = reinterpret_cast<float4*>(acc + 512 * i) + j;
@@ -139,7 +151,7 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
                 auto add = [&](float& x, int d) {
                     const int m = 4 * (j & 1) + d, col = j >> 1;
                     const float v = NT == 0 ? o[0][m][col] + o[0][m][2 + col] : o[i / 2][m][2 * (i & 1) + col];
-                    x = first ? v * n : fmaf(v, n, x * f);
+                    x = (first ? v * n : fmaf(v, n, x * f)) * down;
                 };
                 add(y.x, 0); add(y.y, 1); add(y.z, 2); add(y.w, 3);
                 *at = y;
@@ -148,13 +160,19 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
     };
 
     const int t0 = r.lo >> 4, tiles = any_row ? (r.hi >> 4) - t0 + 1 : 0;
-    const int per = (tiles + a.splits - 1) / a.splits;
+    const int per = max((tiles + a.splits - 1) / a.splits, 2 * a.key_warps);  // a short request in fewer parts
     const int end = min(tiles, (split + 1) * per);
     int at = split * per + phase;
     bool folded = false;
     if (at < end) {
-        KeyTile next;
-        load_keys(next, a.c, r, (t0 + at) * 16, g, t);
+        const bool l1 = a.key_warps == 1;  // the block's warps read the same keys
+        const uint8_t* const ring = reinterpret_cast<const uint8_t*>(smem) + R::SUM_BYTES + warp * RING * TILE_BYTES;
+        const uint32_t ring_at = smem_u32(ring);
+#pragma unroll
+        for (int i = 0; i < RING - 1; i++) {
+            if (at + i * a.key_warps < end) copy_keys(ring_at + i * TILE_BYTES, a.c, r, (t0 + at + i * a.key_warps) * 16, lane, l1);
+            copies_commit();
+        }
         // Queries: 16 dimensions of each of the lane's rows, as fp16 planes of a power-of-two multiple.
         uint32_t qa[R::SETS][R::PLANES][4][4];
         float q_scale[LR];
@@ -200,22 +218,31 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
         }
 
         int chain = 0;
-        for (; at < end; at += a.key_warps) {
+        for (int stage = 0; at < end; at += a.key_warps, stage = (stage + 1) & (RING - 1)) {
             if (++chain == FOLD + 1) {
-                fold(!folded);
+                fold(!folded, false);
                 clear();
                 folded = true;
                 chain = 1;
             }
-            const KeyTile x = next;
             const int u0 = (t0 + at) * 16;
-            if (at + a.key_warps < end) load_keys(next, a.c, r, u0 + 16 * a.key_warps, g, t);
+            __syncwarp();  // every lane has read the tile that is copied over
+            if (at + (RING - 1) * a.key_warps < end)
+                copy_keys(ring_at + ((stage + RING - 1) & (RING - 1)) * TILE_BYTES, a.c, r, u0 + 16 * (RING - 1) * a.key_warps, lane, l1);
+            copies_commit();
+            copies_wait<RING - 1>();
+            __syncwarp();
+            const uint8_t* const x = ring + stage * TILE_BYTES;
+            const float4 ks4 = *reinterpret_cast<const float4*>(x + 2048 + 16 * t), vs4 = *reinterpret_cast<const float4*>(x + 2112 + 16 * t);
+            const float ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w};
+            float vs[4] = {vs4.x, vs4.y, vs4.z, vs4.w};
 
             // Scores (before scaling): 4 keys of each of the lane's rows.
             float s[LR][4];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const uint32_t kw[4] = {x.k[j].x, x.k[j].y, x.k[j].z, x.k[j].w};
+                const uint4 k = *reinterpret_cast<const uint4*>(x + (4 * (g >> 1) + 2 * j + (g & 1)) * 64 + 16 * t);
+                const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
                 float c[R::SETS][4];
 #pragma unroll
                 for (int n = 0; n < R::SETS; n++) { c[n][0] = 0.f; c[n][1] = 0.f; c[n][2] = 0.f; c[n][3] = 0.f; }
@@ -240,36 +267,51 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
                 }
             }
             const bool whole = u0 >= r.in_lo && u0 + 15 <= r.in_hi;
-            // Weights exp2(score - reference). The reference moves only when a score is 8 above it (a
-            // factor of 256, which fp32 sums and the planes' range have room for).
-            float w[LR][4];
-            bool raise = false;
+            if (v_unit == 0.f) v_unit = value_unit(vs);
 #pragma unroll
-            for (int i = 0; i < LR; i++) {
+            for (int k = 0; k < 4; k++) vs[k] *= v_unit;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    s[i][k] *= x.ks[k];
-                    w[i][k] = fmaf(s[i][k], q_scale[i], -ref[i]);
-                    if (!whole) {
-                        const int u = u0 + 4 * t + k;
-                        if (u < lo[i] || u > hi[i]) w[i][k] = -INFINITY;
-                    }
-                }
-                raise |= fmaxf(fmaxf(w[i][0], w[i][1]), fmaxf(w[i][2], w[i][3])) > 8.f;
-            }
-            if (__any_sync(0xffffffffu, raise)) {
+            for (int i = 0; i < LR; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) s[i][k] *= ks[k];
+            // Weights 2^(score - off), times the value rows' scales.
+            float w[LR][4], add[LR];
+            auto weigh = [&](auto masked) {
+                bool fine = true;
 #pragma unroll
                 for (int i = 0; i < LR; i++) {
-                    float top = KV8_REF_NONE;
+                    float p[4];
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        if (w[i][k] != -INFINITY) top = fmaxf(top, s[i][k] * q_scale[i]);
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    if (top - ref[i] > 8.f) {
-                        const float before = ref[i];
-                        ref[i] = top;
-                        const float f = ex2(before - ref[i]);
+                    for (int k = 0; k < 4; k++) {
+                        p[k] = ex2(fmaf(s[i][k], q_scale[i], -off[i]));
+                        w[i][k] = p[k] * vs[k];
+                        if (masked) {
+                            const bool on = u0 + 4 * t + k >= lo[i] && u0 + 4 * t + k <= hi[i];
+                            p[k] = on ? p[k] : 0.f;
+                            w[i][k] = on ? w[i][k] : 0.f;  // a scale of a key that this row does not see may be NaN
+                        }
+                    }
+                    add[i] = (p[0] + p[1]) + (p[2] + p[3]);
+                    fine = fine && fmaxf(fmaxf(fabsf(w[i][0]), fabsf(w[i][1])), fmaxf(fabsf(w[i][2]), fabsf(w[i][3]))) <= KV8_PRODUCT_MAX &&
+                           add[i] <= KV8_WEIGHT_MAX;
+                }
+                return fine;
+            };
+            const bool fine = whole ? weigh(std::false_type{}) : weigh(std::true_type{});
+            if (fresh || __any_sync(0xffffffffu, !fine)) {  // rare: a row's unit is set, or moves
+                bool unset = false;
+#pragma unroll
+                for (int i = 0; i < LR; i++) {
+                    float z[4], v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const bool on = whole || (u0 + 4 * t + k >= lo[i] && u0 + 4 * t + k <= hi[i]);
+                        z[k] = on ? s[i][k] * q_scale[i] : -INFINITY;
+                        v[k] = on ? fabsf(vs[k]) : 0.f;
+                    }
+                    const float2 to = kv8_unit(z, v, off[i], lift[i]);
+                    if (to.x != off[i]) {
+                        const float f = ex2(off[i] - to.x);
                         sum[i] *= f;
 #pragma unroll
                         for (int n = 0; n < 8; n++) {
@@ -280,52 +322,21 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
                                 o[i / 2][n][2 * (i & 1) + 1] *= f;
                             }
                         }
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            if (w[i][k] != -INFINITY) w[i][k] = fmaf(s[i][k], q_scale[i], -ref[i]);
                     }
+                    off[i] = to.x;
+                    lift[i] = to.y;
+                    unset |= to.y == KV8_UNSET;
                 }
+                fresh = __any_sync(0xffffffffu, unset);
+                weigh(std::true_type{});
             }
-            // Weights times the value rows' scales, as planes.
             uint32_t pa[R::SETS][R::PLANES][4];
-            bool over = false;
-#pragma unroll
-            for (int i = 0; i < LR; i++) {
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const float p = ex2(w[i][k]);
-                    sum[i] += p;
-                    // a scale of a key that this row does not see may be NaN
-                    w[i][k] = whole || w[i][k] != -INFINITY ? p * x.vs[k] : 0.f;
-                }
-                over |= fmaxf(fmaxf(fabsf(w[i][0]), fabsf(w[i][1])), fmaxf(fabsf(w[i][2]), fabsf(w[i][3]))) * unit_w[i] > 16384.f;
-            }
-            if (__any_sync(0xffffffffu, over)) {
-#pragma unroll
-                for (int i = 0; i < LR; i++) {
-                    float top = fmaxf(fmaxf(fabsf(w[i][0]), fabsf(w[i][1])), fmaxf(fabsf(w[i][2]), fabsf(w[i][3])));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    if (top * unit_w[i] > 16384.f) {
-                        const float now = power_to(top, 10), f = now * (1.f / unit_w[i]);
-                        unit_w[i] = now;
-#pragma unroll
-                        for (int n = 0; n < 8; n++) {
-                            if (NT == 0) {
-                                o[0][n][0] *= f; o[0][n][1] *= f; o[0][n][2] *= f; o[0][n][3] *= f;
-                            } else {
-                                o[i / 2][n][2 * (i & 1)] *= f;
-                                o[i / 2][n][2 * (i & 1) + 1] *= f;
-                            }
-                        }
-                    }
-                }
-            }
 #pragma unroll
             for (int i = 0; i < LR; i++) {
                 uint32_t h0, l0, h1, l1;
-                split_half2(w[i][0] * unit_w[i], w[i][1] * unit_w[i], h0, l0);
-                split_half2(w[i][2] * unit_w[i], w[i][3] * unit_w[i], h1, l1);
+                sum[i] += add[i];
+                split_half2(w[i][0], w[i][1], h0, l0);
+                split_half2(w[i][2], w[i][3], h1, l1);
                 if (NT == 0) {
                     pa[0][0][0] = h0; pa[0][0][1] = l0; pa[0][0][2] = h1; pa[0][0][3] = l1;
                 } else {
@@ -334,10 +345,14 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
                 }
             }
             // Values: dimensions 8g .. 8g+7 of keys 4t .. 4t+3, the two keys of a pair side by side.
+            uint2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                v[i] = *reinterpret_cast<const uint2*>(x + 1024 + ((4 * t + i) ^ (t & 1)) * 64 + 16 * ((g >> 1) ^ (t & 2)) + 8 * (g & 1));
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const uint32_t v0 = h ? x.v[0].y : x.v[0].x, v1 = h ? x.v[1].y : x.v[1].x;
-                const uint32_t v2 = h ? x.v[2].y : x.v[2].x, v3 = h ? x.v[3].y : x.v[3].x;
+                const uint32_t v0 = h ? v[0].y : v[0].x, v1 = h ? v[1].y : v[1].x;
+                const uint32_t v2 = h ? v[2].y : v[2].x, v3 = h ? v[3].y : v[3].x;
                 uint32_t b0[4], b1[4];
                 to_half<KIND>(__byte_perm(v0, v1, 0x5140), b0[0], b0[1]);
                 to_half<KIND>(__byte_perm(v0, v1, 0x7362), b0[2], b0[3]);
@@ -354,13 +369,15 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
     }
 
     // Join the key_warps warps of each row tile.
-    fold(!folded);
+    fold(!folded, true);
     float2* sml = reinterpret_cast<float2*>(smem + R::WARPS * R::COUNT * 64);
 #pragma unroll
     for (int i = 0; i < LR; i++) {
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-        if (t == 0) sml[warp * R::COUNT + 8 * i + g] = make_float2(ref[i], sum[i]);
+        if (t == 0)
+            sml[warp * R::COUNT + 8 * i + g] =
+                lift[i] == KV8_UNSET ? make_float2(KV8_REF_NONE, sum[i]) : make_float2(off[i] + lift[i], sum[i] * ex2(-lift[i]));
     }
     int* owner = reinterpret_cast<int*>(sml + R::WARPS * R::COUNT);
     if (phase == 0 && t == 0) {
@@ -396,54 +413,62 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
         } else {
             const size_t part = (size_t)target * a.parts + a.part0 + split;
             if (d4 == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(top, l);
-            reinterpret_cast<float4*>(a.part_o + part * 64)[d4] = y;
+            if (top > KV8_REF_NONE || !(l == 0.f)) reinterpret_cast<float4*>(a.part_o + part * 64)[d4] = y;  // else not read
         }
     }
     if (a.beside) pdl_wait();
 }
 
-// Joins the parts of each (row, head): out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. A warp a
-// (row, head): 16 lanes cover the 64 dimensions, the two halves take alternate parts.
+// Joins the parts of each (row, head): out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. A block a
+// (row, head): 16 lanes cover the 64 dimensions, the 8 groups of 16 take parts in turn, so that some 60 parts
+// are two or three round trips to memory and not thirty.
 struct JoinArgs {
     Kv8Rows rows;
-    int total, hq, parts;  // total: requests * rows
+    int hq, parts;
     const float *part_o, *part_ml;
     float* out; int ldo; bool ovec;
 };
-constexpr int JOIN_THREADS = 128;
+constexpr int JOIN_THREADS = 128, JOIN_GROUPS = JOIN_THREADS / 16;
 
 __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const JoinArgs a) {
+    __shared__ float4 partial[JOIN_GROUPS][16];
+    __shared__ float2 total[JOIN_GROUPS];
     pdl_wait();
     pdl_launch();
-    const int lane = threadIdx.x & 31, half = lane >> 4, d4 = lane & 15;
-    const long long e = (long long)blockIdx.x * (JOIN_THREADS / 32) + (threadIdx.x >> 5);
-    if (e >= (long long)a.total * a.hq) return;
-    const int row = (int)(e / a.hq), head = (int)(e - (long long)row * a.hq);
-    const int request = row / a.rows.rows;
+    const int group = threadIdx.x >> 4, d4 = threadIdx.x & 15;
+    const int row = blockIdx.x / a.hq, request = row / a.rows.rows;
     if (row - request * a.rows.rows >= kv8_span(a.rows, request).count) return;
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + e * a.parts;
-    const float4* po = reinterpret_cast<const float4*>(a.part_o + e * a.parts * 64);
-    float top = KV8_REF_NONE;
-    for (int s = lane; s < a.parts; s += 32) top = fmaxf(top, ml[s].x);
-    top = warp_max(top);
-    float l = 0.f;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)blockIdx.x * a.parts;
+    const float4* po = reinterpret_cast<const float4*>(a.part_o) + (size_t)blockIdx.x * a.parts * 16 + d4;
+    float top = KV8_REF_NONE, l = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int s = half; s < a.parts; s += 2) {
+    for (int s = group; s < a.parts; s += JOIN_GROUPS) {
         const float2 p = ml[s];
-        const float4 v = po[(size_t)s * 16 + d4];
+        const bool any = !(p.y == 0.f);  // a part without a key has no sums
+        const float4 v = any ? po[(size_t)s * 16] : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float now = any ? fmaxf(top, p.x) : top, f = ex2(top - now), n = any ? ex2(p.x - now) : 0.f;
+        top = now;
+        l = l * f + (any ? n * p.y : 0.f);
+        y.x = y.x * f + n * v.x; y.y = y.y * f + n * v.y; y.z = y.z * f + n * v.z; y.w = y.w * f + n * v.w;
+    }
+    partial[group][d4] = y;
+    if (d4 == 0) total[group] = make_float2(top, l);
+    __syncthreads();
+    if (group > 0) return;
+    const int groups = min(a.parts, JOIN_GROUPS);
+    for (int s = 0; s < groups; s++) top = fmaxf(top, total[s].x);
+    l = 0.f;
+    y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < groups; s++) {
+        const float2 p = total[s];
+        const float4 v = partial[s][d4];
         const float f = ex2(p.x - top);
         l += f * p.y;
         y.x += f * v.x; y.y += f * v.y; y.z += f * v.z; y.w += f * v.w;
     }
-    l += __shfl_xor_sync(0xffffffffu, l, 16);
-    y.x += __shfl_xor_sync(0xffffffffu, y.x, 16);
-    y.y += __shfl_xor_sync(0xffffffffu, y.y, 16);
-    y.z += __shfl_xor_sync(0xffffffffu, y.z, 16);
-    y.w += __shfl_xor_sync(0xffffffffu, y.w, 16);
-    if (half) return;
     const float n = 1.f / l;
-    float* dst = a.out + (size_t)row * a.ldo + (size_t)head * 64 + 4 * d4;
+    float* dst = a.out + (size_t)row * a.ldo + (size_t)(blockIdx.x - row * a.hq) * 64 + 4 * d4;
     y.x *= n; y.y *= n; y.z *= n; y.w *= n;
     if (a.ovec) {
         *reinterpret_cast<float4*>(dst) = y;
@@ -453,9 +478,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const JoinArgs a
 }
 
 Kv8View view(const mt_kv8_cache* c) {
-    const bool quads = (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 15u) == 0 && c->capacity % 4 == 0 &&
-                       c->request_stride % 4 == 0;
-    return Kv8View{c->k, c->v, c->k_scale, c->v_scale, c->request_stride, c->capacity, c->kind, quads};
+    return Kv8View{c->k, c->v, c->k_scale, c->v_scale, c->request_stride, c->capacity, c->kind};
 }
 
 // How a pass is laid out over the GPU.
@@ -464,24 +487,34 @@ struct PassPlan {
     int nt, units, row_blocks, key_warps, splits, chunk;
 };
 
-constexpr int WIDE_FROM = 97;
-
 // `units` row spaces of `qrows` (row, head) rows each over at most `keys` keys.
 PassPlan plan_pass(int sm_count, long long units, long long qrows, int keys) {
     PassPlan p{};
     if (units < 1) return p;
-    if (qrows >= WIDE_FROM) {
-        p.wide = true;
-        p.units = (int)units;
-        p.row_blocks = (int)((qrows + KV8_WIDE_ROWS - 1) / KV8_WIDE_ROWS);
-        const int tiles = (keys + 15 + KV8_WIDE_KEYS - 1) / KV8_WIDE_KEYS;
-        const long long blocks = units * p.row_blocks;
+    // Which kernel: by their estimated times, in ns. The warp kernel takes 5.5 ps a (row, head) pair and key
+    // once the GPU is full; a wide block takes 14 us to start and finish and 2.2 us for 64 keys, and a later
+    // one on the same SM another 8 us. Measured in us, wide against warp kernel (one request, 14 heads on 2
+    // unless said): 16 rows over 300 keys 15.7 / 6.3, 512 over themselves 24.4 / 24.9, 37 over 4000 keys
+    // 23.5 / 20.8, 64 over 4000 23.9 / 32.7, 256 over 4000 29 / 74; 64 requests of 8 rows over 400 keys
+    // 18.8 / 18.1, of 16 rows 19.1 / 40.5; prefixes of 8000 for 16 requests 20.6 / 21.2, for 64 31.0 / 46.6.
+    {
+        const long long row_blocks = (qrows + KV8_WIDE_ROWS - 1) / KV8_WIDE_ROWS, blocks = units * row_blocks;
+        const long long tiles = (keys + 15 + KV8_WIDE_KEYS - 1) / KV8_WIDE_KEYS;
         long long s = sm_count / blocks;
         if (s > tiles / 4) s = tiles / 4;
         if (s < 1) s = 1;
-        p.chunk = (int)((tiles + s - 1) / s);
-        p.splits = (tiles + p.chunk - 1) / p.chunk;
-        return p;
+        const long long chunk = (tiles + s - 1) / s, waves = (blocks * s + sm_count - 1) / sm_count;
+        const long long each = blocks * tiles / sm_count;
+        const double wide = 14e3 + 8e3 * (double)(waves - 1) + 2.2e3 * (double)(each > chunk ? each : chunk);
+        const double warp = 6e3 + 5.5e-3 * (double)units * (double)qrows * (double)keys;
+        if (wide < warp) {
+            p.wide = true;
+            p.units = (int)units;
+            p.row_blocks = (int)row_blocks;
+            p.chunk = (int)chunk;
+            p.splits = (int)((tiles + chunk - 1) / chunk);
+            return p;
+        }
     }
     const int key_tiles = (keys + 15) / 16 + 1;
     const long long warps_fit = 16ll * sm_count;
@@ -499,8 +532,8 @@ PassPlan plan_pass(int sm_count, long long units, long long qrows, int keys) {
     p.units = (int)units;
     const long long blocks = blocks_at(p.key_warps);
     p.row_blocks = (int)(blocks / units);
-    // Split the keys over blocks while there are SMs without one and every warp keeps 4 tiles.
-    long long s = (2ll * sm_count + blocks - 1) / blocks;
+    // Split the keys over as many blocks as are resident at once, while every warp keeps 4 tiles.
+    long long s = 2ll * sm_count / blocks;
     const long long most = key_tiles / (4 * p.key_warps);
     if (s > most) s = most;
     p.splits = s < 1 ? 1 : (int)s;
@@ -535,8 +568,9 @@ Plan make_plan(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int
 template <int KIND, int NT>
 void launch_pass_as(const PassArgs& a, cudaStream_t s) {
     using R = Rows<NT>;
-    const size_t smem = (size_t)R::WARPS * R::COUNT * (64 + 2 + 1) * sizeof(float);
-    launch_k(kv8_pass_kernel<KIND, NT>, dim3((unsigned)(a.units * a.row_blocks * a.splits)), R::WARPS * 32, smem, s, a);
+    static PerDeviceOnce once;
+    once([] { cudaFuncSetAttribute(kv8_pass_kernel<KIND, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM); });
+    launch_k(kv8_pass_kernel<KIND, NT>, dim3((unsigned)(a.units * a.row_blocks * a.splits)), R::WARPS * 32, R::SMEM, s, a);
 }
 
 void launch_pass(const PassArgs& a, int nt, cudaStream_t s) {
@@ -590,9 +624,8 @@ mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q,
     a.beside = prefix_len > 0;
     run(plan.own);
     if (plan.parts > 1) {
-        JoinArgs j{a.rows, requests * rows, hq, plan.parts, a.part_o, a.part_ml, out, ldo, a.ovec};
-        const long long n = (long long)requests * rows * hq;
-        launch_k(kv8_join_kernel, dim3((unsigned)((n + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32))), JOIN_THREADS, 0, s, j);
+        const JoinArgs j{a.rows, hq, plan.parts, a.part_o, a.part_ml, out, ldo, a.ovec};
+        launch_k(kv8_join_kernel, dim3((unsigned)((long long)requests * rows * hq)), JOIN_THREADS, 0, s, j);
     }
     return check_launch(ctx, what);
 }

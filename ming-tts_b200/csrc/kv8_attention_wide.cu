@@ -45,10 +45,6 @@ constexpr int WD_STAGES = 4;
 constexpr int WD_PLANE = 128 * 128;      // bytes of a plane of a row tile's queries
 constexpr size_t WD_SMEM = 2 * WD_STAGES * WD_STAGE + 4 * WD_PLANE + 1024;
 constexpr uint32_t T_O = 128, T_TILE = 256;
-constexpr int WD_LIFT_TO = 0;         // exponent that a row's largest scaled product is brought to ..
-constexpr float WD_PRODUCT_MAX = 32768.f;  // .. once one is above this (fp16 ends at 65504)
-constexpr float WD_WEIGHT_MAX = 0x1p100f;  // what a sum of four weights may be in units of 2^off
-
 // 16 lanes x 16 columns of TMEM to and from 8 registers: fp32 (register 4 n + 2 slot + i is column 8 n + 2 t
 // + i of row g + 8 slot) or fp16 pairs (register 2 n + slot is column 4 n + t). A load's registers are
 // operands of the wait for it, so that nothing uses them before.
@@ -130,11 +126,8 @@ struct Shared {
     int abort;
 };
 
-// The state of a lane's two rows. Weights are 2^(score - off), off = reference - lift: the reference is
-// near a score that was the row's largest, the lift brings the largest weight times value scale to 2^8,
-// where the planes have 22 bits for weights down to 2^-20 of it. The sums and outputs are in units of
-// 2^off; a sum is the lane's own part of the row.
-constexpr float WD_UNSET = 1000.f;  // the lift of a row that has no unit yet (its off is 0)
+// The state of a lane's two rows. Sums and outputs are in units of 2^off (see kv8_unit); a sum is the lane's
+// own part of the row.
 struct RowState {
     float off[2], lift[2], rs[2];  // rs: scores in powers of two are TMEM value x key scale x rs
     int lo[2], hi[2];              // keys that the row sees
@@ -230,7 +223,7 @@ __device__ __forceinline__ int row_weights(uint32_t tm, const TileKeys& t, RowSt
         tmem_ld_tile(tm + 16 * c, s);
         tmem_ld_wait(s);
         const float top = row_products<false>(t, row, c, s, planes, add);
-        if (__any_sync(0xffffffffu, !(top <= WD_PRODUCT_MAX && add[0] <= WD_WEIGHT_MAX && add[1] <= WD_WEIGHT_MAX))) break;
+        if (__any_sync(0xffffffffu, !(top <= KV8_PRODUCT_MAX && add[0] <= KV8_WEIGHT_MAX && add[1] <= KV8_WEIGHT_MAX))) break;
         row.sum[0] += add[0];
         row.sum[1] += add[1];
         tmem_st_planes(tm + 16 * c, planes);
@@ -252,44 +245,27 @@ __device__ __forceinline__ void row_weights_slowly(uint32_t tm, const TileKeys& 
 #pragma unroll 1
         for (int tries = 0; tries < 2; tries++) {
             const float top = row_products<true>(t, row, c, s, planes, add);
-            if (!row.fresh && !__any_sync(0xffffffffu, !(top <= WD_PRODUCT_MAX && add[0] <= WD_WEIGHT_MAX && add[1] <= WD_WEIGHT_MAX))) break;
+            if (!row.fresh && !__any_sync(0xffffffffu, !(top <= KV8_PRODUCT_MAX && add[0] <= KV8_WEIGHT_MAX && add[1] <= KV8_WEIGHT_MAX))) break;
             settle(1);
             float f[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                float z[4], v[4], most = -INFINITY;
+                float z[4], v[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int key = 16 * c + 8 * (j >> 1) + (j & 1);
                     const bool on = t.u + key >= row.lo[i] && t.u + key <= row.hi[i];
                     z[j] = on ? s[4 * (j >> 1) + 2 * i + (j & 1)] * t.ks[key] * row.rs[i] : -INFINITY;
                     v[j] = on ? fabsf(t.vs[key]) : 0.f;
-                    most = fmaxf(most, z[j]);
                 }
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                auto product = [&](float from) {  // the row's largest in these keys, in units of 2^from
-                    float x = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) x = fmaxf(x, ex2(z[j] - from) * v[j]);
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                    return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                };
-                float off = row.off[i], lift = row.lift[i];
-                const bool unset = lift == WD_UNSET;
-                const float now = product(off);
-                if (most > -INFINITY && (unset || most - off > 90.f || now > WD_PRODUCT_MAX)) off = unset ? most : fmaxf(off + lift, most);
-                const float then = product(off);
-                if (off != row.off[i] || now > WD_PRODUCT_MAX || (unset && most > -INFINITY)) {
-                    lift = then > 0.f ? fminf(80.f, fmaxf(-100.f, (float)(WD_LIFT_TO + 127 - (int)(__float_as_uint(then) >> 23)))) : 0.f;
-                    off -= lift;
-                }
-                f[i] = row.lift[i] == WD_UNSET ? 1.f : ex2(row.off[i] - off);
+                const float2 to = kv8_unit(z, v, row.off[i], row.lift[i]);
+                const float off = to.x, lift = to.y;
+                f[i] = row.lift[i] == KV8_UNSET ? 1.f : ex2(row.off[i] - off);
                 if (off != row.off[i]) row.scale(i, f[i]);
                 row.off[i] = off;
                 row.lift[i] = lift;
             }
-            row.fresh = __any_sync(0xffffffffu, row.lift[0] == WD_UNSET || row.lift[1] == WD_UNSET);
+            row.fresh = __any_sync(0xffffffffu, row.lift[0] == KV8_UNSET || row.lift[1] == KV8_UNSET);
             row_rescale(tm, c, f[0], f[1]);
         }
         row.sum[0] += add[0];
@@ -417,7 +393,7 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
                     // up is a power of two within 2^+-126: so is its reciprocal
                     row.rs[i] = 0.125f * 1.4426950408889634f * __uint_as_float(0x7F000000u - __float_as_uint(up[i]));
                     row.off[i] = 0.f;
-                    row.lift[i] = WD_UNSET;
+                    row.lift[i] = KV8_UNSET;
                     row.sum[i] = 0.f;
                 }
                 row.fresh = true;
@@ -474,7 +450,7 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
                     s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
                     s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
                     if (target[i] < 0) continue;
-                    const float lift = row.lift[i] == WD_UNSET ? 0.f : row.lift[i], down = ex2(-lift), total = s0 * down;
+                    const float lift = row.lift[i] == KV8_UNSET ? 0.f : row.lift[i], down = ex2(-lift), total = s0 * down;
                     float f = sh.unit * down;
                     float* dst;
                     bool vec = true;
