@@ -53,21 +53,45 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool l1) {
 // codes that are NaN, which a weight of zero would not silence. Value rows are placed so that the reads
 // below (4 rows 256 bytes apart, 8 bytes each of 4 places) touch every bank once: odd groups of four rows
 // have their rows swapped in pairs, the last eight rows their halves.
-__device__ __forceinline__ void copy_keys(uint32_t to, const Kv8View& c, const KeyRange& r, int u0, int lane, bool l1) {
-    const int part = lane & 3, key = lane & 15;
-    const float* const scales = lane < 16 ? c.ks : c.vs;
-    const bool whole = r.whole(u0, 16);
-    const size_t first = r.row + (u0 >= r.capacity ? u0 - r.capacity : u0);
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-        const int row = 8 * j + (lane >> 2);
-        const size_t from = (whole ? first + row : r.slot(u0 + row)) * 64 + 16 * part;
-        copy16(to + row * 64 + 16 * part, c.k + from, l1);
-        copy16(to + 1024 + (row ^ ((row >> 2) & 1)) * 64 + 16 * (part ^ (2 * j)), c.v + from, l1);
+struct KeyCopy {
+    const uint8_t *k, *v;  // this lane's first: row lane / 4, 16 bytes at lane % 4
+    const float* scale;    // key lane % 16, of the keys (lanes 0-15) or values
+    uint32_t to_k, to_v, to_scale;
+    bool l1;
+
+    __device__ __forceinline__ KeyCopy(const Kv8View& c, const KeyRange& r, uint32_t ring, int lane, bool l1_) : l1(l1_) {
+        const int part = lane & 3, row = lane >> 2;
+        k = c.k + (r.row + row) * 64 + 16 * part;
+        v = c.v + (r.row + row) * 64 + 16 * part;
+        scale = (lane < 16 ? c.ks : c.vs) + r.row + (lane & 15);
+        to_k = ring + row * 64 + 16 * part;
+        to_v = ring + 1024 + (row ^ ((row >> 2) & 1)) * 64 + 16 * part;
+        to_scale = ring + 2048 + 4 * lane;
     }
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 2048 + 4 * lane), "l"(scales + (whole ? first + key : r.slot(u0 + key)))
-                 : "memory");
-}
+    __device__ __forceinline__ void tile(const KeyRange& r, int u0, int stage, int lane) const {
+        const uint32_t at = stage * TILE_BYTES;
+        int slot[2], key;  // less the lane's own row
+        if (r.whole(u0, 16)) {
+            slot[0] = u0 >= r.capacity ? u0 - r.capacity : u0;
+            slot[1] = slot[0] + 8;
+            key = slot[0];
+        } else {
+            auto nearest = [&](int n) {
+                const int u = min(max(u0 + n, r.lo), r.hi);
+                return (u >= r.capacity ? u - r.capacity : u) - n;
+            };
+            slot[0] = nearest(lane >> 2);
+            slot[1] = nearest((lane >> 2) + 8) + 8;
+            key = nearest(lane & 15);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            copy16(to_k + at + 512 * j, k + (long long)slot[j] * 64, l1);
+            copy16((to_v ^ (32 * j)) + at + 512 * j, v + (long long)slot[j] * 64, l1);
+        }
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to_scale + at), "l"(scale + key) : "memory");
+    }
+};
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -167,10 +191,10 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
     if (at < end) {
         const bool l1 = a.key_warps == 1;  // the block's warps read the same keys
         const uint8_t* const ring = reinterpret_cast<const uint8_t*>(smem) + R::SUM_BYTES + warp * RING * TILE_BYTES;
-        const uint32_t ring_at = smem_u32(ring);
+        const KeyCopy copy(a.c, r, smem_u32(ring), lane, l1);
 #pragma unroll
         for (int i = 0; i < RING - 1; i++) {
-            if (at + i * a.key_warps < end) copy_keys(ring_at + i * TILE_BYTES, a.c, r, (t0 + at + i * a.key_warps) * 16, lane, l1);
+            if (at + i * a.key_warps < end) copy.tile(r, (t0 + at + i * a.key_warps) * 16, i, lane);
             copies_commit();
         }
         // Queries: 16 dimensions of each of the lane's rows, as fp16 planes of a power-of-two multiple.
@@ -228,7 +252,7 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
             const int u0 = (t0 + at) * 16;
             __syncwarp();  // every lane has read the tile that is copied over
             if (at + (RING - 1) * a.key_warps < end)
-                copy_keys(ring_at + ((stage + RING - 1) & (RING - 1)) * TILE_BYTES, a.c, r, u0 + 16 * (RING - 1) * a.key_warps, lane, l1);
+                copy.tile(r, u0 + 16 * (RING - 1) * a.key_warps, (stage + RING - 1) & (RING - 1), lane);
             copies_commit();
             copies_wait<RING - 1>();
             __syncwarp();
