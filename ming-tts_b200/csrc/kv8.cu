@@ -35,6 +35,7 @@ namespace {
 
 constexpr int AP_THREADS = 256;
 constexpr int AP_MAX_ROWS = 8;  // rows of a block: their 32 angles each are one per thread
+constexpr int AP_HEADS = 4;     // query heads of a group in flight (of 14, when 8 rows leave a row 4 groups)
 
 struct AppendArgs {
     const float* qkv; int ldq;
@@ -43,6 +44,7 @@ struct AppendArgs {
     int total;           // requests * rows
     int hq, hkv;
     int block_rows;      // rows per block, <= AP_MAX_ROWS
+    int parts;           // groups of 8 lanes per row
     bool vec;            // 16-byte loads and stores of the fp32 rows
     const float* inv_freq;
     uint8_t *k, *v;
@@ -63,112 +65,142 @@ __device__ __forceinline__ void store4(float* p, float4 x, bool vec) {
     }
 }
 
-// x / scale as a float that rounds to a coarser grid as the exact quotient does: the rounded quotient,
-// moved by one unit to the neighbour with an odd last bit where the division left a remainder. No
-// coarser value and no border between two such values is odd, so a second rounding cannot be caught
-// on a tie that the first one made.
-__device__ __forceinline__ float quotient_odd(float x, float scale) {
-    const float q = __fdiv_rn(x, scale);
-    const float rest = fmaf(-q, scale, x);  // exact: its sign is the remainder's
-    const uint32_t u = __float_as_uint(q);
-    if (rest == 0.f || (u & 1u)) return q;
-    return __uint_as_float((rest > 0.f) == (x > 0.f) ? u + 1u : u - 1u);
-}
-
+// Codes of four values: x / scale, whose exact quotient is rounded once, to the nearest code, ties to
+// even. The product with the rounded reciprocal is off by a unit or two of fp32, which only matters
+// next to a border between two codes; the remainder there, from one multiply-add, is exact and decides.
+// int8: c is the nearest whole number (the sum with 1.5 * 2^23 has it in its low bits) or its neighbour,
+//   and d = x - c scale is a multiple of half a unit of scale below 2^24 of them. 2|d| against scale says
+//   whether c has to take a step towards x; at a tie an odd c takes it.
+// e4m3: t is the quotient to 12 bits. Codes and borders between them have 5 bits or fewer, so where the
+//   quotient is next to one, t is that one; d = x - t scale has the exact sign of the difference, and t
+//   moves by its own last bit to that side. The conversion cannot be caught on a tie after that.
+// Scales below 2^-60 are taken 2^64 higher, with x, so that no d is lost below the smallest number.
 template <int KIND>
-__device__ __forceinline__ uint32_t encode4(float4 x, float scale) {
-    const float a = quotient_odd(x.x, scale), b = quotient_odd(x.y, scale), c = quotient_odd(x.z, scale),
-                d = quotient_odd(x.w, scale);
-    if (KIND == MT_KV_INT8) {
-        auto code = [](float q) { return (uint32_t)(uint8_t)(int8_t)min(127, max(-127, __float2int_rn(q))); };
-        return code(a) | code(b) << 8 | code(c) << 16 | code(d) << 24;
+__device__ __forceinline__ uint32_t encode4(float4 x4, float scale, float rcp) {
+    const float x[4] = {x4.x, x4.y, x4.z, x4.w};
+    uint32_t code[4];
+    if constexpr (KIND == MT_KV_INT8) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float m = fmaf(x[i], rcp, 12582912.f), c = m - 12582912.f;
+            const float d = fmaf(-c, scale, x[i]), twice = fabsf(d) + fabsf(d);
+            const uint32_t u = __float_as_uint(m);
+            const bool step = twice > scale || (twice == scale && (u & 1u));
+            code[i] = step ? u + (d < 0.f ? ~0u : 1u) : u;
+        }
+        return __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t t = (__float_as_uint(x[i] * rcp) + 0x800u) & 0xFFFFF000u;
+            const float d = fmaf(-__uint_as_float(t), scale, x[i]);
+            const uint32_t away = (uint32_t)((int)(__float_as_uint(d) ^ t) >> 31) | 1u;  // 1: |x / scale| > |t|, else -1
+            code[i] = d == 0.f ? t : t + away;
+        }
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(code[0]), __uint_as_float(code[1])), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(code[2]), __uint_as_float(code[3])), __NV_SATFINITE, __NV_E4M3);
+        return lo | hi << 16;
     }
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-    return lo | hi << 16;
 }
 
-// RoPE, quantisation and the cache write. A block takes block_rows rows: first their angles, one
-// thread each, in 64 bits (a position of 10^5 leaves an fp32 angle with 2 digits less, and a code is
-// the same for every caller only if the rotated key is: rounding it once from 64 bits makes it so),
-// then every head: 8 lanes a head, lane j the pairs (4j .. 4j+3, +32), so that loads and stores of
-// a head are whole 128-byte lines and a code row is 16 words.
+// RoPE, quantisation and the cache write. A block takes block_rows rows; 8 lanes are a group, which has
+// one row and every parts-th of its heads; lane j has the pairs (4j .. 4j+3, +32), so that loads and
+// stores of a head are whole 128-byte lines and a code row is 16 words. The angles are made in 64 bits,
+// one thread each (a position of 10^5 leaves an fp32 angle with 2 digits less, and a code is the same for
+// every caller only if the rotated key is: rounding it once from 64 bits makes it so), while the loads of
+// the group's first heads are under way. Queries are turned in 32 bits.
 template <int KIND>
-__global__ void __launch_bounds__(AP_THREADS) rope_cache_kv8_kernel(AppendArgs a) {
-    __shared__ double turn[AP_MAX_ROWS][2][32];  // cos, sin
-    __shared__ int place[AP_MAX_ROWS];           // slot, or -1: padding
-    __shared__ int owner[AP_MAX_ROWS];           // request
-    pdl_wait();
-    pdl_launch();
+__global__ void __launch_bounds__(AP_THREADS, 3) rope_cache_kv8_kernel(const AppendArgs a) {
+    __shared__ __align__(16) double turn[AP_MAX_ROWS][2][32];  // cos, sin
+    __shared__ __align__(16) float turn_f[AP_MAX_ROWS][2][32];
+    const int j = threadIdx.x & 7, group = threadIdx.x >> 3;
     const int row0 = blockIdx.x * a.block_rows;
     const int n = min(a.block_rows, a.total - row0);
-    if (threadIdx.x < n * 32) {
-        const int i = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        const int request = (row0 + i) / a.rows.rows, at = (row0 + i) - request * a.rows.rows;
-        const Kv8Span s = kv8_span(a.rows, request);
-        const bool live = at < s.count;
-        if (lane == 0) {
-            place[i] = live ? (s.pos + at - a.rows.base) % a.capacity : -1;
-            owner[i] = request;
-        }
-        if (live) {
-            double sn, cs;
-            sincos((double)(s.pos + at) * (double)a.inv_freq[lane], &sn, &cs);
-            turn[i][0][lane] = cs;
-            turn[i][1][lane] = sn;
+    const int i = group / a.parts, part = group - i * a.parts;
+    const int request = (row0 + i) / a.rows.rows, at = (row0 + i) - request * a.rows.rows;
+    pdl_wait();
+    pdl_launch();
+    const Kv8Span s = kv8_span(a.rows, i < n ? request : 0);
+    const bool on = i < n && at < s.count;
+    const float* src = a.qkv + (size_t)(row0 + i) * a.ldq + 4 * j;
+    const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto load = [&](float4 (&x)[2], int head, int end) {
+        const bool here = on && head < end;
+        x[0] = here ? load4(src + (size_t)head * 64, a.vec) : none;
+        x[1] = here ? load4(src + (size_t)head * 64 + 32, a.vec) : none;
+    };
+    float4 c[2], q[AP_HEADS][2];
+    load(c, a.hq + part, a.hq + 2 * a.hkv);
+#pragma unroll
+    for (int h = 0; h < AP_HEADS; h++) load(q[h], part + h * a.parts, a.hq);
+
+    {
+        const int row = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        const int request_r = (row0 + row) / a.rows.rows, at_r = (row0 + row) - request_r * a.rows.rows;
+        if (row < n) {
+            const Kv8Span r = kv8_span(a.rows, request_r);
+            if (at_r < r.count) {
+                double sn, cs;
+                sincos((double)(r.pos + at_r) * (double)a.inv_freq[lane], &sn, &cs);
+                turn[row][0][lane] = cs;
+                turn[row][1][lane] = sn;
+                turn_f[row][0][lane] = (float)cs;
+                turn_f[row][1][lane] = (float)sn;
+            }
         }
     }
     __syncthreads();
-    const int vecs = a.hq + 2 * a.hkv;
-    const int j = threadIdx.x & 7;
-    // Whole warps run every iteration (the scale is a maximum over 8 lanes).
-    for (int u = threadIdx.x >> 3; u < ((n * vecs + 3) & ~3); u += AP_THREADS / 8) {
-        const int i = min(u / vecs, n - 1), head = u - (u / vecs) * vecs;
-        const int slot = place[i];
-        const bool on = u < n * vecs && slot >= 0;
-        const float* src = a.qkv + (size_t)(row0 + i) * a.ldq + (size_t)head * 64 + 4 * j;
-        float4 x0 = make_float4(0.f, 0.f, 0.f, 0.f), x1 = x0;
-        if (on) {
-            x0 = load4(src, a.vec);
-            x1 = load4(src + 32, a.vec);
+
+    if (on) {
+        const float4 cs = *reinterpret_cast<const float4*>(&turn_f[i][0][4 * j]);
+        const float4 sn = *reinterpret_cast<const float4*>(&turn_f[i][1][4 * j]);
+        float* dst = a.q_out + (size_t)(row0 + i) * a.ldqo + 4 * j;
+        for (int h0 = part; h0 < a.hq; h0 += AP_HEADS * a.parts) {
+#pragma unroll
+            for (int h = 0; h < AP_HEADS; h++) {
+                const int head = h0 + h * a.parts;
+                if (head >= a.hq) break;
+                const float4 x = q[h][0], y = q[h][1];
+                store4(dst + (size_t)head * 64, make_float4(x.x * cs.x - y.x * sn.x, x.y * cs.y - y.y * sn.y,
+                                                            x.z * cs.z - y.z * sn.z, x.w * cs.w - y.w * sn.w), a.vec);
+                store4(dst + (size_t)head * 64 + 32, make_float4(y.x * cs.x + x.x * sn.x, y.y * cs.y + x.y * sn.y,
+                                                                 y.z * cs.z + x.z * sn.z, y.w * cs.w + x.w * sn.w), a.vec);
+            }
+            if (h0 + AP_HEADS * a.parts < a.hq) {
+#pragma unroll
+                for (int h = 0; h < AP_HEADS; h++) load(q[h], h0 + (AP_HEADS + h) * a.parts, a.hq);
+            }
         }
-        if (on && head < a.hq + a.hkv) {
+    }
+    // Whole warps run every iteration (the scale is a maximum over 8 lanes).
+    const int slot = on ? (s.pos + at - a.rows.base) % a.capacity : 0;
+    for (int u0 = 0; u0 < 2 * a.hkv; u0 += a.parts) {
+        const int unit = u0 + part;
+        const bool here = on && unit < 2 * a.hkv, value = unit >= a.hkv;
+        if (u0 > 0) load(c, a.hq + unit, a.hq + 2 * a.hkv);
+        float4 x = c[0], y = c[1];
+        if (here && !value) {
             const double2* cs = reinterpret_cast<const double2*>(&turn[i][0][4 * j]);
             const double2* sn = reinterpret_cast<const double2*>(&turn[i][1][4 * j]);
             const double2 c0 = cs[0], c1 = cs[1], s0 = sn[0], s1 = sn[1];
-            if (head < a.hq) {  // queries: 32-bit products of the exact angle's cosine and sine
-                auto rot = [](float& p, float& q, double c, double s) {
-                    const float cf = (float)c, sf = (float)s, r = p * cf - q * sf;
-                    q = q * cf + p * sf;
-                    p = r;
-                };
-                rot(x0.x, x1.x, c0.x, s0.x); rot(x0.y, x1.y, c0.y, s0.y);
-                rot(x0.z, x1.z, c1.x, s1.x); rot(x0.w, x1.w, c1.y, s1.y);
-                float* dst = a.q_out + (size_t)(row0 + i) * a.ldqo + (size_t)head * 64 + 4 * j;
-                store4(dst, x0, a.vec);
-                store4(dst + 32, x1, a.vec);
-            } else {
-                auto rot = [](float& p, float& q, double c, double s) {
-                    const double pd = p, qd = q;
-                    p = (float)(pd * c - qd * s);
-                    q = (float)(qd * c + pd * s);
-                };
-                rot(x0.x, x1.x, c0.x, s0.x); rot(x0.y, x1.y, c0.y, s0.y);
-                rot(x0.z, x1.z, c1.x, s1.x); rot(x0.w, x1.w, c1.y, s1.y);
-            }
+            auto rot = [](float& p, float& q, double c, double s) {
+                const double pd = p, qd = q;
+                p = (float)(pd * c - qd * s);
+                q = (float)(qd * c + pd * s);
+            };
+            rot(x.x, y.x, c0.x, s0.x); rot(x.y, y.y, c0.y, s0.y);
+            rot(x.z, y.z, c1.x, s1.x); rot(x.w, y.w, c1.y, s1.y);
         }
         // max|x| over the head's 8 lanes as bit patterns: those of NaN and infinity are the largest.
-        const float m0 = fmaxf(fmaxf(fabsf(x0.x), fabsf(x0.y)), fmaxf(fabsf(x0.z), fabsf(x0.w)));
-        const float m1 = fmaxf(fmaxf(fabsf(x1.x), fabsf(x1.y)), fmaxf(fabsf(x1.z), fabsf(x1.w)));
-        const float sum = fabsf(x0.x) + fabsf(x0.y) + fabsf(x0.z) + fabsf(x0.w) + fabsf(x1.x) + fabsf(x1.y) +
-                          fabsf(x1.z) + fabsf(x1.w);  // NaN if any is (fmaxf drops NaN)
+        const float m0 = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+        const float m1 = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
+        const float sum = fabsf(x.x) + fabsf(x.y) + fabsf(x.z) + fabsf(x.w) + fabsf(y.x) + fabsf(y.y) + fabsf(y.z) +
+                          fabsf(y.w);  // NaN if any is (fmaxf drops NaN)
         uint32_t top = sum != sum ? 0x7FFFFFFFu : __float_as_uint(fmaxf(m0, m1));
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (!on || head < a.hq) continue;
-        const bool value = head >= a.hq + a.hkv;
-        const int kh = head - a.hq - (value ? a.hkv : 0);
-        const size_t at = (size_t)owner[i] * a.request_stride + (size_t)kh * a.capacity + slot;
+        if (!here) continue;
+        const size_t to = (size_t)request * a.request_stride + (size_t)(value ? unit - a.hkv : unit) * a.capacity + slot;
         float scale = __fdiv_rn(__uint_as_float(top), KIND == MT_KV_INT8 ? 127.f : 448.f);
         uint32_t w0 = 0, w1 = 0;
         if (top >= 0x7F800000u) {
@@ -176,13 +208,21 @@ __global__ void __launch_bounds__(AP_THREADS) rope_cache_kv8_kernel(AppendArgs a
         } else if (scale < 1.17549435e-38f) {
             scale = 0.f;
         } else {
-            w0 = encode4<KIND>(x0, scale);
-            w1 = encode4<KIND>(x1, scale);
+            float by = scale;
+            if (scale < 8.67361738e-19f) {  // 2^-60
+                const float up = 1.8446744e19f;  // 2^64
+                by *= up;
+                x.x *= up; x.y *= up; x.z *= up; x.w *= up;
+                y.x *= up; y.y *= up; y.z *= up; y.w *= up;
+            }
+            const float rcp = __fdiv_rn(1.f, by);
+            w0 = encode4<KIND>(x, by, rcp);
+            w1 = encode4<KIND>(y, by, rcp);
         }
-        uint32_t* codes = reinterpret_cast<uint32_t*>((value ? a.v : a.k) + at * 64);
+        uint32_t* codes = reinterpret_cast<uint32_t*>((value ? a.v : a.k) + to * 64);
         codes[j] = w0;
         codes[8 + j] = w1;
-        if (j == 0) (value ? a.v_scale : a.k_scale)[at] = scale;
+        if (j == 0) (value ? a.v_scale : a.k_scale)[to] = scale;
     }
 }
 
@@ -276,6 +316,7 @@ extern "C" mt_status mt_rope_cache_kv8(mt_ctx* ctx, void* stream, const float* q
     // One row a block until the rows are two waves of blocks: a decode step is bound by its latency.
     const int per_sm = (a.total + 2 * ctx->sm_count - 1) / (2 * ctx->sm_count);
     a.block_rows = per_sm < AP_MAX_ROWS ? per_sm : AP_MAX_ROWS;
+    a.parts = AP_THREADS / 8 / a.block_rows;
     a.vec = (((uintptr_t)qkv | (uintptr_t)q_out) & 15u) == 0 && ldq % 4 == 0 && ldqo % 4 == 0;
     a.inv_freq = inv_freq;
     a.k = cache->k; a.v = cache->v; a.k_scale = cache->k_scale; a.v_scale = cache->v_scale;
