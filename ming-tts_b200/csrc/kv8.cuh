@@ -48,10 +48,13 @@ struct PassArgs {
     int requests, hq, hkv, group, window;
     Kv8View c;
     int prefix_len;                  // > 0: the prefix pass
-    int units, row_blocks, splits;   // grid: units x row_blocks x splits
+    int units, row_blocks, splits;   // grid: units x row_blocks x splits, or
+    int slots;                       // > 0: slots x kv heads x row_blocks, the slots shared out by length (kv8_share)
+    int2* shares;                    // per request: its first slot and their number, for the join
     int key_warps;                   // warps of a block that share a row tile and interleave its keys
-    float *part_o, *part_ml;         // parts: [row * hq + head][parts][64] and [..][parts][2] (reference, sum)
-    int parts, part0;                // parts of the whole call, and this pass's first
+    bool parted;                     // the outputs go to parts, for the join: 64 sums, and (reference, sum of weights)
+    float *part_o, *part_ml;         // [row * hq + head][splits], or request by request [pair][its slots]
+    size_t part0;                    // this pass's first
     // The pass before this one in the stream is the same call's other pass: they write different parts, so
     // this one runs beside it and waits for it at its end (every block of that pass has waited for what
     // came before the call, or this one would not have been launched).

@@ -120,19 +120,112 @@ struct Rows {
 
 constexpr int FOLD = 8;               // key tiles summed in the matrix unit's accumulators at a time
 
-template <int KIND, int NT>
+// The slots of a kv head (and row block) are shared out so that the longest walk is the shortest: requests
+// get ceil(rounds / q) each, with the smallest q that the slots allow, a round being a key tile for each of
+// the block's warps. Every block computes the same from all positions. With an equal number of slots each,
+// 8 requests of 4000 to 32000 keys took as long as 8 of 32000.
+constexpr int SHARE_LANES = 5;  // requests per lane at most
+struct Share {
+    int request, first, parts;  // parts 0: no request's slot
+};
+__device__ __forceinline__ Share share_of(const PassArgs& a, int slot, int lane) {
+    float rounds[SHARE_LANES];  // less a half: ceil(n / q) = floor((n - 1/2) / q) + 1, exact in fp32 up to 2^21
+    int total = 0, most = 0;
+#pragma unroll
+    for (int j = 0; j < SHARE_LANES; j++) {
+        rounds[j] = -1.f;
+        const int request = 32 * j + lane;
+        if (32 * j >= a.requests) break;
+        if (request < a.requests) {
+            const Kv8Span s = kv8_span(a.rows, request);
+            int keys = min(s.pos + s.count - a.rows.base, a.c.capacity);
+            if (a.window > 0) keys = min(keys, a.window + s.count - 1);
+            const int n = s.count > 0 ? (keys + 15 + 16 * a.key_warps) / (16 * a.key_warps) : 0;
+            rounds[j] = (float)n - 0.5f;
+            total += n;
+            most = max(most, n);
+        }
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    most = __reduce_max_sync(0xffffffffu, most);
+    auto parts = [&](int j, float one_over) { return rounds[j] < 0.f ? 0 : (int)(rounds[j] * one_over) + 1; };
+    // A part a request is allowed, and so is what leaves each request one slot to round up into.
+    int lo = max(2, (total + a.slots - 1) / a.slots);
+    int hi = max(lo, min(most, (total + a.slots - a.requests - 1) / (a.slots - a.requests)));
+#pragma unroll 1
+    for (int i = 0; i < 4 && lo < hi; i++) {
+        const int q = (lo + hi) >> 1;
+        const float one_over = __frcp_rn((float)q);
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < SHARE_LANES; j++) {
+            if (32 * j >= a.requests) break;
+            n += parts(j, one_over);
+        }
+        if (__reduce_add_sync(0xffffffffu, n) <= a.slots) hi = q;
+        else lo = q + 1;
+    }
+    const float one_over = __frcp_rn((float)hi);
+    Share mine{0, 0, 0};
+    int before = 0;
+#pragma unroll
+    for (int j = 0; j < SHARE_LANES; j++) {
+        if (32 * j >= a.requests) break;
+        const int n = parts(j, one_over);
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const uint32_t here = __ballot_sync(0xffffffffu, before + upto > slot && before + upto - n <= slot && n > 0);
+        if (here) {
+            const int from = __ffs(here) - 1;
+            mine.request = 32 * j + from;
+            mine.parts = __shfl_sync(0xffffffffu, n, from);
+            mine.first = before + __shfl_sync(0xffffffffu, upto, from) - mine.parts;
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return mine;
+}
+
+template <int KIND, int NT, bool SHARE>
 __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pass_kernel(const PassArgs a) {
     using R = Rows<NT>;
     constexpr int LR = R::LANE;
     // [warp][row][64] sums, [warp][row][2] reference and sum, [row] owner, [warp] ring
-    extern __shared__ __align__(16) float smem[];
+    extern __shared__ __align__(128) float smem[];  // KeyCopy places rows of the rings by their address bits
     if (!a.beside) pdl_wait();
     pdl_launch();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     // Blocks with the most keys (the last rows) first.
-    const int split = blockIdx.x % a.splits;
-    const int unit = (blockIdx.x / a.splits) % a.units;
-    const int row_block = a.row_blocks - 1 - blockIdx.x / (a.splits * a.units);
+    int split = blockIdx.x % a.splits, splits = a.splits;
+    int unit = (blockIdx.x / a.splits) % a.units;
+    int row_block = a.row_blocks - 1 - blockIdx.x / (a.splits * a.units);
+    long long part0 = a.part0;
+    if constexpr (SHARE) {
+        const int kvh = blockIdx.x % a.hkv;
+        row_block = blockIdx.x / a.hkv % a.row_blocks;
+        const int slot = blockIdx.x / (a.hkv * a.row_blocks);
+        __shared__ Share shared_share;
+        if (warp == 0) {
+            const Share found = share_of(a, slot, lane);
+            if (lane == 0) shared_share = found;
+        }
+        __syncthreads();
+        const Share share = shared_share;
+        if (share.parts == 0) {
+            if (a.beside) pdl_wait();
+            return;
+        }
+        if (threadIdx.x == 0) a.shares[share.request] = make_int2(share.first, share.parts);
+        unit = share.request * a.hkv + kvh;
+        split = slot - share.first;
+        splits = share.parts;
+        part0 += (share.first - (long long)share.request * splits) * a.rows.rows * a.hq;
+    }
     const int phase = warp % a.key_warps;
     const int tile = row_block * (R::WARPS / a.key_warps) + warp / a.key_warps;
     UnitRows rows(a, unit);
@@ -184,7 +277,7 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
     };
 
     const int t0 = r.lo >> 4, tiles = any_row ? (r.hi >> 4) - t0 + 1 : 0;
-    const int per = max((tiles + a.splits - 1) / a.splits, 2 * a.key_warps);  // a short request in fewer parts
+    const int per = max((tiles + splits - 1) / splits, 2 * a.key_warps);  // a short request in fewer parts
     const int end = min(tiles, (split + 1) * per);
     int at = split * per + phase;
     bool folded = false;
@@ -424,7 +517,7 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
             l += f * ml.y;
             y.x += f * v.x; y.y += f * v.y; y.z += f * v.z; y.w += f * v.w;
         }
-        if (a.parts == 1) {
+        if (!a.parted) {
             const int qrow = target / a.hq, head = target - qrow * a.hq;
             float* dst = a.out + (size_t)qrow * a.ldo + (size_t)head * 64 + 4 * d4;
             const float n = 1.f / l;
@@ -435,7 +528,7 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
                 dst[0] = y.x; dst[1] = y.y; dst[2] = y.z; dst[3] = y.w;
             }
         } else {
-            const size_t part = (size_t)target * a.parts + a.part0 + split;
+            const long long part = part0 + (long long)target * splits + split;
             if (d4 == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(top, l);
             if (top > KV8_REF_NONE || !(l == 0.f)) reinterpret_cast<float4*>(a.part_o + part * 64)[d4] = y;  // else not read
         }
@@ -448,7 +541,9 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
 // are two or three round trips to memory and not thirty.
 struct JoinArgs {
     Kv8Rows rows;
-    int hq, parts;
+    int hq, splits, prefix_splits;  // parts of a request's own pass (shares: by request) and of the prefix's
+    const int2* shares;
+    long long own0;                 // first part of the own pass, behind the prefix's
     const float *part_o, *part_ml;
     float* out; int ldo; bool ovec;
 };
@@ -462,15 +557,19 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const JoinArgs a
     const int group = threadIdx.x >> 4, d4 = threadIdx.x & 15;
     const int row = blockIdx.x / a.hq, request = row / a.rows.rows;
     if (row - request * a.rows.rows >= kv8_span(a.rows, request).count) return;
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)blockIdx.x * a.parts;
-    const float4* po = reinterpret_cast<const float4*>(a.part_o) + (size_t)blockIdx.x * a.parts * 16 + d4;
+    const int2 own = a.shares ? a.shares[request] : make_int2(request * a.splits, a.splits);
+    const int parts = a.prefix_splits + own.y;
+    const long long size = (long long)a.rows.rows * a.hq;
+    const long long prefix_at = (long long)blockIdx.x * a.prefix_splits;
+    const long long own_at = a.own0 + (own.x - (long long)request * own.y) * size + (long long)blockIdx.x * own.y - a.prefix_splits;
     float top = KV8_REF_NONE, l = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int s = group; s < a.parts; s += JOIN_GROUPS) {
-        const float2 p = ml[s];
+    for (int s = group; s < parts; s += JOIN_GROUPS) {
+        const long long at = (s < a.prefix_splits ? prefix_at : own_at) + s;
+        const float2 p = reinterpret_cast<const float2*>(a.part_ml)[at];
         const bool any = !(p.y == 0.f);  // a part without a key has no sums
-        const float4 v = any ? po[(size_t)s * 16] : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 v = any ? reinterpret_cast<const float4*>(a.part_o)[at * 16 + d4] : make_float4(0.f, 0.f, 0.f, 0.f);
         const float now = any ? fmaxf(top, p.x) : top, f = ex2(top - now), n = any ? ex2(p.x - now) : 0.f;
         top = now;
         l = l * f + (any ? n * p.y : 0.f);
@@ -480,7 +579,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const JoinArgs a
     if (d4 == 0) total[group] = make_float2(top, l);
     __syncthreads();
     if (group > 0) return;
-    const int groups = min(a.parts, JOIN_GROUPS);
+    const int groups = min(parts, JOIN_GROUPS);
     for (int s = 0; s < groups; s++) top = fmaxf(top, total[s].x);
     l = 0.f;
     y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -508,11 +607,12 @@ Kv8View view(const mt_kv8_cache* c) {
 // How a pass is laid out over the GPU.
 struct PassPlan {
     bool wide;
-    int nt, units, row_blocks, key_warps, splits, chunk;
+    int nt, units, row_blocks, key_warps, splits, chunk, slots;
 };
 
-// `units` row spaces of `qrows` (row, head) rows each over at most `keys` keys.
-PassPlan plan_pass(int sm_count, long long units, long long qrows, int keys) {
+// `units` row spaces of `qrows` (row, head) rows each over at most `keys` keys, `requests` of them of
+// lengths that may differ.
+PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows, int keys) {
     PassPlan p{};
     if (units < 1) return p;
     // Which kernel: by their estimated times, in ns. The warp kernel takes 5.5 ps a (row, head) pair and key
@@ -561,13 +661,19 @@ PassPlan plan_pass(int sm_count, long long units, long long qrows, int keys) {
     const long long most = key_tiles / (4 * p.key_warps);
     if (s > most) s = most;
     p.splits = s < 1 ? 1 : (int)s;
+    // Slots by length where a warp's walk over the longest request would be 10 tiles or more: sharing them out
+    // takes 0.8 us for 8 requests, 1.5 us for 64.
+    const long long slots = 2ll * sm_count * requests / blocks;
+    if (requests > 1 && requests <= 32 * SHARE_LANES && slots > requests && most > 1 && keys <= 1 << 24 &&
+        key_tiles >= 10ll * p.key_warps * p.splits)
+        p.slots = (int)(slots < most * requests ? slots : most * requests);
     return p;
 }
 
 struct Plan {
     PassPlan own, prefix;
-    int parts;
-    size_t o_bytes, bytes;
+    long long own0, parts;  // first part of the own pass, all parts; 0 parts: written out at once
+    size_t o_bytes, ml_bytes, bytes;
 };
 
 Plan make_plan(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int requests, int rows, int hq, int window) {
@@ -575,33 +681,40 @@ Plan make_plan(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int
     const int hkv = cache->kv_heads > 0 ? cache->kv_heads : 1;
     const long long group = hq / hkv;
     const long long seen = window > 0 ? (long long)window + rows - 1 : cache->capacity;
-    p.own = plan_pass(ctx->sm_count, (long long)requests * hkv, rows * group, (int)(seen < cache->capacity ? seen : cache->capacity));
-    p.parts = p.own.splits;
+    const long long size = (long long)rows * hq;
+    p.own = plan_pass(ctx->sm_count, (long long)requests * hkv, requests, rows * group, (int)(seen < cache->capacity ? seen : cache->capacity));
     if (prefix_len > 0) {
-        p.prefix = plan_pass(ctx->sm_count, hkv, (long long)requests * rows * group, prefix_len);
-        p.parts += p.prefix.splits;
+        p.prefix = plan_pass(ctx->sm_count, hkv, 1, (long long)requests * rows * group, prefix_len);
+        p.own0 = p.prefix.splits * requests * size;
     }
-    if (p.parts > 1) {
-        const size_t n = (size_t)requests * rows * hq * p.parts;
-        p.o_bytes = n * 64 * sizeof(float);
-        p.bytes = p.o_bytes + n * 2 * sizeof(float);
+    if (prefix_len > 0 || p.own.splits > 1 || p.own.slots > 0) {
+        p.parts = p.own0 + (p.own.slots > 0 ? p.own.slots : (long long)requests * p.own.splits) * size;
+        p.o_bytes = (size_t)p.parts * 64 * sizeof(float);
+        p.ml_bytes = (size_t)p.parts * 2 * sizeof(float);
+        p.bytes = p.o_bytes + p.ml_bytes + (p.own.slots > 0 ? requests * sizeof(int2) : 0);
     }
     return p;
 }
 
-template <int KIND, int NT>
+template <int KIND, int NT, bool SHARE>
 void launch_pass_as(const PassArgs& a, cudaStream_t s) {
     using R = Rows<NT>;
     static PerDeviceOnce once;
-    once([] { cudaFuncSetAttribute(kv8_pass_kernel<KIND, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM); });
-    launch_k(kv8_pass_kernel<KIND, NT>, dim3((unsigned)(a.units * a.row_blocks * a.splits)), R::WARPS * 32, R::SMEM, s, a);
+    once([] { cudaFuncSetAttribute(kv8_pass_kernel<KIND, NT, SHARE>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM); });
+    const int blocks = SHARE ? a.slots * a.hkv * a.row_blocks : a.units * a.row_blocks * a.splits;
+    launch_k(kv8_pass_kernel<KIND, NT, SHARE>, dim3((unsigned)blocks), R::WARPS * 32, R::SMEM, s, a);
+}
+
+template <int KIND, int NT>
+void launch_pass_of(const PassArgs& a, cudaStream_t s) {
+    a.slots > 0 ? launch_pass_as<KIND, NT, true>(a, s) : launch_pass_as<KIND, NT, false>(a, s);
 }
 
 void launch_pass(const PassArgs& a, int nt, cudaStream_t s) {
     if (a.c.kind == MT_KV_INT8)
-        nt == 0 ? launch_pass_as<MT_KV_INT8, 0>(a, s) : nt == 1 ? launch_pass_as<MT_KV_INT8, 1>(a, s) : launch_pass_as<MT_KV_INT8, 2>(a, s);
+        nt == 0 ? launch_pass_of<MT_KV_INT8, 0>(a, s) : nt == 1 ? launch_pass_of<MT_KV_INT8, 1>(a, s) : launch_pass_of<MT_KV_INT8, 2>(a, s);
     else
-        nt == 0 ? launch_pass_as<MT_KV_E4M3, 0>(a, s) : nt == 1 ? launch_pass_as<MT_KV_E4M3, 1>(a, s) : launch_pass_as<MT_KV_E4M3, 2>(a, s);
+        nt == 0 ? launch_pass_of<MT_KV_E4M3, 0>(a, s) : nt == 1 ? launch_pass_of<MT_KV_E4M3, 1>(a, s) : launch_pass_of<MT_KV_E4M3, 2>(a, s);
 }
 
 mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q, int ldq, int requests, int rows, int hq,
@@ -634,22 +747,26 @@ mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q,
     a.requests = requests; a.hq = hq; a.hkv = hkv; a.group = hq / hkv;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + plan.o_bytes / sizeof(float);
-    a.parts = plan.parts;
+    int2* const shares = reinterpret_cast<int2*>(static_cast<char*>(workspace) + plan.o_bytes + plan.ml_bytes);
+    a.parted = plan.parts > 0;
     auto run = [&](const PassPlan& p) {
         a.units = p.units; a.row_blocks = p.row_blocks; a.splits = p.splits; a.key_warps = p.key_warps;
+        a.slots = p.slots; a.shares = shares;
         if (p.wide) launch_kv8_wide(a, p.chunk, ctx->d_status, s);
         else launch_pass(a, p.nt, s);
     };
+    const long long size = (long long)rows * hq;
     if (prefix_len > 0) {
         a.c = view(prefix); a.prefix_len = prefix_len; a.part0 = 0;
         run(plan.prefix);
     }
-    a.c = view(cache); a.prefix_len = 0; a.part0 = plan.parts - plan.own.splits; a.window = window;
+    a.c = view(cache); a.prefix_len = 0; a.part0 = plan.own0; a.window = window;
     a.beside = prefix_len > 0;
     run(plan.own);
-    if (plan.parts > 1) {
-        const JoinArgs j{a.rows, hq, plan.parts, a.part_o, a.part_ml, out, ldo, a.ovec};
-        launch_k(kv8_join_kernel, dim3((unsigned)((long long)requests * rows * hq)), JOIN_THREADS, 0, s, j);
+    if (a.parted) {
+        const JoinArgs j{a.rows, hq, plan.own.splits, plan.prefix.splits, plan.own.slots > 0 ? shares : nullptr,
+                         plan.own0, a.part_o, a.part_ml, out, ldo, a.ovec};
+        launch_k(kv8_join_kernel, dim3((unsigned)(requests * size)), JOIN_THREADS, 0, s, j);
     }
     return check_launch(ctx, what);
 }

@@ -300,7 +300,7 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
             int lo, hi;
             const int target = threadIdx.x < KV8_WIDE_ROWS ? rows.pair(e0 + threadIdx.x, lo, hi) : -1;
             if (target >= 0)
-                reinterpret_cast<float2*>(a.part_ml)[(size_t)target * a.parts + a.part0 + split] = make_float2(KV8_REF_NONE, 0.f);
+                reinterpret_cast<float2*>(a.part_ml)[a.part0 + (size_t)target * a.splits + split] = make_float2(KV8_REF_NONE, 0.f);
         }
         return;
     }
@@ -454,13 +454,13 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
                     float f = sh.unit * down;
                     float* dst;
                     bool vec = true;
-                    if (a.parts == 1) {
+                    if (!a.parted) {
                         const int at = target[i] / a.hq;
                         dst = a.out + (size_t)at * a.ldo + (size_t)(target[i] - at * a.hq) * 64;
                         vec = a.ovec;
                         f /= total;
                     } else {
-                        const size_t at = (size_t)target[i] * a.parts + a.part0 + split;
+                        const size_t at = (size_t)target[i] * a.splits + a.part0 + split;
                         if (col == 0) reinterpret_cast<float2*>(a.part_ml)[at] = make_float2(s0 == 0.f ? KV8_REF_NONE : row.off[i] + lift, total);
                         dst = a.part_o + at * 64;
                     }
