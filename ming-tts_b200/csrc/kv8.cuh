@@ -213,6 +213,28 @@ __device__ __forceinline__ float2 kv8_unit(const float (&z)[4], const float (&v)
     return make_float2(ref - lift, lift);
 }
 
+// A row's sum of weights, in units of 2^off, as (reference, sum) with sum in [1, 2): whatever its units,
+// sums of several parts can be compared and added. The outputs that go with it are already divided by it,
+// so that no step on the way is larger than the largest value, which may be near fp32's largest.
+__device__ __forceinline__ float2 kv8_total(float off, float sum) {
+    if (sum == 0.f) return make_float2(KV8_REF_NONE, 0.f);
+    const float p = power_to(sum, 0);
+    return make_float2(off + (float)(127 - (int)(__float_as_uint(p) >> 23)), sum * p);
+}
+
+// Output x (in units of `unit`, a power of two) divided by the sum of weights: `unit` in two halves, so that
+// neither a product with it nor one with over (one over the sum) leaves fp32 where the result does not.
+struct OverSum {
+    float first, second, over;
+    __device__ __forceinline__ OverSum(float unit, float sum) {
+        const int e = (int)(__float_as_uint(unit) >> 23) - 127, half = e >> 1;
+        first = __uint_as_float((uint32_t)(half + 127) << 23);
+        second = __uint_as_float((uint32_t)(e - half + 127) << 23);
+        over = sum == 0.f ? 0.f : 1.f / sum;
+    }
+    __device__ __forceinline__ float operator()(float x) const { return x * first * over * second; }
+};
+
 // Makes a device current for a call and puts the caller's back.
 struct DeviceGuard {
     int before = -1;

@@ -255,11 +255,10 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
                 for (int j = 0; j < 4; j++) o[n][i][j] = 0.f;
     };
     clear();
-    auto fold = [&](bool first, bool last) {
-        const float n = v_unit > 0.f ? 1.f / v_unit : 0.f;
+    auto fold = [&](bool first) {
 #pragma unroll
         for (int i = 0; i < LR; i++) {
-            const float f = first ? 0.f : ex2(at_off[i] - off[i]), down = last && lift[i] != KV8_UNSET ? ex2(-lift[i]) : 1.f;
+            const float f = first ? 0.f : ex2(at_off[i] - off[i]);
             at_off[i] = off[i];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -268,7 +267,7 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
                 auto add = [&](float& x, int d) {
                     const int m = 4 * (j & 1) + d, col = j >> 1;
                     const float v = NT == 0 ? o[0][m][col] + o[0][m][2 + col] : o[i / 2][m][2 * (i & 1) + col];
-                    x = (first ? v * n : fmaf(v, n, x * f)) * down;
+                    x = first ? v : fmaf(x, f, v);
                 };
                 add(y.x, 0); add(y.y, 1); add(y.z, 2); add(y.w, 3);
                 *at = y;
@@ -337,7 +336,7 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
         int chain = 0;
         for (int stage = 0; at < end; at += a.key_warps, stage = (stage + 1) & (RING - 1)) {
             if (++chain == FOLD + 1) {
-                fold(!folded, false);
+                fold(!folded);
                 clear();
                 folded = true;
                 chain = 1;
@@ -486,15 +485,19 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
     }
 
     // Join the key_warps warps of each row tile.
-    fold(!folded, true);
+    fold(!folded);
     float2* sml = reinterpret_cast<float2*>(smem + R::WARPS * R::COUNT * 64);
 #pragma unroll
     for (int i = 0; i < LR; i++) {
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-        if (t == 0)
-            sml[warp * R::COUNT + 8 * i + g] =
-                lift[i] == KV8_UNSET ? make_float2(KV8_REF_NONE, sum[i]) : make_float2(off[i] + lift[i], sum[i] * ex2(-lift[i]));
+        const OverSum out(v_unit > 0.f ? 1.f / v_unit : 1.f, sum[i]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float4* at = reinterpret_cast<float4*>(acc + 512 * i) + j;
+            *at = make_float4(out(at->x), out(at->y), out(at->z), out(at->w));
+        }
+        if (t == 0) sml[warp * R::COUNT + 8 * i + g] = kv8_total(off[i], sum[i]);
     }
     int* owner = reinterpret_cast<int*>(sml + R::WARPS * R::COUNT);
     if (phase == 0 && t == 0) {
@@ -509,19 +512,18 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
         const int base = (row / R::COUNT) * a.key_warps * R::COUNT + row % R::COUNT;
         float top = KV8_REF_NONE, l = 0.f;
         for (int k = 0; k < a.key_warps; k++) top = fmaxf(top, sml[base + k * R::COUNT].x);
+        for (int k = 0; k < a.key_warps; k++) l += ex2(sml[base + k * R::COUNT].x - top) * sml[base + k * R::COUNT].y;
+        const float over = 1.f / l;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int k = 0; k < a.key_warps; k++) {
             const float2 ml = sml[base + k * R::COUNT];
-            const float f = ex2(ml.x - top);
+            const float f = ex2(ml.x - top) * ml.y * over;
             const float4 v = reinterpret_cast<const float4*>(smem + (base + k * R::COUNT) * 64)[d4];
-            l += f * ml.y;
             y.x += f * v.x; y.y += f * v.y; y.z += f * v.z; y.w += f * v.w;
         }
         if (!a.parted) {
             const int qrow = target / a.hq, head = target - qrow * a.hq;
             float* dst = a.out + (size_t)qrow * a.ldo + (size_t)head * 64 + 4 * d4;
-            const float n = 1.f / l;
-            y.x *= n; y.y *= n; y.z *= n; y.w *= n;
             if (a.ovec) {
                 *reinterpret_cast<float4*>(dst) = y;
             } else {
@@ -530,15 +532,15 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
         } else {
             const long long part = part0 + (long long)target * splits + split;
             if (d4 == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(top, l);
-            if (top > KV8_REF_NONE || !(l == 0.f)) reinterpret_cast<float4*>(a.part_o + part * 64)[d4] = y;  // else not read
+            if (!(l == 0.f)) reinterpret_cast<float4*>(a.part_o + part * 64)[d4] = y;  // else not read
         }
     }
     if (a.beside) pdl_wait();
 }
 
-// Joins the parts of each (row, head): out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s. A block a
-// (row, head): 16 lanes cover the 64 dimensions, the 8 groups of 16 take parts in turn, so that some 60 parts
-// are two or three round trips to memory and not thirty.
+// Joins the parts of each (row, head): out = sum_s w_s O_s, w_s = 2^(m_s - M) l_s / (the sum of these). A
+// block a (row, head): a thread a part for the weights; 16 lanes cover the 64 dimensions, the 8 groups of 16
+// take parts in turn, so that 64 parts are one round trip to memory, begun before the weights are known.
 struct JoinArgs {
     Kv8Rows rows;
     int hq, splits, prefix_splits;  // parts of a request's own pass (shares: by request) and of the prefix's
@@ -547,14 +549,16 @@ struct JoinArgs {
     const float *part_o, *part_ml;
     float* out; int ldo; bool ovec;
 };
-constexpr int JOIN_THREADS = 128, JOIN_GROUPS = JOIN_THREADS / 16;
+constexpr int JOIN_THREADS = 128, JOIN_GROUPS = JOIN_THREADS / 16, JOIN_AHEAD = 8;
+constexpr int MOST_SPLITS = 512;  // of a pass
 
 __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const JoinArgs a) {
-    __shared__ float4 partial[JOIN_GROUPS][16];
-    __shared__ float2 total[JOIN_GROUPS];
+    __shared__ float2 weight[2 * MOST_SPLITS];  // (reference, sum), then (weight, -)
+    __shared__ float warp_top[JOIN_THREADS / 32], warp_sum[JOIN_THREADS / 32];
+    __shared__ float4 partial[JOIN_THREADS / 32][16];
     pdl_wait();
     pdl_launch();
-    const int group = threadIdx.x >> 4, d4 = threadIdx.x & 15;
+    const int group = threadIdx.x >> 4, d4 = threadIdx.x & 15, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = blockIdx.x / a.hq, request = row / a.rows.rows;
     if (row - request * a.rows.rows >= kv8_span(a.rows, request).count) return;
     const int2 own = a.shares ? a.shares[request] : make_int2(request * a.splits, a.splits);
@@ -562,37 +566,57 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const JoinArgs a
     const long long size = (long long)a.rows.rows * a.hq;
     const long long prefix_at = (long long)blockIdx.x * a.prefix_splits;
     const long long own_at = a.own0 + (own.x - (long long)request * own.y) * size + (long long)blockIdx.x * own.y - a.prefix_splits;
-    float top = KV8_REF_NONE, l = 0.f;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = group; s < parts; s += JOIN_GROUPS) {
-        const long long at = (s < a.prefix_splits ? prefix_at : own_at) + s;
-        const float2 p = reinterpret_cast<const float2*>(a.part_ml)[at];
-        const bool any = !(p.y == 0.f);  // a part without a key has no sums
-        const float4 v = any ? reinterpret_cast<const float4*>(a.part_o)[at * 16 + d4] : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float now = any ? fmaxf(top, p.x) : top, f = ex2(top - now), n = any ? ex2(p.x - now) : 0.f;
-        top = now;
-        l = l * f + (any ? n * p.y : 0.f);
-        y.x = y.x * f + n * v.x; y.y = y.y * f + n * v.y; y.z = y.z * f + n * v.z; y.w = y.w * f + n * v.w;
+    auto at = [&](int s) { return (s < a.prefix_splits ? prefix_at : own_at) + s; };
+    auto output = [&](int s) { return reinterpret_cast<const float4*>(a.part_o)[at(s) * 16 + d4]; };
+    float4 ahead[JOIN_AHEAD];
+#pragma unroll
+    for (int i = 0; i < JOIN_AHEAD; i++)
+        ahead[i] = group + i * JOIN_GROUPS < parts ? output(group + i * JOIN_GROUPS) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = KV8_REF_NONE, sum = 0.f;
+    for (int s = threadIdx.x; s < parts; s += JOIN_THREADS) {
+        const float2 p = reinterpret_cast<const float2*>(a.part_ml)[at(s)];
+        weight[s] = p;
+        top = fmaxf(top, p.x);
     }
-    partial[group][d4] = y;
-    if (d4 == 0) total[group] = make_float2(top, l);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) warp_top[warp] = top;
     __syncthreads();
-    if (group > 0) return;
-    const int groups = min(parts, JOIN_GROUPS);
-    for (int s = 0; s < groups; s++) top = fmaxf(top, total[s].x);
-    l = 0.f;
-    y = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < groups; s++) {
-        const float2 p = total[s];
-        const float4 v = partial[s][d4];
-        const float f = ex2(p.x - top);
-        l += f * p.y;
-        y.x += f * v.x; y.y += f * v.y; y.z += f * v.z; y.w += f * v.w;
+    top = fmaxf(fmaxf(warp_top[0], warp_top[1]), fmaxf(warp_top[2], warp_top[3]));
+    for (int s = threadIdx.x; s < parts; s += JOIN_THREADS) {
+        const float2 p = weight[s];
+        const float w = ex2(p.x - top) * p.y;
+        sum += w;
+        weight[s].x = p.y == 0.f ? -1.f : w;  // a part without a key has no outputs
     }
-    const float n = 1.f / l;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) warp_sum[warp] = sum;
+    __syncthreads();
+    const float over = 1.f / ((warp_sum[0] + warp_sum[1]) + (warp_sum[2] + warp_sum[3]));
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](int s, const float4& v) {
+        const float w = weight[s].x, f = w * over;
+        if (w < 0.f) return;
+        y.x += f * v.x; y.y += f * v.y; y.z += f * v.z; y.w += f * v.w;
+    };
+#pragma unroll
+    for (int i = 0; i < JOIN_AHEAD; i++) {
+        if (group + i * JOIN_GROUPS < parts) add(group + i * JOIN_GROUPS, ahead[i]);
+    }
+#pragma unroll 4
+    for (int s = group + JOIN_AHEAD * JOIN_GROUPS; s < parts; s += JOIN_GROUPS) add(s, output(s));
+    y.x += __shfl_xor_sync(0xffffffffu, y.x, 16);
+    y.y += __shfl_xor_sync(0xffffffffu, y.y, 16);
+    y.z += __shfl_xor_sync(0xffffffffu, y.z, 16);
+    y.w += __shfl_xor_sync(0xffffffffu, y.w, 16);
+    if (lane < 16) partial[warp][d4] = y;
+    __syncthreads();
+    if (threadIdx.x >= 16) return;
+    const float4 p0 = partial[0][d4], p1 = partial[1][d4], p2 = partial[2][d4], p3 = partial[3][d4];
+    y = make_float4((p0.x + p1.x) + (p2.x + p3.x), (p0.y + p1.y) + (p2.y + p3.y), (p0.z + p1.z) + (p2.z + p3.z),
+                    (p0.w + p1.w) + (p2.w + p3.w));
     float* dst = a.out + (size_t)row * a.ldo + (size_t)(blockIdx.x - row * a.hq) * 64 + 4 * d4;
-    y.x *= n; y.y *= n; y.z *= n; y.w *= n;
     if (a.ovec) {
         *reinterpret_cast<float4*>(dst) = y;
     } else {
@@ -624,7 +648,7 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
     {
         const long long row_blocks = (qrows + KV8_WIDE_ROWS - 1) / KV8_WIDE_ROWS, blocks = units * row_blocks;
         const long long tiles = (keys + 15 + KV8_WIDE_KEYS - 1) / KV8_WIDE_KEYS;
-        long long s = sm_count / blocks;
+        long long s = (sm_count < MOST_SPLITS ? sm_count : MOST_SPLITS) / blocks;
         if (s > tiles / 4) s = tiles / 4;
         if (s < 1) s = 1;
         const long long chunk = (tiles + s - 1) / s, waves = (blocks * s + sm_count - 1) / sm_count;
@@ -660,11 +684,12 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
     long long s = 2ll * sm_count / blocks;
     const long long most = key_tiles / (4 * p.key_warps);
     if (s > most) s = most;
+    if (s > MOST_SPLITS) s = MOST_SPLITS;
     p.splits = s < 1 ? 1 : (int)s;
     // Slots by length where a warp's walk over the longest request would be 10 tiles or more: sharing them out
     // takes 0.8 us for 8 requests, 1.5 us for 64.
     const long long slots = 2ll * sm_count * requests / blocks;
-    if (requests > 1 && requests <= 32 * SHARE_LANES && slots > requests && most > 1 && keys <= 1 << 24 &&
+    if (requests > 1 && requests <= 32 * SHARE_LANES && slots > requests && slots - requests < MOST_SPLITS && most > 1 && keys <= 1 << 24 &&
         key_tiles >= 10ll * p.key_warps * p.splits)
         p.slots = (int)(slots < most * requests ? slots : most * requests);
     return p;

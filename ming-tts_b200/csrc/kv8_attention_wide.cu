@@ -450,18 +450,16 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
                     s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
                     s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
                     if (target[i] < 0) continue;
-                    const float lift = row.lift[i] == KV8_UNSET ? 0.f : row.lift[i], down = ex2(-lift), total = s0 * down;
-                    float f = sh.unit * down;
+                    const OverSum out(sh.unit, s0);
                     float* dst;
                     bool vec = true;
                     if (!a.parted) {
                         const int at = target[i] / a.hq;
                         dst = a.out + (size_t)at * a.ldo + (size_t)(target[i] - at * a.hq) * 64;
                         vec = a.ovec;
-                        f /= total;
                     } else {
                         const size_t at = (size_t)target[i] * a.splits + a.part0 + split;
-                        if (col == 0) reinterpret_cast<float2*>(a.part_ml)[at] = make_float2(s0 == 0.f ? KV8_REF_NONE : row.off[i] + lift, total);
+                        if (col == 0) reinterpret_cast<float2*>(a.part_ml)[at] = kv8_total(row.off[i], s0);
                         dst = a.part_o + at * 64;
                     }
                     dst += col;
@@ -471,10 +469,10 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
                         for (int j = 0; j < 2; j++) {
                             const float* o = row.o[c] + 4 * j + 2 * i;
                             if (vec) {
-                                *reinterpret_cast<float2*>(dst + 16 * c + 8 * j) = make_float2(o[0] * f, o[1] * f);
+                                *reinterpret_cast<float2*>(dst + 16 * c + 8 * j) = make_float2(out(o[0]), out(o[1]));
                             } else {
-                                dst[16 * c + 8 * j] = o[0] * f;
-                                dst[16 * c + 8 * j + 1] = o[1] * f;
+                                dst[16 * c + 8 * j] = out(o[0]);
+                                dst[16 * c + 8 * j + 1] = out(o[1]);
                             }
                         }
                 }

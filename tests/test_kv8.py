@@ -610,6 +610,134 @@ def test_offsets_past_32_bits(ctx, mt, kind):
     assert float((outs[0] - outs[1]).abs().max()) <= tol
 
 
+# Sizes at which calls of many rows, and long batches of different lengths, are laid out in their own ways.
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,window,capacity,positions", [
+    (500, 300, 900, [0, 1000, 333]), (300, 0, 500, [0, 450, 900]), (400, 1, 701, [0, 301, 302]), (513, 64, 1001, [3, 977]),
+    (257, 1000, 1256, [999, 5000, 0]),
+])
+def test_many_rows_window_and_ring(ctx, mt, kind, rows, window, capacity, positions):
+    check_attention(ctx, mt, kind, 14, 2, capacity, positions, rows, window=window)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hq,hkv", [(14, 2), (5, 5), (40, 1)])
+def test_many_rows_padding_idle_and_strides(ctx, mt, kind, hq, hkv):
+    positions, counts = [3, -1, 140, 0, 260, 999], [400, 400, 0, 1, 377, 129]
+    check_attention(ctx, mt, kind, hq, hkv, 1130, positions, 400, counts=counts, pad_q=8, pad_o=4)
+    check_attention(ctx, mt, kind, hq, hkv, 1131, positions, 400, counts=counts, pad_q=3, pad_o=1, layers=3)
+    check_attention(ctx, mt, kind, hq, hkv, 900, [200, 100, 150, 400, 99], 470, base=100, layers=2)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_rows_scales_of_very_different_sizes(ctx, mt, kind):
+    check_attention(ctx, mt, kind, 14, 2, 1300, [800], 400, spread=3.0)
+    check_attention(ctx, mt, kind, 14, 2, 1300, [800], 400, spread=0.1, q_scale=60.0)
+    check_attention(ctx, mt, kind, 14, 2, 1300, [800], 400, q_scale=1e-6)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_rows_extreme_scales(ctx, mt, kind):
+    """As test_extreme_scales."""
+    import torch
+    rows, hq, n = 600, 8, 1400
+    g = torch.Generator().manual_seed(5)
+    codes = torch.randint(-127, 128, (1, 1, n, 64), generator=g, dtype=torch.int8)
+    codes = codes if kind == "int8" else (codes.float() * 3).to(torch.float8_e4m3fn)
+    unit = torch.rand(1, 1, n, generator=g) + 0.5
+    q = torch.randn(rows, hq * 64, generator=g)
+    pos = torch.tensor([n - rows], dtype=torch.int32, device="cuda")
+    outs = []
+    for kf, vf, qf in ((2.0 ** -6, 1.0, 1.0), (2.0 ** -106, 2.0 ** -120, 2.0 ** 100), (2.0 ** 94, 2.0 ** 110, 2.0 ** -100),
+                       (2.0 ** -6, 0.0, 1.0)):
+        cache = mt.KV8Cache(codes.cuda(), codes.flip(2).contiguous().cuda(), (unit * kf).cuda(), (unit * vf).cuda())
+        out = torch.empty(rows, hq * 64, device="cuda")
+        ctx.attention_kv8((q * qf).cuda(), hq * 64, 1, rows, hq, pos, None, 0, cache, out, hq * 64)
+        ctx.check()
+        outs.append(out.cpu().double())
+    assert torch.isfinite(outs[0]).all() and torch.all(outs[3] == 0)
+    top = outs[0].abs().amax()
+    assert torch.all((outs[1] * 2.0 ** 120 - outs[0]).abs() <= 2.0 ** -20 * top)
+    assert torch.all((outs[2] * 2.0 ** -110 - outs[0]).abs() <= 2.0 ** -20 * top)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_rows_nan_reaches_only_rows_that_see_it(ctx, mt, kind):
+    import torch
+    n, rows, hq = 900, 900, 8
+    for bad_at in (0, 450, 899):
+        for which in (2, 3):
+            cache = Cache(mt, kind, 2, n, [(0, n)], 9)
+            cache.kv.tensors[which][0, 1, bad_at] = math.nan
+            q = torch.randn(rows, hq * 64, device="cuda")
+            q[600, :64] = math.nan
+            out = torch.empty_like(q)
+            pos = torch.zeros(1, dtype=torch.int32, device="cuda")
+            ctx.attention_kv8(q, hq * 64, 1, rows, hq, pos, None, 0, cache.kv, out, hq * 64)
+            ctx.check()
+            bad = torch.isnan(out).view(rows, hq, 64).all(-1).cpu()
+            some = torch.isnan(out).view(rows, hq, 64).any(-1).cpu()
+            want = torch.zeros(rows, hq, dtype=torch.bool)
+            want[bad_at:, 4:] = True
+            want[600, 0] = True
+            assert torch.equal(bad, want) and torch.equal(some, want)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_rows_prefix(ctx, mt, kind):
+    """The rows of all requests in one pass over the prefix, padding and idle requests among them."""
+    n = 22
+    positions = [2000 + 7 * i for i in range(n - 2)] + [-1, 1999]
+    counts = [9, 0, 4, 9, 1] * 4 + [9, 9]
+    check_attention(ctx, mt, kind, 14, 2, 150, positions, 9, counts=counts, prefix_len=2000, pad_q=1, pad_o=3, layers=2)
+    check_attention(ctx, mt, kind, 14, 2, 60, positions, 9, counts=counts, prefix_len=2000)  # own parts that wrap
+    check_attention(ctx, mt, kind, 6, 3, 700, [1500, 1600], 600, prefix_len=1500)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hq,hkv,rows,base", [(14, 2, 1, 0), (20, 1, 2, 3), (14, 1, 1, 3)])
+def test_long_batch_of_different_lengths(ctx, mt, kind, hq, hkv, rows, base):
+    check_attention(ctx, mt, kind, hq, hkv, 40000, [39998, -1, 50, 12345, 3, 30000], rows, base=base)
+    check_attention(ctx, mt, kind, hq, hkv, 40000, [39998, 2, 50, 12345, 3, 30000], rows, counts=[1, 0, 1, rows, 1, 0], base=base)
+    check_attention(ctx, mt, kind, hq, hkv, 40000, [-1] * 6, rows, base=base)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_long_batch_of_many_requests(ctx, mt, kind):
+    positions = [100 + 137 * i for i in range(40)]
+    positions[3], positions[20], positions[33], positions[39] = 19999, 0, -1, 16000
+    check_attention(ctx, mt, kind, 7, 1, 20000, positions, 1)
+    check_attention(ctx, mt, kind, 7, 1, 20000, positions, 1, counts=[1] * 20 + [0] * 15 + [1] * 5)
+    check_attention(ctx, mt, kind, 7, 1, 10001, [p + 8000 for p in positions], 2, window=10000)
+    check_attention(ctx, mt, kind, 7, 1, 20000, [p + 100 for p in positions], 1, prefix_len=100)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("args", [(14, 2, 40000, [39000, 10, 1000, 0, 25000, 4000], 1), (14, 2, 1500, [0, 700], 600)])
+def test_long_calls_repeat_bit_for_bit(ctx, mt, kind, args):
+    import torch
+    first = check_attention(ctx, mt, kind, *args)
+
+    def both(call):
+        s = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        for t in s:
+            with torch.cuda.stream(t):
+                call()
+        torch.cuda.synchronize()
+
+    assert torch.equal(check_attention(ctx, mt, kind, *args, run=both), first)
+
+
 # ------------------------------------------------------------------------------------------------
 # As a program uses them
 # ------------------------------------------------------------------------------------------------
