@@ -148,6 +148,12 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ float rcp(float x) {  // within one unit of the last place
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Codes of bytes 0, 1 and of bytes 2, 3 as two fp16 pairs. Integers: the byte with its sign bit
 // flipped, put under fp16's 1024 (0x64), is 1024 + 128 + code.
 template <int KIND>
@@ -222,17 +228,17 @@ __device__ __forceinline__ float2 kv8_total(float off, float sum) {
     return make_float2(off + (float)(127 - (int)(__float_as_uint(p) >> 23)), sum * p);
 }
 
-// Output x (in units of `unit`, a power of two) divided by the sum of weights: `unit` in two halves, so that
-// neither a product with it nor one with over (one over the sum) leaves fp32 where the result does not.
+// Outputs (in units of `unit`, a power of two) divided by the sum of weights: unit and the sum's power of two
+// in two halves, the rest of the sum, in [1, 2), with the first. No product leaves fp32 where the result does not.
 struct OverSum {
-    float first, second, over;
+    float first, second;
     __device__ __forceinline__ OverSum(float unit, float sum) {
-        const int e = (int)(__float_as_uint(unit) >> 23) - 127, half = e >> 1;
-        first = __uint_as_float((uint32_t)(half + 127) << 23);
+        const float p = power_to(sum, 0);
+        const int e = (int)(__float_as_uint(unit) >> 23) + (int)(__float_as_uint(p) >> 23) - 2 * 127, half = e >> 1;
+        first = sum == 0.f ? 0.f : __uint_as_float((uint32_t)(half + 127) << 23) * rcp(sum * p);
         second = __uint_as_float((uint32_t)(e - half + 127) << 23);
-        over = sum == 0.f ? 0.f : 1.f / sum;
     }
-    __device__ __forceinline__ float operator()(float x) const { return x * first * over * second; }
+    __device__ __forceinline__ float operator()(float x) const { return x * first * second; }
 };
 
 // Makes a device current for a call and puts the caller's back.

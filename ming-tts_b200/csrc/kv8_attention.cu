@@ -114,7 +114,7 @@ struct Rows {
     static constexpr int COUNT = NT == 0 ? 8 : 16 * NT;   // rows of a warp
     static constexpr int WARPS = NT == 0 ? 8 : 4;
     static constexpr int BLOCKS = NT == 2 ? 2 : NT == 1 ? 3 : 2;  // resident blocks the registers allow
-    static constexpr int SUM_BYTES = WARPS * COUNT * (64 + 2 + 1) * 4;   // sums, references, owners
+    static constexpr int SUM_BYTES = WARPS * COUNT * (64 + 4 + 1) * 4;   // sums, references and units, owners
     static constexpr int SMEM = SUM_BYTES + WARPS * RING * TILE_BYTES;
 };
 
@@ -486,18 +486,14 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
 
     // Join the key_warps warps of each row tile.
     fold(!folded);
-    float2* sml = reinterpret_cast<float2*>(smem + R::WARPS * R::COUNT * 64);
+    float4* sml = reinterpret_cast<float4*>(smem + R::WARPS * R::COUNT * 64);  // reference, sum; halves of the unit
 #pragma unroll
     for (int i = 0; i < LR; i++) {
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+        const float2 ml = kv8_total(off[i], sum[i]);
         const OverSum out(v_unit > 0.f ? 1.f / v_unit : 1.f, sum[i]);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            float4* at = reinterpret_cast<float4*>(acc + 512 * i) + j;
-            *at = make_float4(out(at->x), out(at->y), out(at->z), out(at->w));
-        }
-        if (t == 0) sml[warp * R::COUNT + 8 * i + g] = kv8_total(off[i], sum[i]);
+        if (t == 0) sml[warp * R::COUNT + 8 * i + g] = make_float4(ml.x, ml.y, out.first, out.second);
     }
     int* owner = reinterpret_cast<int*>(sml + R::WARPS * R::COUNT);
     if (phase == 0 && t == 0) {
@@ -513,13 +509,14 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
         float top = KV8_REF_NONE, l = 0.f;
         for (int k = 0; k < a.key_warps; k++) top = fmaxf(top, sml[base + k * R::COUNT].x);
         for (int k = 0; k < a.key_warps; k++) l += ex2(sml[base + k * R::COUNT].x - top) * sml[base + k * R::COUNT].y;
-        const float over = 1.f / l;
+        const float over = rcp(l);
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int k = 0; k < a.key_warps; k++) {
-            const float2 ml = sml[base + k * R::COUNT];
+            const float4 ml = sml[base + k * R::COUNT];
             const float f = ex2(ml.x - top) * ml.y * over;
             const float4 v = reinterpret_cast<const float4*>(smem + (base + k * R::COUNT) * 64)[d4];
-            y.x += f * v.x; y.y += f * v.y; y.z += f * v.z; y.w += f * v.w;
+            y.x += f * (v.x * ml.z * ml.w); y.y += f * (v.y * ml.z * ml.w);
+            y.z += f * (v.z * ml.z * ml.w); y.w += f * (v.w * ml.z * ml.w);
         }
         if (!a.parted) {
             const int qrow = target / a.hq, head = target - qrow * a.hq;
@@ -593,7 +590,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const JoinArgs a
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) warp_sum[warp] = sum;
     __syncthreads();
-    const float over = 1.f / ((warp_sum[0] + warp_sum[1]) + (warp_sum[2] + warp_sum[3]));
+    const float over = rcp((warp_sum[0] + warp_sum[1]) + (warp_sum[2] + warp_sum[3]));
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](int s, const float4& v) {
         const float w = weight[s].x, f = w * over;
@@ -617,6 +614,52 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const JoinArgs a
     y = make_float4((p0.x + p1.x) + (p2.x + p3.x), (p0.y + p1.y) + (p2.y + p3.y), (p0.z + p1.z) + (p2.z + p3.z),
                     (p0.w + p1.w) + (p2.w + p3.w));
     float* dst = a.out + (size_t)row * a.ldo + (size_t)(blockIdx.x - row * a.hq) * 64 + 4 * d4;
+    if (a.ovec) {
+        *reinterpret_cast<float4*>(dst) = y;
+    } else {
+        dst[0] = y.x; dst[1] = y.y; dst[2] = y.z; dst[3] = y.w;
+    }
+}
+
+// The same for at most JOIN_GROUPS parts: a group of 16 lanes a (row, head), every lane all weights. The
+// reductions over a block above take 0.5 us longer.
+__global__ void __launch_bounds__(JOIN_THREADS) kv8_join_few_kernel(const JoinArgs a, int pairs) {
+    pdl_wait();
+    pdl_launch();
+    const int pair = blockIdx.x * JOIN_GROUPS + (threadIdx.x >> 4), d4 = threadIdx.x & 15;
+    if (pair >= pairs) return;
+    const int row = pair / a.hq, request = row / a.rows.rows;
+    if (row - request * a.rows.rows >= kv8_span(a.rows, request).count) return;
+    const long long prefix_at = (long long)pair * a.prefix_splits, own_at = a.own0 + (long long)pair * a.splits - a.prefix_splits;
+    const int parts = a.prefix_splits + a.splits;
+    float2 p[JOIN_GROUPS];
+    float4 v[JOIN_GROUPS];
+    float top = KV8_REF_NONE, sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < JOIN_GROUPS; s++) {
+        const long long at = (s < a.prefix_splits ? prefix_at : own_at) + s;
+        p[s] = make_float2(KV8_REF_NONE, 0.f);
+        if (s < parts) {
+            p[s] = reinterpret_cast<const float2*>(a.part_ml)[at];
+            v[s] = reinterpret_cast<const float4*>(a.part_o)[at * 16 + d4];
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < JOIN_GROUPS; s++) top = fmaxf(top, p[s].x);
+#pragma unroll
+    for (int s = 0; s < JOIN_GROUPS; s++) {
+        p[s].x = ex2(p[s].x - top) * p[s].y;
+        sum += p[s].x;
+    }
+    const float over = rcp(sum);
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < JOIN_GROUPS; s++) {
+        if (p[s].y == 0.f) continue;  // a part without a key has no outputs
+        const float f = p[s].x * over;
+        y.x += f * v[s].x; y.y += f * v[s].y; y.z += f * v[s].z; y.w += f * v[s].w;
+    }
+    float* dst = a.out + (size_t)row * a.ldo + (size_t)(pair - row * a.hq) * 64 + 4 * d4;
     if (a.ovec) {
         *reinterpret_cast<float4*>(dst) = y;
     } else {
@@ -791,7 +834,11 @@ mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q,
     if (a.parted) {
         const JoinArgs j{a.rows, hq, plan.own.splits, plan.prefix.splits, plan.own.slots > 0 ? shares : nullptr,
                          plan.own0, a.part_o, a.part_ml, out, ldo, a.ovec};
-        launch_k(kv8_join_kernel, dim3((unsigned)(requests * size)), JOIN_THREADS, 0, s, j);
+        const unsigned pairs = (unsigned)(requests * size);
+        if (!j.shares && j.splits + j.prefix_splits <= JOIN_GROUPS)
+            launch_k(kv8_join_few_kernel, dim3((pairs + JOIN_GROUPS - 1) / JOIN_GROUPS), JOIN_THREADS, 0, s, j, (int)pairs);
+        else
+            launch_k(kv8_join_kernel, dim3(pairs), JOIN_THREADS, 0, s, j);
     }
     return check_launch(ctx, what);
 }
