@@ -11,16 +11,22 @@
 // a power of two per row, weights by one per row that follows the largest weight times scale, so that
 // the planes use fp16's range whatever the units.
 //
-// A warp owns a tile of query rows (8, 16 or 32: rows x grouped heads, flattened) and walks its keys 16
-// at a time. Its lanes load codes straight from the cache into the layout of the matrix instruction
-// (m16n8k16): which key or dimension a fragment's row or column stands for is free as long as both
-// operands agree, so a lane takes 16 consecutive bytes of one key row for the scores, 8 consecutive
-// bytes of four key rows for the values, and the conversion to fp16 pairs the bytes of two keys. No
-// shared memory and no barrier until the partial results of the block's warps are joined.
+// A warp owns a tile of 8 query rows (rows x grouped heads, flattened) and walks its keys 16 at a time, copied
+// ahead into a ring in shared memory. The rows' hi planes are rows 0-7 and their lo planes rows 8-15 of the
+// 16-row operand of m16n8k16, for the queries and again for the weights. Which key or dimension a fragment's
+// row or column stands for is free as long as both operands agree, so a lane takes 16 consecutive bytes of
+// one key row for the scores, 8 consecutive bytes of four key rows for the values, and the conversion to
+// fp16 pairs the bytes of two keys. Warps meet only when the partial results of a block are merged.
 //   Lane (g, t) = (lane / 4, lane % 4), in a tile of keys 0..15:
 //     scores, column g of half j is key 4 (g / 2) + 2 j + g % 2, so lane t's scores are keys 4t .. 4t+3
 //     values, contraction index 2t, 2t+1, 2t+8, 2t+9 is key 4t .. 4t+3; column g of block i is dimension
 //     8 g + i, so lane t's outputs are dimensions 16 t .. 16 t + 15.
+// Bounded by instruction issue: 332 a tile of 16 keys, of which 32 are matrix instructions, 100 the conversion
+// of codes and 40 the weights, 57% of the issue slots used at 16 warps an SM; 64 requests of 8000 keys run at
+// 52% of the copy bandwidth. Tiles of 16 and 32 rows (the planes as operands of their own, each code
+// converted once for all of them) were 530 and 974 instructions a tile, but their registers leave room for 12
+// and 8 warps, which used 40% of the slots, and the fixed part of a call took 3 and 7 us longer: slower at
+// every size, or no faster. Many rows against many keys go to kv8_attention_wide.cu.
 #include <math.h>
 
 #include <type_traits>
@@ -104,20 +110,9 @@ __device__ __forceinline__ float value_unit(const float (&vs)[4]) {
     return x > 0.f ? power_to(x, 0) : 1.f;
 }
 
-// NT 0: 8 rows, whose hi planes are rows 0-7 and lo planes rows 8-15 of one 16-row operand (a decode
-// step's group of heads); NT 1, 2: 16 or 32 rows, the planes as two operands.
-template <int NT>
-struct Rows {
-    static constexpr int SETS = NT == 0 ? 1 : NT;         // 16-row operands
-    static constexpr int PLANES = NT == 0 ? 1 : 2;        // of each
-    static constexpr int LANE = NT == 0 ? 1 : 2 * NT;     // rows of which a lane holds a part
-    static constexpr int COUNT = NT == 0 ? 8 : 16 * NT;   // rows of a warp
-    static constexpr int WARPS = NT == 0 ? 8 : 4;
-    static constexpr int BLOCKS = NT == 2 ? 2 : NT == 1 ? 3 : 2;  // resident blocks the registers allow
-    static constexpr int SUM_BYTES = WARPS * COUNT * (64 + 4 + 1) * 4;   // sums, references and units, owners
-    static constexpr int SMEM = SUM_BYTES + WARPS * RING * TILE_BYTES;
-};
-
+constexpr int ROWS = 8, WARPS = 8;  // rows of a warp, warps of a block (two blocks an SM)
+constexpr int SUM_BYTES = WARPS * ROWS * (64 + 4 + 1) * 4;  // sums, references and units, owners
+constexpr int SMEM = SUM_BYTES + WARPS * RING * TILE_BYTES;
 constexpr int FOLD = 8;               // key tiles summed in the matrix unit's accumulators at a time
 
 // The slots of a kv head (and row block) are shared out so that the longest walk is the shortest: requests
@@ -191,10 +186,8 @@ __device__ __forceinline__ Share share_of(const PassArgs& a, int slot, int lane)
     return mine;
 }
 
-template <int KIND, int NT, bool SHARE>
-__global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pass_kernel(const PassArgs a) {
-    using R = Rows<NT>;
-    constexpr int LR = R::LANE;
+template <int KIND, bool SHARE>
+__global__ void __launch_bounds__(WARPS * 32, 2) kv8_pass_kernel(const PassArgs a) {
     // [warp][row][64] sums, [warp][row][2] reference and sum, [row] owner, [warp] ring
     extern __shared__ __align__(128) float smem[];  // KeyCopy places rows of the rings by their address bits
     if (!a.beside) pdl_wait();
@@ -227,51 +220,42 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
         part0 += (share.first - (long long)share.request * splits) * a.rows.rows * a.hq;
     }
     const int phase = warp % a.key_warps;
-    const int tile = row_block * (R::WARPS / a.key_warps) + warp / a.key_warps;
+    const int tile = row_block * (WARPS / a.key_warps) + warp / a.key_warps;
     UnitRows rows(a, unit);
-    const int e0 = tile * R::COUNT;
+    const int e0 = tile * ROWS;
     const bool any_row = e0 < rows.size();
-    if (any_row) rows.tile(e0, R::COUNT);
+    if (any_row) rows.tile(e0, ROWS);
     const KeyRange& r = rows.keys;
-    int row_of[LR], hi[LR], lo[LR];
-#pragma unroll
-    for (int i = 0; i < LR; i++) row_of[i] = any_row ? rows.pair(e0 + 8 * i + g, lo[i], hi[i]) : -1;
+    int hi, lo;  // keys of the lane's row, g
+    const int row_of = any_row ? rows.pair(e0 + g, lo, hi) : -1;
 
     // Sums of the rows in shared memory, in units of 2^at_off: the matrix unit drops the bits of a sum
     // that its 24 do not hold (it does not round them), so a long chain of products drifts towards
     // zero: 256 key tiles in one chain were 4e-6 off. Every FOLD tiles the registers are added here.
-    float* const acc = smem + (warp * R::COUNT + g) * 64 + 16 * t;  // row i of the lane: + 512 i
-    float off[LR], at_off[LR], lift[LR], sum[LR], v_unit = 0.f;  // see kv8_unit; v_unit divides the value scales
+    float4* const acc = reinterpret_cast<float4*>(smem + (warp * ROWS + g) * 64 + 16 * t);
+    float off = 0.f, at_off = 0.f, lift = KV8_UNSET, sum = 0.f, v_unit = 0.f;  // see kv8_unit; v_unit divides the value scales
     bool fresh = true;
-    float o[R::SETS][8][4];
-#pragma unroll
-    for (int i = 0; i < LR; i++) { off[i] = 0.f; at_off[i] = 0.f; lift[i] = KV8_UNSET; sum[i] = 0.f; }
+    float o[8][4];
     auto clear = [&]() {
 #pragma unroll
-        for (int n = 0; n < R::SETS; n++)
+        for (int i = 0; i < 8; i++)
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) o[n][i][j] = 0.f;
+            for (int j = 0; j < 4; j++) o[i][j] = 0.f;
     };
     clear();
     auto fold = [&](bool first) {
+        const float f = first ? 0.f : ex2(at_off - off);
+        at_off = off;
 #pragma unroll
-        for (int i = 0; i < LR; i++) {
-            const float f = first ? 0.f : ex2(at_off[i] - off[i]);
-            at_off[i] = off[i];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float4* at = reinterpret_cast<float4*>(acc + 512 * i) + j;
-                float4 y = first ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
-                auto add = [&](float& x, int d) {
-                    const int m = 4 * (j & 1) + d, col = j >> 1;
-                    const float v = NT == 0 ? o[0][m][col] + o[0][m][2 + col] : o[i / 2][m][2 * (i & 1) + col];
-                    x = first ? v : fmaf(x, f, v);
-                };
-                add(y.x, 0); add(y.y, 1); add(y.z, 2); add(y.w, 3);
-                *at = y;
-            }
+        for (int j = 0; j < 4; j++) {
+            float4 y = first ? make_float4(0.f, 0.f, 0.f, 0.f) : acc[j];
+            auto add = [&](float& x, int d) {
+                const float* const from = o[4 * (j & 1) + d] + (j >> 1);
+                const float v = from[0] + from[2];  // the planes
+                x = first ? v : fmaf(x, f, v);
+            };
+            add(y.x, 0); add(y.y, 1); add(y.z, 2); add(y.w, 3);
+            acc[j] = y;
         }
     };
 
@@ -282,22 +266,21 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
     bool folded = false;
     if (at < end) {
         const bool l1 = a.key_warps == 1;  // the block's warps read the same keys
-        const uint8_t* const ring = reinterpret_cast<const uint8_t*>(smem) + R::SUM_BYTES + warp * RING * TILE_BYTES;
+        const uint8_t* const ring = reinterpret_cast<const uint8_t*>(smem) + SUM_BYTES + warp * RING * TILE_BYTES;
         const KeyCopy copy(a.c, r, smem_u32(ring), lane, l1);
 #pragma unroll
         for (int i = 0; i < RING - 1; i++) {
             if (at + i * a.key_warps < end) copy.tile(r, (t0 + at + i * a.key_warps) * 16, i, lane);
             copies_commit();
         }
-        // Queries: 16 dimensions of each of the lane's rows, as fp16 planes of a power-of-two multiple.
-        uint32_t qa[R::SETS][R::PLANES][4][4];
-        float q_scale[LR];
-#pragma unroll
-        for (int i = 0; i < LR; i++) {
+        // Queries: 16 dimensions of the lane's row, as fp16 planes of a power-of-two multiple.
+        uint32_t qa[4][4];
+        float q_scale;
+        {
             float x[16];
             float top = 0.f;
-            if (row_of[i] >= 0) {
-                const int row = row_of[i] / a.hq, head = row_of[i] - row * a.hq;
+            if (row_of >= 0) {
+                const int row = row_of / a.hq, head = row_of - row * a.hq;
                 const float* src = a.q + (size_t)row * a.ldq + (size_t)head * 64 + 16 * t;
                 if (a.qvec) {
 #pragma unroll
@@ -318,18 +301,11 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const float up = power_to(top, 13);
-            q_scale[i] = 0.125f * 1.4426950408889634f / up;  // scores in powers of two
+            q_scale = 0.125f * 1.4426950408889634f / up;  // scores in powers of two
 #pragma unroll
             for (int s = 0; s < 4; s++) {
-                uint32_t h0, l0, h1, l1;
-                split_half2(x[4 * s] * up, x[4 * s + 1] * up, h0, l0);
-                split_half2(x[4 * s + 2] * up, x[4 * s + 3] * up, h1, l1);
-                if (NT == 0) {
-                    qa[0][0][s][0] = h0; qa[0][0][s][1] = l0; qa[0][0][s][2] = h1; qa[0][0][s][3] = l1;
-                } else {
-                    qa[i / 2][0][s][i & 1] = h0; qa[i / 2][0][s][2 + (i & 1)] = h1;
-                    qa[i / 2][R::PLANES - 1][s][i & 1] = l0; qa[i / 2][R::PLANES - 1][s][2 + (i & 1)] = l1;
-                }
+                split_half2(x[4 * s] * up, x[4 * s + 1] * up, qa[s][0], qa[s][1]);
+                split_half2(x[4 * s + 2] * up, x[4 * s + 3] * up, qa[s][2], qa[s][3]);
             }
         }
 
@@ -353,113 +329,74 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
             const float ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w};
             float vs[4] = {vs4.x, vs4.y, vs4.z, vs4.w};
 
-            // Scores (before scaling): 4 keys of each of the lane's rows.
-            float s[LR][4];
+            // Scores (before scaling): 4 keys of the lane's row.
+            float s[4];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const uint4 k = *reinterpret_cast<const uint4*>(x + (4 * (g >> 1) + 2 * j + (g & 1)) * 64 + 16 * t);
                 const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
-                float c[R::SETS][4];
-#pragma unroll
-                for (int n = 0; n < R::SETS; n++) { c[n][0] = 0.f; c[n][1] = 0.f; c[n][2] = 0.f; c[n][3] = 0.f; }
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
                     uint32_t b0, b1;
                     to_half<KIND>(kw[w], b0, b1);
-#pragma unroll
-                    for (int n = 0; n < R::SETS; n++)
-#pragma unroll
-                        for (int p = 0; p < R::PLANES; p++) mma16816(c[n], qa[n][p][w], b0, b1);
+                    mma16816(c, qa[w], b0, b1);
                 }
-                if (NT == 0) {
-                    s[0][2 * j] = c[0][0] + c[0][2];
-                    s[0][2 * j + 1] = c[0][1] + c[0][3];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < LR; i++) {
-                        s[i][2 * j] = c[i / 2][2 * (i & 1)];
-                        s[i][2 * j + 1] = c[i / 2][2 * (i & 1) + 1];
-                    }
-                }
+                s[2 * j] = c[0] + c[2];
+                s[2 * j + 1] = c[1] + c[3];
             }
             const bool whole = u0 >= r.in_lo && u0 + 15 <= r.in_hi;
             if (v_unit == 0.f) v_unit = value_unit(vs);
 #pragma unroll
-            for (int k = 0; k < 4; k++) vs[k] *= v_unit;
-#pragma unroll
-            for (int i = 0; i < LR; i++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) s[i][k] *= ks[k];
+            for (int k = 0; k < 4; k++) {
+                vs[k] *= v_unit;
+                s[k] *= ks[k];
+            }
             // Weights 2^(score - off), times the value rows' scales.
-            float w[LR][4], add[LR];
+            float w[4], add;
             auto weigh = [&](auto masked) {
-                bool fine = true;
+                float p[4];
 #pragma unroll
-                for (int i = 0; i < LR; i++) {
-                    float p[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        p[k] = ex2(fmaf(s[i][k], q_scale[i], -off[i]));
-                        w[i][k] = p[k] * vs[k];
-                        if (masked) {
-                            const bool on = u0 + 4 * t + k >= lo[i] && u0 + 4 * t + k <= hi[i];
-                            p[k] = on ? p[k] : 0.f;
-                            w[i][k] = on ? w[i][k] : 0.f;  // a scale of a key that this row does not see may be NaN
-                        }
+                for (int k = 0; k < 4; k++) {
+                    p[k] = ex2(fmaf(s[k], q_scale, -off));
+                    w[k] = p[k] * vs[k];
+                    if (masked) {
+                        const bool on = u0 + 4 * t + k >= lo && u0 + 4 * t + k <= hi;
+                        p[k] = on ? p[k] : 0.f;
+                        w[k] = on ? w[k] : 0.f;  // a scale of a key that this row does not see may be NaN
                     }
-                    add[i] = (p[0] + p[1]) + (p[2] + p[3]);
-                    fine = fine && fmaxf(fmaxf(fabsf(w[i][0]), fabsf(w[i][1])), fmaxf(fabsf(w[i][2]), fabsf(w[i][3]))) <= KV8_PRODUCT_MAX &&
-                           add[i] <= KV8_WEIGHT_MAX;
                 }
-                return fine;
+                add = (p[0] + p[1]) + (p[2] + p[3]);
+                return fmaxf(fmaxf(fabsf(w[0]), fabsf(w[1])), fmaxf(fabsf(w[2]), fabsf(w[3]))) <= KV8_PRODUCT_MAX &&
+                       add <= KV8_WEIGHT_MAX;
             };
             const bool fine = whole ? weigh(std::false_type{}) : weigh(std::true_type{});
             if (fresh || __any_sync(0xffffffffu, !fine)) {  // rare: a row's unit is set, or moves
-                bool unset = false;
+                float z[4], v[4];
 #pragma unroll
-                for (int i = 0; i < LR; i++) {
-                    float z[4], v[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const bool on = whole || (u0 + 4 * t + k >= lo[i] && u0 + 4 * t + k <= hi[i]);
-                        z[k] = on ? s[i][k] * q_scale[i] : -INFINITY;
-                        v[k] = on ? fabsf(vs[k]) : 0.f;
-                    }
-                    const float2 to = kv8_unit(z, v, off[i], lift[i]);
-                    if (to.x != off[i]) {
-                        const float f = ex2(off[i] - to.x);
-                        sum[i] *= f;
-#pragma unroll
-                        for (int n = 0; n < 8; n++) {
-                            if (NT == 0) {
-                                o[0][n][0] *= f; o[0][n][1] *= f; o[0][n][2] *= f; o[0][n][3] *= f;
-                            } else {
-                                o[i / 2][n][2 * (i & 1)] *= f;
-                                o[i / 2][n][2 * (i & 1) + 1] *= f;
-                            }
-                        }
-                    }
-                    off[i] = to.x;
-                    lift[i] = to.y;
-                    unset |= to.y == KV8_UNSET;
+                for (int k = 0; k < 4; k++) {
+                    const bool on = whole || (u0 + 4 * t + k >= lo && u0 + 4 * t + k <= hi);
+                    z[k] = on ? s[k] * q_scale : -INFINITY;
+                    v[k] = on ? fabsf(vs[k]) : 0.f;
                 }
-                fresh = __any_sync(0xffffffffu, unset);
+                const float2 to = kv8_unit(z, v, off, lift);
+                if (to.x != off) {
+                    const float f = ex2(off - to.x);
+                    sum *= f;
+#pragma unroll
+                    for (int n = 0; n < 8; n++) {
+                        o[n][0] *= f; o[n][1] *= f; o[n][2] *= f; o[n][3] *= f;
+                    }
+                }
+                off = to.x;
+                lift = to.y;
+                fresh = __any_sync(0xffffffffu, lift == KV8_UNSET);
                 weigh(std::true_type{});
             }
-            uint32_t pa[R::SETS][R::PLANES][4];
-#pragma unroll
-            for (int i = 0; i < LR; i++) {
-                uint32_t h0, l0, h1, l1;
-                sum[i] += add[i];
-                split_half2(w[i][0], w[i][1], h0, l0);
-                split_half2(w[i][2], w[i][3], h1, l1);
-                if (NT == 0) {
-                    pa[0][0][0] = h0; pa[0][0][1] = l0; pa[0][0][2] = h1; pa[0][0][3] = l1;
-                } else {
-                    pa[i / 2][0][i & 1] = h0; pa[i / 2][0][2 + (i & 1)] = h1;
-                    pa[i / 2][R::PLANES - 1][i & 1] = l0; pa[i / 2][R::PLANES - 1][2 + (i & 1)] = l1;
-                }
-            }
+            uint32_t pa[4];
+            sum += add;
+            split_half2(w[0], w[1], pa[0], pa[1]);
+            split_half2(w[2], w[3], pa[2], pa[3]);
             // Values: dimensions 8g .. 8g+7 of keys 4t .. 4t+3, the two keys of a pair side by side.
             uint2 v[4];
 #pragma unroll
@@ -475,48 +412,40 @@ __global__ void __launch_bounds__(Rows<NT>::WARPS * 32, Rows<NT>::BLOCKS) kv8_pa
                 to_half<KIND>(__byte_perm(v2, v3, 0x5140), b1[0], b1[1]);
                 to_half<KIND>(__byte_perm(v2, v3, 0x7362), b1[2], b1[3]);
 #pragma unroll
-                for (int d = 0; d < 4; d++)
-#pragma unroll
-                    for (int n = 0; n < R::SETS; n++)
-#pragma unroll
-                        for (int p = 0; p < R::PLANES; p++) mma16816(o[n][4 * h + d], pa[n][p], b0[d], b1[d]);
+                for (int d = 0; d < 4; d++) mma16816(o[4 * h + d], pa, b0[d], b1[d]);
             }
         }
     }
 
-    // Join the key_warps warps of each row tile.
+    // Merge the key_warps warps of each row tile.
     fold(!folded);
-    float4* sml = reinterpret_cast<float4*>(smem + R::WARPS * R::COUNT * 64);  // reference, sum; halves of the unit
-#pragma unroll
-    for (int i = 0; i < LR; i++) {
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-        const float2 ml = kv8_total(off[i], sum[i]);
-        const OverSum out(v_unit > 0.f ? 1.f / v_unit : 1.f, sum[i]);
-        if (t == 0) sml[warp * R::COUNT + 8 * i + g] = make_float4(ml.x, ml.y, out.first, out.second);
-    }
-    int* owner = reinterpret_cast<int*>(sml + R::WARPS * R::COUNT);
-    if (phase == 0 && t == 0) {
-#pragma unroll
-        for (int i = 0; i < LR; i++) owner[(warp / a.key_warps) * R::COUNT + 8 * i + g] = row_of[i];
+    float4* const ml = reinterpret_cast<float4*>(smem + WARPS * ROWS * 64);  // reference, sum; halves of the unit
+    int* const owner = reinterpret_cast<int*>(ml + WARPS * ROWS);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    if (t == 0) {
+        const float2 total = kv8_total(off, sum);
+        const OverSum out(v_unit > 0.f ? 1.f / v_unit : 1.f, sum);
+        ml[warp * ROWS + g] = make_float4(total.x, total.y, out.first, out.second);
+        if (phase == 0) owner[warp / a.key_warps * ROWS + g] = row_of;
     }
     __syncthreads();
-    const int rows_here = R::WARPS / a.key_warps * R::COUNT;
-    for (int e = threadIdx.x; e < rows_here * 16; e += R::WARPS * 32) {
+    const int rows_here = WARPS / a.key_warps * ROWS;
+    for (int e = threadIdx.x; e < rows_here * 16; e += WARPS * 32) {
         const int row = e >> 4, d4 = e & 15, target = owner[row];
         if (target < 0) continue;
-        const int base = (row / R::COUNT) * a.key_warps * R::COUNT + row % R::COUNT;
+        const int base = row / ROWS * a.key_warps * ROWS + row % ROWS;
         float top = KV8_REF_NONE, l = 0.f;
-        for (int k = 0; k < a.key_warps; k++) top = fmaxf(top, sml[base + k * R::COUNT].x);
-        for (int k = 0; k < a.key_warps; k++) l += ex2(sml[base + k * R::COUNT].x - top) * sml[base + k * R::COUNT].y;
+        for (int k = 0; k < a.key_warps; k++) top = fmaxf(top, ml[base + k * ROWS].x);
+        for (int k = 0; k < a.key_warps; k++) l += ex2(ml[base + k * ROWS].x - top) * ml[base + k * ROWS].y;
         const float over = rcp(l);
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int k = 0; k < a.key_warps; k++) {
-            const float4 ml = sml[base + k * R::COUNT];
-            const float f = ex2(ml.x - top) * ml.y * over;
-            const float4 v = reinterpret_cast<const float4*>(smem + (base + k * R::COUNT) * 64)[d4];
-            y.x += f * (v.x * ml.z * ml.w); y.y += f * (v.y * ml.z * ml.w);
-            y.z += f * (v.z * ml.z * ml.w); y.w += f * (v.w * ml.z * ml.w);
+            const float4 m = ml[base + k * ROWS];
+            const float f = ex2(m.x - top) * m.y * over;
+            const float4 v = reinterpret_cast<const float4*>(smem + (base + k * ROWS) * 64)[d4];
+            y.x += f * (v.x * m.z * m.w); y.y += f * (v.y * m.z * m.w);
+            y.z += f * (v.z * m.z * m.w); y.w += f * (v.w * m.z * m.w);
         }
         if (!a.parted) {
             const int qrow = target / a.hq, head = target - qrow * a.hq;
@@ -674,20 +603,21 @@ Kv8View view(const mt_kv8_cache* c) {
 // How a pass is laid out over the GPU.
 struct PassPlan {
     bool wide;
-    int nt, units, row_blocks, key_warps, splits, chunk, slots;
+    int units, row_blocks, key_warps, splits, chunk, slots;
 };
 
 // `units` row spaces of `qrows` (row, head) rows each over at most `keys` keys, `requests` of them of
-// lengths that may differ.
-PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows, int keys) {
+// lengths that may differ; the first row sees `unseen` fewer keys than the last.
+PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows, int keys, int unseen) {
     PassPlan p{};
     if (units < 1) return p;
-    // Which kernel: by their estimated times, in ns. The warp kernel takes 5.5 ps a (row, head) pair and key
-    // once the GPU is full; a wide block takes 14 us to start and finish and 2.2 us for 64 keys, and a later
-    // one on the same SM another 8 us. Measured in us, wide against warp kernel (one request, 14 heads on 2
-    // unless said): 16 rows over 300 keys 15.7 / 6.3, 512 over themselves 24.4 / 24.9, 37 over 4000 keys
-    // 23.5 / 20.8, 64 over 4000 23.9 / 32.7, 256 over 4000 29 / 74; 64 requests of 8 rows over 400 keys
-    // 18.8 / 18.1, of 16 rows 19.1 / 40.5; prefixes of 8000 for 16 requests 20.6 / 21.2, for 64 31.0 / 46.6.
+    // Which kernel: by their estimated times, in ns. The warp kernel takes 5 ps a (row, head) pair and key that
+    // it sees, once the GPU is full; a wide block takes 14 us to start and finish and 2.2 us for 64 keys, and a
+    // later one on the same SM another 8 us. Measured in us, wide against warp kernel (14 heads on 2 unless
+    // said): one request of 16 rows over 300 keys 15.5 / 6.3, 512 over themselves 24.4 / 20.4, 37 over 4000 keys
+    // 23.5 / 15.9, 64 over 4000 24.0 / 23.5; 8 requests of 64 rows over 1000 24.0 / 40.0; 64 requests of 8 rows
+    // over 400 keys 19.2 / 20.1, of 16 rows 19.5 / 34.6; 11 requests of 113 rows over 350, 16 heads on 16,
+    // 42.4 / 54.3; prefixes of 9000 for 32 requests 24.3 / 24.3, for 414 rows 67.9 / 293.
     {
         const long long row_blocks = (qrows + KV8_WIDE_ROWS - 1) / KV8_WIDE_ROWS, blocks = units * row_blocks;
         const long long tiles = (keys + 15 + KV8_WIDE_KEYS - 1) / KV8_WIDE_KEYS;
@@ -697,7 +627,7 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
         const long long chunk = (tiles + s - 1) / s, waves = (blocks * s + sm_count - 1) / sm_count;
         const long long each = blocks * tiles / sm_count;
         const double wide = 14e3 + 8e3 * (double)(waves - 1) + 2.2e3 * (double)(each > chunk ? each : chunk);
-        const double warp = 6e3 + 5.5e-3 * (double)units * (double)qrows * (double)keys;
+        const double warp = 6e3 + 5e-3 * (double)units * (double)qrows * ((double)keys - 0.5 * unseen);
         if (wide < warp) {
             p.wide = true;
             p.units = (int)units;
@@ -708,17 +638,11 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
         }
     }
     const int key_tiles = (keys + 15) / 16 + 1;
-    const long long warps_fit = 16ll * sm_count;
-    // Tiles of 8 rows while that leaves every SM room: a warp's chain of dependent steps is shortest.
-    // 16 or 32 rows convert each key's codes once for more rows.
-    const long long tiles8 = (qrows + 7) / 8;
-    p.nt = qrows <= 8 || units * tiles8 * ((key_tiles + 3) / 4) <= warps_fit ? 0 : qrows <= 16 ? 1 : 2;
-    const int count = p.nt == 0 ? 8 : 16 * p.nt, warps = p.nt == 0 ? 8 : 4;
-    const long long row_tiles = (qrows + count - 1) / count;
+    const long long row_tiles = (qrows + ROWS - 1) / ROWS;
     // Warps of a block: over the keys of one row tile, unless that makes more blocks than are resident
     // at once or there are not that many key tiles; then over row tiles.
-    auto blocks_at = [&](int kw) { return units * ((row_tiles + warps / kw - 1) / (warps / kw)); };
-    p.key_warps = warps;
+    auto blocks_at = [&](int kw) { return units * ((row_tiles + WARPS / kw - 1) / (WARPS / kw)); };
+    p.key_warps = WARPS;
     while (p.key_warps > 1 && (blocks_at(p.key_warps) > 2ll * sm_count || p.key_warps > key_tiles)) p.key_warps /= 2;
     p.units = (int)units;
     const long long blocks = blocks_at(p.key_warps);
@@ -732,7 +656,7 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
     // Slots by length where a warp's walk over the longest request would be 10 tiles or more: sharing them out
     // takes 0.8 us for 8 requests, 1.5 us for 64.
     const long long slots = 2ll * sm_count * requests / blocks;
-    if (requests > 1 && requests <= 32 * SHARE_LANES && slots > requests && slots - requests < MOST_SPLITS && most > 1 && keys <= 1 << 24 &&
+    if (p.splits > 1 && requests > 1 && requests <= 32 * SHARE_LANES && slots > requests && slots - requests < MOST_SPLITS && keys <= 1 << 24 &&
         key_tiles >= 10ll * p.key_warps * p.splits)
         p.slots = (int)(slots < most * requests ? slots : most * requests);
     return p;
@@ -750,9 +674,10 @@ Plan make_plan(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int
     const long long group = hq / hkv;
     const long long seen = window > 0 ? (long long)window + rows - 1 : cache->capacity;
     const long long size = (long long)rows * hq;
-    p.own = plan_pass(ctx->sm_count, (long long)requests * hkv, requests, rows * group, (int)(seen < cache->capacity ? seen : cache->capacity));
+    const int keys = (int)(seen < cache->capacity ? seen : cache->capacity);
+    p.own = plan_pass(ctx->sm_count, (long long)requests * hkv, requests, rows * group, keys, window > 0 ? 0 : rows - 1);
     if (prefix_len > 0) {
-        p.prefix = plan_pass(ctx->sm_count, hkv, 1, (long long)requests * rows * group, prefix_len);
+        p.prefix = plan_pass(ctx->sm_count, hkv, 1, (long long)requests * rows * group, prefix_len, 0);
         p.own0 = p.prefix.splits * requests * size;
     }
     if (prefix_len > 0 || p.own.splits > 1 || p.own.slots > 0) {
@@ -764,25 +689,17 @@ Plan make_plan(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int
     return p;
 }
 
-template <int KIND, int NT, bool SHARE>
+template <int KIND, bool SHARE>
 void launch_pass_as(const PassArgs& a, cudaStream_t s) {
-    using R = Rows<NT>;
     static PerDeviceOnce once;
-    once([] { cudaFuncSetAttribute(kv8_pass_kernel<KIND, NT, SHARE>, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM); });
+    once([] { cudaFuncSetAttribute(kv8_pass_kernel<KIND, SHARE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
     const int blocks = SHARE ? a.slots * a.hkv * a.row_blocks : a.units * a.row_blocks * a.splits;
-    launch_k(kv8_pass_kernel<KIND, NT, SHARE>, dim3((unsigned)blocks), R::WARPS * 32, R::SMEM, s, a);
+    launch_k(kv8_pass_kernel<KIND, SHARE>, dim3((unsigned)blocks), WARPS * 32, SMEM, s, a);
 }
 
-template <int KIND, int NT>
-void launch_pass_of(const PassArgs& a, cudaStream_t s) {
-    a.slots > 0 ? launch_pass_as<KIND, NT, true>(a, s) : launch_pass_as<KIND, NT, false>(a, s);
-}
-
-void launch_pass(const PassArgs& a, int nt, cudaStream_t s) {
-    if (a.c.kind == MT_KV_INT8)
-        nt == 0 ? launch_pass_of<MT_KV_INT8, 0>(a, s) : nt == 1 ? launch_pass_of<MT_KV_INT8, 1>(a, s) : launch_pass_of<MT_KV_INT8, 2>(a, s);
-    else
-        nt == 0 ? launch_pass_of<MT_KV_E4M3, 0>(a, s) : nt == 1 ? launch_pass_of<MT_KV_E4M3, 1>(a, s) : launch_pass_of<MT_KV_E4M3, 2>(a, s);
+void launch_pass(const PassArgs& a, cudaStream_t s) {
+    if (a.c.kind == MT_KV_INT8) a.slots > 0 ? launch_pass_as<MT_KV_INT8, true>(a, s) : launch_pass_as<MT_KV_INT8, false>(a, s);
+    else a.slots > 0 ? launch_pass_as<MT_KV_E4M3, true>(a, s) : launch_pass_as<MT_KV_E4M3, false>(a, s);
 }
 
 mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q, int ldq, int requests, int rows, int hq,
@@ -821,7 +738,7 @@ mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q,
         a.units = p.units; a.row_blocks = p.row_blocks; a.splits = p.splits; a.key_warps = p.key_warps;
         a.slots = p.slots; a.shares = shares;
         if (p.wide) launch_kv8_wide(a, p.chunk, ctx->d_status, s);
-        else launch_pass(a, p.nt, s);
+        else launch_pass(a, s);
     };
     const long long size = (long long)rows * hq;
     if (prefix_len > 0) {
