@@ -48,7 +48,8 @@ struct PassArgs {
     int requests, hq, hkv, group, window;
     Kv8View c;
     int prefix_len;                  // > 0: the prefix pass
-    int units, row_blocks, splits;   // grid: units x row_blocks x splits, or
+    int units, row_blocks, splits;   // grid: units (pack of them a block) x row_blocks x splits, or
+    int pack, unit_tiles;            // units with fewer row tiles (unit_tiles) than a block has room for share it
     int slots;                       // > 0: slots x kv heads x row_blocks, the slots shared out by length (kv8_share)
     int2* shares;                    // per request: its first slot and their number, for the join
     int key_warps;                   // warps of a block that share a row tile and interleave its keys

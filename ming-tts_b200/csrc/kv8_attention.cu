@@ -195,8 +195,9 @@ __global__ void __launch_bounds__(WARPS * 32, 2) kv8_pass_kernel(const PassArgs 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     // Blocks with the most keys (the last rows) first.
     int split = blockIdx.x % a.splits, splits = a.splits;
-    int unit = (blockIdx.x / a.splits) % a.units;
-    int row_block = a.row_blocks - 1 - blockIdx.x / (a.splits * a.units);
+    const int unit_blocks = (a.units + a.pack - 1) / a.pack, group = warp / a.key_warps;
+    int unit = (blockIdx.x / a.splits) % unit_blocks * a.pack + group / a.unit_tiles;
+    int row_block = a.row_blocks - 1 - blockIdx.x / (a.splits * unit_blocks);
     long long part0 = a.part0;
     if constexpr (SHARE) {
         const int kvh = blockIdx.x % a.hkv;
@@ -220,10 +221,10 @@ __global__ void __launch_bounds__(WARPS * 32, 2) kv8_pass_kernel(const PassArgs 
         part0 += (share.first - (long long)share.request * splits) * a.rows.rows * a.hq;
     }
     const int phase = warp % a.key_warps;
-    const int tile = row_block * (WARPS / a.key_warps) + warp / a.key_warps;
-    UnitRows rows(a, unit);
+    const int tile = row_block * (WARPS / a.key_warps) + group % a.unit_tiles;
+    UnitRows rows(a, min(unit, a.units - 1));
     const int e0 = tile * ROWS;
-    const bool any_row = e0 < rows.size();
+    const bool any_row = unit < a.units && group < a.pack * a.unit_tiles && e0 < rows.size();
     if (any_row) rows.tile(e0, ROWS);
     const KeyRange& r = rows.keys;
     int hi, lo;  // keys of the lane's row, g
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) kv8_pass_kernel(const PassArgs 
         const float2 total = kv8_total(off, sum);
         const OverSum out(v_unit > 0.f ? 1.f / v_unit : 1.f, sum);
         ml[warp * ROWS + g] = make_float4(total.x, total.y, out.first, out.second);
-        if (phase == 0) owner[warp / a.key_warps * ROWS + g] = row_of;
+        if (phase == 0) owner[group * ROWS + g] = row_of;
     }
     __syncthreads();
     const int rows_here = WARPS / a.key_warps * ROWS;
@@ -603,7 +604,7 @@ Kv8View view(const mt_kv8_cache* c) {
 // How a pass is laid out over the GPU.
 struct PassPlan {
     bool wide;
-    int units, row_blocks, key_warps, splits, chunk, slots;
+    int units, row_blocks, key_warps, pack, unit_tiles, splits, chunk, slots;
 };
 
 // `units` row spaces of `qrows` (row, head) rows each over at most `keys` keys, `requests` of them of
@@ -639,14 +640,20 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
     }
     const int key_tiles = (keys + 15) / 16 + 1;
     const long long row_tiles = (qrows + ROWS - 1) / ROWS;
-    // Warps of a block: over the keys of one row tile, unless that makes more blocks than are resident
-    // at once or there are not that many key tiles; then over row tiles.
-    auto blocks_at = [&](int kw) { return units * ((row_tiles + WARPS / kw - 1) / (WARPS / kw)); };
+    // Warps of a block: over the keys of one row tile, unless that makes more blocks than are resident at once
+    // or there are not that many key tiles; then over row tiles, of several units where one has too few.
+    auto pack_at = [&](int kw) { return row_tiles < WARPS / kw ? (int)(WARPS / kw / row_tiles) : 1; };
+    auto blocks_at = [&](int kw) {
+        const int pack = pack_at(kw);
+        return pack > 1 ? (units + pack - 1) / pack : units * ((row_tiles + WARPS / kw - 1) / (WARPS / kw));
+    };
     p.key_warps = WARPS;
     while (p.key_warps > 1 && (blocks_at(p.key_warps) > 2ll * sm_count || p.key_warps > key_tiles)) p.key_warps /= 2;
     p.units = (int)units;
+    p.pack = pack_at(p.key_warps);
+    p.unit_tiles = p.pack > 1 ? (int)row_tiles : WARPS;
     const long long blocks = blocks_at(p.key_warps);
-    p.row_blocks = (int)(blocks / units);
+    p.row_blocks = p.pack > 1 ? 1 : (int)(blocks / units);
     // Split the keys over as many blocks as are resident at once, while every warp keeps 4 tiles.
     long long s = 2ll * sm_count / blocks;
     const long long most = key_tiles / (4 * p.key_warps);
@@ -656,7 +663,7 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
     // Slots by length where a warp's walk over the longest request would be 10 tiles or more: sharing them out
     // takes 0.8 us for 8 requests, 1.5 us for 64.
     const long long slots = 2ll * sm_count * requests / blocks;
-    if (p.splits > 1 && requests > 1 && requests <= 32 * SHARE_LANES && slots > requests && slots - requests < MOST_SPLITS && keys <= 1 << 24 &&
+    if (p.splits > 1 && p.pack == 1 && requests > 1 && requests <= 32 * SHARE_LANES && slots > requests && slots - requests < MOST_SPLITS && keys <= 1 << 24 &&
         key_tiles >= 10ll * p.key_warps * p.splits)
         p.slots = (int)(slots < most * requests ? slots : most * requests);
     return p;
@@ -693,7 +700,7 @@ template <int KIND, bool SHARE>
 void launch_pass_as(const PassArgs& a, cudaStream_t s) {
     static PerDeviceOnce once;
     once([] { cudaFuncSetAttribute(kv8_pass_kernel<KIND, SHARE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
-    const int blocks = SHARE ? a.slots * a.hkv * a.row_blocks : a.units * a.row_blocks * a.splits;
+    const int blocks = SHARE ? a.slots * a.hkv * a.row_blocks : (a.units + a.pack - 1) / a.pack * a.row_blocks * a.splits;
     launch_k(kv8_pass_kernel<KIND, SHARE>, dim3((unsigned)blocks), WARPS * 32, SMEM, s, a);
 }
 
@@ -736,6 +743,7 @@ mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q,
     a.parted = plan.parts > 0;
     auto run = [&](const PassPlan& p) {
         a.units = p.units; a.row_blocks = p.row_blocks; a.splits = p.splits; a.key_warps = p.key_warps;
+        a.pack = p.pack; a.unit_tiles = p.unit_tiles;
         a.slots = p.slots; a.shares = shares;
         if (p.wide) launch_kv8_wide(a, p.chunk, ctx->d_status, s);
         else launch_pass(a, s);

@@ -667,10 +667,11 @@ def test_many_rows_extreme_scales(ctx, mt, kind):
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
-def test_many_rows_nan_reaches_only_rows_that_see_it(ctx, mt, kind):
+@pytest.mark.parametrize("rows", [900, 1500])
+def test_many_rows_nan_reaches_only_rows_that_see_it(ctx, mt, kind, rows):
     import torch
-    n, rows, hq = 900, 900, 8
-    for bad_at in (0, 450, 899):
+    n, hq = rows, 8
+    for bad_at in (0, 450, rows - 1):
         for which in (2, 3):
             cache = Cache(mt, kind, 2, n, [(0, n)], 9)
             cache.kv.tensors[which][0, 1, bad_at] = math.nan
@@ -686,6 +687,20 @@ def test_many_rows_nan_reaches_only_rows_that_see_it(ctx, mt, kind):
             want[bad_at:, 4:] = True
             want[600, 0] = True
             assert torch.equal(bad, want) and torch.equal(some, want)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hq,hkv,requests,rows", [(16, 16, 47, 2), (16, 16, 64, 8), (8, 8, 61, 9), (16, 16, 21, 17), (32, 32, 50, 1),
+                                                  (9, 3, 37, 5), (16, 1, 300, 1)])
+def test_many_small_requests(ctx, mt, kind, hq, hkv, requests, rows):
+    """More requests and heads than blocks: several share one."""
+    positions = [(13 * i) % 50 for i in range(requests)]
+    counts = [rows - i % (rows + 1) if i % 3 else rows for i in range(requests)]
+    check_attention(ctx, mt, kind, hq, hkv, 70, positions, rows)
+    check_attention(ctx, mt, kind, hq, hkv, 41, positions, rows, counts=counts, window=20)
+    check_attention(ctx, mt, kind, hq, hkv, 70, [p + 30 if i % 7 else -1 for i, p in enumerate(positions)], rows, counts=counts,
+                    prefix_len=30, pad_q=1, pad_o=2)
 
 
 @gpu
