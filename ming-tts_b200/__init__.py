@@ -327,6 +327,8 @@ class Context:
     def _enough(self, cache, requests: int):
         if cache.requests < requests:
             raise MingError(MT_ERR_SHAPE, f"{requests} requests, but a cache of {cache.requests}")
+        if cache.index != self.device:
+            raise MingError(MT_ERR_ARG, f"a cache on {cache.device}, but a context of cuda:{self.device}")
 
     def _workspace(self, nbytes: int, given):
         """(tensor, pointer, bytes): the caller's workspace, or a new one from torch's allocator."""
@@ -373,6 +375,8 @@ class Context:
         """mt_attention_prefix_kv8: attention over a prefix all requests share and each one's own cache.
         The workspace as in attention_kv8."""
         self._enough(cache, requests)
+        if prefix is not None:
+            self._enough(prefix, 1)
         need = lib().mt_attention_prefix_kv8_workspace(self._ctx, prefix_len, cache.ref, requests, rows, hq)
         keep, wp, wn = self._workspace(need, workspace) if need else (None, None, 0)
         st = lib().mt_attention_prefix_kv8(self._ctx, self._device_stream() if stream is None else stream, q.data_ptr(),
@@ -415,7 +419,7 @@ class KV8Cache:
                 raise ValueError(f"KV8Cache: strides {t.stride()} of a tensor [{requests}, {heads}, {capacity}, ...]")
         self.tensors = (k, v, k_scale, v_scale)  # kept alive
         self.k, self.v, self.k_scale, self.v_scale = self.tensors
-        self.requests, self.base, self.device = requests, base, k.device
+        self.requests, self.base, self.device, self.index = requests, base, k.device, k.device.index
         self.struct = KV8CacheStruct(kinds[k.dtype], heads, capacity, base, stride, *(t.data_ptr() for t in self.tensors))
         self.ref = ctypes.byref(self.struct)
 

@@ -314,14 +314,14 @@ extern "C" mt_status mt_rope_cache_kv8(mt_ctx* ctx, void* stream, const float* q
     a.rows = Kv8Rows{positions, counts, rows, cache->base};
     a.total = requests * rows; a.hq = hq; a.hkv = hkv;
     // One row a block until the rows are two waves of blocks: a decode step is bound by its latency.
-    const int per_sm = (a.total + 2 * ctx->sm_count - 1) / (2 * ctx->sm_count);
+    const int per_sm = (a.total - 1) / (2 * ctx->sm_count) + 1;
     a.block_rows = per_sm < AP_MAX_ROWS ? per_sm : AP_MAX_ROWS;
     a.parts = AP_THREADS / 8 / a.block_rows;
     a.vec = (((uintptr_t)qkv | (uintptr_t)q_out) & 15u) == 0 && ldq % 4 == 0 && ldqo % 4 == 0;
     a.inv_freq = inv_freq;
     a.k = cache->k; a.v = cache->v; a.k_scale = cache->k_scale; a.v_scale = cache->v_scale;
     a.request_stride = cache->request_stride; a.capacity = cache->capacity;
-    const int blocks = (a.total + a.block_rows - 1) / a.block_rows;
+    const int blocks = (a.total - 1) / a.block_rows + 1;
     launch_k(cache->kind == MT_KV_INT8 ? rope_cache_kv8_kernel<MT_KV_INT8> : rope_cache_kv8_kernel<MT_KV_E4M3>, blocks,
              AP_THREADS, 0, as_stream(stream), a);
     return check_launch(ctx, what);

@@ -62,6 +62,14 @@ struct PassArgs {
     bool beside;
 };
 
+// Begins a pass. Beside another, what the kernels before the call wrote is complete and in L2; the fence is
+// there for lines of it that this SM's L1 may still hold from an earlier step.
+__device__ __forceinline__ void pass_begin(bool beside) {
+    if (beside) asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    else pdl_wait();
+    pdl_launch();
+}
+
 // Where the keys of a tile of rows are. Index u counts positions from a multiple of the capacity, so that
 // slot(u) is u or u - capacity; the tile's rows see [lo, hi] at most, and all of [in_lo, in_hi].
 struct KeyRange {

@@ -21,12 +21,12 @@
 //     scores, column g of half j is key 4 (g / 2) + 2 j + g % 2, so lane t's scores are keys 4t .. 4t+3
 //     values, contraction index 2t, 2t+1, 2t+8, 2t+9 is key 4t .. 4t+3; column g of block i is dimension
 //     8 g + i, so lane t's outputs are dimensions 16 t .. 16 t + 15.
-// Bounded by instruction issue: 332 a tile of 16 keys, of which 32 are matrix instructions, 100 the conversion
-// of codes and 40 the weights, 57% of the issue slots used at 16 warps an SM; 64 requests of 8000 keys run at
-// 52% of the copy bandwidth. Tiles of 16 and 32 rows (the planes as operands of their own, each code
-// converted once for all of them) were 530 and 974 instructions a tile, but their registers leave room for 12
-// and 8 warps, which used 40% of the slots, and the fixed part of a call took 3 and 7 us longer: slower at
-// every size, or no faster. Many rows against many keys go to kv8_attention_wide.cu.
+// Bounded by instruction issue: 332 a tile of 16 keys, of which 16 are matrix instructions and some 90 the
+// conversion of codes, 57% of the issue slots used at 16 warps an SM; 64 requests of 8000 keys run at half of
+// the copy bandwidth. Tiles of 16 and 32 rows (the planes as operands of their own, each code converted once
+// for all of them) were no faster at any size: 974 instructions a tile of 32, but registers for 8 warps an
+// SM, which used 40% of the slots, and 16 rows over 300 keys took 9.1 and 13.6 us instead of 6.3. Many rows
+// against many keys go to kv8_attention_wide.cu.
 #include <math.h>
 
 #include <type_traits>
@@ -190,8 +190,7 @@ template <int KIND, bool SHARE>
 __global__ void __launch_bounds__(WARPS * 32, 2) kv8_pass_kernel(const PassArgs a) {
     // [warp][row][64] sums, [warp][row][2] reference and sum, [row] owner, [warp] ring
     extern __shared__ __align__(128) float smem[];  // KeyCopy places rows of the rings by their address bits
-    if (!a.beside) pdl_wait();
-    pdl_launch();
+    pass_begin(a.beside);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     // Blocks with the most keys (the last rows) first.
     int split = blockIdx.x % a.splits, splits = a.splits;
@@ -663,8 +662,8 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
     // Slots by length where a warp's walk over the longest request would be 10 tiles or more: sharing them out
     // takes 0.8 us for 8 requests, 1.5 us for 64.
     const long long slots = 2ll * sm_count * requests / blocks;
-    if (p.splits > 1 && p.pack == 1 && requests > 1 && requests <= 32 * SHARE_LANES && slots > requests && slots - requests < MOST_SPLITS && keys <= 1 << 24 &&
-        key_tiles >= 10ll * p.key_warps * p.splits)
+    if (p.splits > 1 && p.pack == 1 && requests > 1 && requests <= 32 * SHARE_LANES && slots > requests &&
+        slots - requests < MOST_SPLITS && keys <= 1 << 24 && key_tiles >= 10ll * p.key_warps * p.splits)
         p.slots = (int)(slots < most * requests ? slots : most * requests);
     return p;
 }

@@ -620,8 +620,7 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
 
 template <int KIND>
 __global__ void __launch_bounds__(WD_THREADS, 1) kv8_wide_kernel(const PassArgs a, int chunk, unsigned int* status) {
-    if (!a.beside) pdl_wait();
-    pdl_launch();
+    pass_begin(a.beside);
     wide_block<KIND>(a, chunk, status);
     if (a.beside) pdl_wait();
 }

@@ -114,6 +114,25 @@ def test_cache_object_refuses_other_layouts(mt):
         mt.KV8Cache(k, k, s, s)
 
 
+def test_calls_refuse_caches_of_fewer_requests_or_another_device(mt):
+    from types import SimpleNamespace
+    ctx = object.__new__(mt.Context)
+    ctx.device = 0
+    good = SimpleNamespace(requests=2, index=0, device="cuda:0")
+    for bad, status in ((SimpleNamespace(requests=1, index=0, device="cuda:0"), mt.MT_ERR_SHAPE),
+                        (SimpleNamespace(requests=2, index=1, device="cuda:1"), mt.MT_ERR_ARG)):
+        for call in (lambda: ctx.rope_cache_kv8(None, 1152, 2, 1, 14, None, None, None, bad, None, 896),
+                     lambda: ctx.kv8_read(bad, 2, 1, None, None, None, None, 1),
+                     lambda: ctx.attention_kv8(None, 896, 2, 1, 14, None, None, 0, bad, None, 896),
+                     lambda: ctx.attention_prefix_kv8(None, 896, 2, 1, 14, None, None, good, 3, bad, None, 896)):
+            with pytest.raises(mt.MingError) as e:
+                call()
+            assert e.value.status == status
+    with pytest.raises(mt.MingError):
+        ctx.attention_prefix_kv8(None, 896, 2, 1, 14, None, None, SimpleNamespace(requests=1, index=1, device="cuda:1"), 3, good,
+                                 None, 896)
+
+
 # ------------------------------------------------------------------------------------------------
 # The plain implementation, 64 bits
 # ------------------------------------------------------------------------------------------------
@@ -833,6 +852,41 @@ def test_shared_prefix_equals_copies(ctx, mt, kind):
     tol = 4 * (2 * 136 * 32 + 16 + 90) * 2.0 ** -24 * 6
     for x, y in zip(a, b):
         assert float((x - y).abs().max()) <= tol
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,plen,cap", [(3, 40, 90), (40, 1500, 90), (64, 4000, 100)])
+def test_steps_in_the_same_buffers(ctx, mt, kind, n, plen, cap):
+    """Steps one behind the other without a pause, in buffers that every step writes again: no kernel starts
+    on what an earlier step left there. The same as with the device idle between calls."""
+    import torch
+    hq, hkv, steps = 14, 2, 40
+    g = torch.Generator(device="cuda").manual_seed(8)
+    inv = torch.from_numpy(INV_FREQ).cuda()
+    prefix = Cache(mt, kind, hkv, plen, [(0, plen)], 1).kv
+    xs = torch.randn(steps, n, (hq + 2 * hkv) * 64, device="cuda", generator=g)
+    x, q, out = torch.empty_like(xs[0]), torch.empty(n, hq * 64, device="cuda"), torch.empty(n, hq * 64, device="cuda")
+    runs = []
+    for pause in (False, True):
+        cache = mt.KV8Cache.allocate(n, hkv, cap, torch_kind(kind), base=plen)
+        pos = torch.full((n,), plen, dtype=torch.int32, device="cuda")
+        outs = torch.zeros(steps, n, hq * 64, device="cuda")
+        work = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        for i in range(steps):
+            x.copy_(xs[i])
+            ctx.rope_cache_kv8(x, (hq + 2 * hkv) * 64, n, 1, hq, pos, None, inv, cache, q, hq * 64)
+            if pause:
+                torch.cuda.synchronize()
+            ctx.attention_prefix_kv8(q, hq * 64, n, 1, hq, pos, None, prefix, plen, cache, out, hq * 64, workspace=work)
+            if pause:
+                torch.cuda.synchronize()
+            outs[i] = out
+            pos += 1
+        ctx.check()
+        runs.append(outs)
+    assert torch.equal(runs[0], runs[1])
 
 
 @gpu
