@@ -250,12 +250,14 @@ __global__ void __launch_bounds__(RD_THREADS) kv8_read_kernel(ReadArgs a) {
     const Kv8Span s = kv8_span(a.rows, request);
     const int lane = threadIdx.x & 15;
     const size_t from = (size_t)request * a.request_stride + (size_t)head * a.capacity;
+    const int start = s.count > 0 ? (s.pos - a.rows.base) % a.capacity : 0;
     uint32_t w[2][RD_ROWS / 16];
     float sc[2][RD_ROWS / 16];
 #pragma unroll
     for (int i = 0; i < RD_ROWS / 16; i++) {
         const int row = tile * RD_ROWS + i * 16 + (threadIdx.x >> 4);
-        const size_t at = from + (row < s.count ? (s.pos + row - a.rows.base) % a.capacity : 0);
+        const int slot = row < s.count ? start + row : 0;  // row < capacity
+        const size_t at = from + (slot >= a.capacity ? slot - a.capacity : slot);
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             const bool on = row < s.count && a.out[t];
@@ -273,7 +275,9 @@ __global__ void __launch_bounds__(RD_THREADS) kv8_read_kernel(ReadArgs a) {
             float4 x;
             const uint32_t c = w[t][i];
             if (KIND == MT_KV_INT8) {
-                x = make_float4((float)(int8_t)c, (float)(int8_t)(c >> 8), (float)(int8_t)(c >> 16), (float)(int8_t)(c >> 24));
+                const uint32_t u = c ^ 0x80808080u;  // code + 128, the low byte of 2^23 + 128 + code
+                auto code = [u](uint32_t byte) { return __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540u | byte)) - 8388736.f; };
+                x = make_float4(code(0), code(1), code(2), code(3));
             } else {
                 const __half2 lo = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c & 0xFFFFu), __NV_E4M3));
                 const __half2 hi = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c >> 16), __NV_E4M3));

@@ -614,15 +614,16 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
     // Which kernel: by their estimated times, in ns. The warp kernel takes 5 ps a (row, head) pair and key that
     // it sees, once the GPU is full; a wide block takes 14 us to start and finish and 2.2 us for 64 keys, and a
     // later one on the same SM another 8 us. Measured in us, wide against warp kernel (14 heads on 2 unless
-    // said): one request of 16 rows over 300 keys 15.5 / 6.3, 512 over themselves 24.4 / 20.4, 37 over 4000 keys
-    // 23.5 / 15.9, 64 over 4000 24.0 / 23.5; 8 requests of 64 rows over 1000 24.0 / 40.0; 64 requests of 8 rows
-    // over 400 keys 19.2 / 20.1, of 16 rows 19.5 / 34.6; 11 requests of 113 rows over 350, 16 heads on 16,
-    // 42.4 / 54.3; prefixes of 9000 for 32 requests 24.3 / 24.3, for 414 rows 67.9 / 293.
+    // said): one request of 16 rows over 300 keys 12.6 / 6.4, 512 over themselves 21.5 / 20.1, 37 over 4000 keys
+    // 19.1 / 15.7, 64 over 4000 19.2 / 23.5; 8 requests of 64 rows over 1000 23.8 / 40.0; 64 requests of 8 rows
+    // over 400 keys 19.1 / 19.9, of 16 rows 19.4 / 34.6; 11 requests of 113 rows over 350, 16 heads on 16,
+    // 42.2 / 53.9; a prefix of 9000 for 32 requests 21.5 / 24.1, for 414 rows 64.8 / 291. Its keys are split over
+    // the SMs that its blocks leave free, two tiles a part or more (four: 64 rows over 4000 keys 24.0).
     {
         const long long row_blocks = (qrows + KV8_WIDE_ROWS - 1) / KV8_WIDE_ROWS, blocks = units * row_blocks;
         const long long tiles = (keys + 15 + KV8_WIDE_KEYS - 1) / KV8_WIDE_KEYS;
         long long s = (sm_count < MOST_SPLITS ? sm_count : MOST_SPLITS) / blocks;
-        if (s > tiles / 4) s = tiles / 4;
+        if (s > tiles / 2) s = tiles / 2;
         if (s < 1) s = 1;
         const long long chunk = (tiles + s - 1) / s, waves = (blocks * s + sm_count - 1) / sm_count;
         const long long each = blocks * tiles / sm_count;
