@@ -187,21 +187,20 @@ __device__ __forceinline__ Share share_of(const PassArgs& a, int slot, int lane)
 }
 
 template <int KIND, bool SHARE>
-__global__ void __launch_bounds__(WARPS * 32, 2) kv8_pass_kernel(const PassArgs a) {
+__device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
     // [warp][row][64] sums, [warp][row][2] reference and sum, [row] owner, [warp] ring
     extern __shared__ __align__(128) float smem[];  // KeyCopy places rows of the rings by their address bits
-    pass_begin(a.beside);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     // Blocks with the most keys (the last rows) first.
-    int split = blockIdx.x % a.splits, splits = a.splits;
+    int split = block % a.splits, splits = a.splits;
     const int unit_blocks = (a.units + a.pack - 1) / a.pack, group = warp / a.key_warps;
-    int unit = (blockIdx.x / a.splits) % unit_blocks * a.pack + group / a.unit_tiles;
-    int row_block = a.row_blocks - 1 - blockIdx.x / (a.splits * unit_blocks);
+    int unit = (block / a.splits) % unit_blocks * a.pack + group / a.unit_tiles;
+    int row_block = a.row_blocks - 1 - block / (a.splits * unit_blocks);
     long long part0 = a.part0;
     if constexpr (SHARE) {
-        const int kvh = blockIdx.x % a.hkv;
-        row_block = blockIdx.x / a.hkv % a.row_blocks;
-        const int slot = blockIdx.x / (a.hkv * a.row_blocks);
+        const int kvh = block % a.hkv;
+        row_block = block / a.hkv % a.row_blocks;
+        const int slot = block / (a.hkv * a.row_blocks);
         __shared__ Share shared_share;
         if (warp == 0) {
             const Share found = share_of(a, slot, lane);
@@ -209,10 +208,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) kv8_pass_kernel(const PassArgs 
         }
         __syncthreads();
         const Share share = shared_share;
-        if (share.parts == 0) {
-            if (a.beside) pdl_wait();
-            return;
-        }
+        if (share.parts == 0) return;
         if (threadIdx.x == 0) a.shares[share.request] = make_int2(share.first, share.parts);
         unit = share.request * a.hkv + kvh;
         split = slot - share.first;
@@ -461,7 +457,22 @@ __global__ void __launch_bounds__(WARPS * 32, 2) kv8_pass_kernel(const PassArgs 
             if (!(l == 0.f)) reinterpret_cast<float4*>(a.part_o + part * 64)[d4] = y;  // else not read
         }
     }
+}
+
+template <int KIND, bool SHARE>
+__global__ void __launch_bounds__(WARPS * 32, 2) kv8_pass_kernel(const PassArgs a) {
+    pass_begin(a.beside);
+    pass_block<KIND, SHARE>(a, blockIdx.x);
     if (a.beside) pdl_wait();
+}
+
+// The two passes of a call behind a prefix in one launch.
+template <int PREFIX_KIND, int KIND>
+__global__ void __launch_bounds__(WARPS * 32, 2) kv8_passes_kernel(const PassArgs prefix, const PassArgs own, int prefix_blocks) {
+    pass_begin(false);
+    const int block = blockIdx.x;
+    if (block < prefix_blocks) pass_block<PREFIX_KIND, false>(prefix, block);
+    else pass_block<KIND, false>(own, block - prefix_blocks);
 }
 
 // Joins the parts of each (row, head): out = sum_s w_s O_s, w_s = 2^(m_s - M) l_s / (the sum of these). A
@@ -696,17 +707,38 @@ Plan make_plan(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int
     return p;
 }
 
+unsigned pass_blocks(const PassArgs& a) {
+    return (unsigned)(a.slots > 0 ? a.slots * a.hkv * a.row_blocks : (a.units + a.pack - 1) / a.pack * a.row_blocks * a.splits);
+}
+
+template <typename... Params, typename... Args>
+void launch_warps(void (*kernel)(Params...), PerDeviceOnce& once, unsigned blocks, cudaStream_t s, const Args&... args) {
+    once([kernel] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
+    launch_k(kernel, dim3(blocks), WARPS * 32, SMEM, s, args...);
+}
+
 template <int KIND, bool SHARE>
 void launch_pass_as(const PassArgs& a, cudaStream_t s) {
     static PerDeviceOnce once;
-    once([] { cudaFuncSetAttribute(kv8_pass_kernel<KIND, SHARE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
-    const int blocks = SHARE ? a.slots * a.hkv * a.row_blocks : (a.units + a.pack - 1) / a.pack * a.row_blocks * a.splits;
-    launch_k(kv8_pass_kernel<KIND, SHARE>, dim3((unsigned)blocks), WARPS * 32, SMEM, s, a);
+    launch_warps(kv8_pass_kernel<KIND, SHARE>, once, pass_blocks(a), s, a);
 }
 
 void launch_pass(const PassArgs& a, cudaStream_t s) {
     if (a.c.kind == MT_KV_INT8) a.slots > 0 ? launch_pass_as<MT_KV_INT8, true>(a, s) : launch_pass_as<MT_KV_INT8, false>(a, s);
     else a.slots > 0 ? launch_pass_as<MT_KV_E4M3, true>(a, s) : launch_pass_as<MT_KV_E4M3, false>(a, s);
+}
+
+template <int PREFIX_KIND, int KIND>
+void launch_passes_as(const PassArgs& prefix, const PassArgs& own, cudaStream_t s) {
+    static PerDeviceOnce once;
+    launch_warps(kv8_passes_kernel<PREFIX_KIND, KIND>, once, pass_blocks(prefix) + pass_blocks(own), s, prefix, own, (int)pass_blocks(prefix));
+}
+
+void launch_passes(const PassArgs& prefix, const PassArgs& own, cudaStream_t s) {
+    if (prefix.c.kind == MT_KV_INT8)
+        own.c.kind == MT_KV_INT8 ? launch_passes_as<MT_KV_INT8, MT_KV_INT8>(prefix, own, s) : launch_passes_as<MT_KV_INT8, MT_KV_E4M3>(prefix, own, s);
+    else
+        own.c.kind == MT_KV_INT8 ? launch_passes_as<MT_KV_E4M3, MT_KV_INT8>(prefix, own, s) : launch_passes_as<MT_KV_E4M3, MT_KV_E4M3>(prefix, own, s);
 }
 
 mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q, int ldq, int requests, int rows, int hq,
@@ -741,21 +773,29 @@ mt_status attention(mt_ctx* ctx, const char* what, void* stream, const float* q,
     a.part_ml = a.part_o + plan.o_bytes / sizeof(float);
     int2* const shares = reinterpret_cast<int2*>(static_cast<char*>(workspace) + plan.o_bytes + plan.ml_bytes);
     a.parted = plan.parts > 0;
-    auto run = [&](const PassPlan& p) {
+    auto lay_out = [&](const PassPlan& p) {
         a.units = p.units; a.row_blocks = p.row_blocks; a.splits = p.splits; a.key_warps = p.key_warps;
         a.pack = p.pack; a.unit_tiles = p.unit_tiles;
         a.slots = p.slots; a.shares = shares;
+    };
+    auto run = [&](const PassPlan& p) {
         if (p.wide) launch_kv8_wide(a, p.chunk, ctx->d_status, s);
         else launch_pass(a, s);
     };
     const long long size = (long long)rows * hq;
+    const bool together = prefix_len > 0 && !plan.prefix.wide && !plan.own.wide && plan.own.slots == 0;
+    PassArgs before{};
     if (prefix_len > 0) {
+        lay_out(plan.prefix);
         a.c = view(prefix); a.prefix_len = prefix_len; a.part0 = 0;
-        run(plan.prefix);
+        if (together) before = a;
+        else run(plan.prefix);
     }
+    lay_out(plan.own);
     a.c = view(cache); a.prefix_len = 0; a.part0 = plan.own0; a.window = window;
-    a.beside = prefix_len > 0;
-    run(plan.own);
+    a.beside = prefix_len > 0 && !together;
+    if (together) launch_passes(before, a, s);
+    else run(plan.own);
     if (a.parted) {
         const JoinArgs j{a.rows, hq, plan.own.splits, plan.prefix.splits, plan.own.slots > 0 ? shares : nullptr,
                          plan.own0, a.part_o, a.part_ml, out, ldo, a.ovec};
