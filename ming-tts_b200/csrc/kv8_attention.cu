@@ -118,7 +118,7 @@ constexpr int FOLD = 8;               // key tiles summed in the matrix unit's a
 // The slots of a kv head (and row block) are shared out so that the longest walk is the shortest: requests
 // get ceil(rounds / q) each, with the smallest q that the slots allow, a round being a key tile for each of
 // the block's warps. Every block computes the same from all positions. With an equal number of slots each,
-// 8 requests of 4000 to 32000 keys took as long as 8 of 32000.
+// 8 requests of 4000 to 32768 keys took 23.1 us, nearly as long as 8 of 32000; so they take 19.4.
 constexpr int SHARE_LANES = 5;  // requests per lane at most
 struct Share {
     int request, first, parts;  // parts 0: no request's slot
@@ -188,7 +188,7 @@ __device__ __forceinline__ Share share_of(const PassArgs& a, int slot, int lane)
 
 template <int KIND, bool SHARE>
 __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
-    // [warp][row][64] sums, [warp][row][2] reference and sum, [row] owner, [warp] ring
+    // [warp][row][64] sums, [warp][row][4] reference, sum and unit, [row] owner, [warp] ring
     extern __shared__ __align__(128) float smem[];  // KeyCopy places rows of the rings by their address bits
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     // Blocks with the most keys (the last rows) first.

@@ -26,6 +26,10 @@
 // columns to 4 registers: lane (g, t) = (lane / 4, lane % 4) has columns 2t, 2t+1 of every 8, of rows g
 // and g + 8 (its slots 0 and 1). Four such warps a scheduler hide one another's latencies: with 8 warps of
 // 32 rows a key tile took 3400 cycles, of which 2200 were these warps' own.
+//
+// Bounded by the row warps' issue (69% of the SM's slots): 2.2 us for 64 keys of 256 rows in the steady state,
+// 14 us more for a block's start and end. 4096 rows over themselves, 14 heads on 2: 132 us, 458 TFLOP/s of matrix
+// work in two planes; the warp kernel took 304.
 #include <math.h>
 
 #include "kv8.cuh"
