@@ -330,6 +330,13 @@ class Context:
         if cache.index != self.device:
             raise MingError(MT_ERR_ARG, f"a cache on {cache.device}, but a context of cuda:{self.device}")
 
+    def _places(self, requests: int, positions, counts):
+        import torch
+        for t in (positions, counts):
+            if t is not None and (t.dtype != torch.int32 or t.numel() < requests or not t.is_contiguous()):
+                raise TypeError(f"positions and counts are dense torch.int32 of {requests} requests, got {t.dtype} "
+                                f"{tuple(t.shape)}")
+
     def _workspace(self, nbytes: int, given):
         """(tensor, pointer, bytes): the caller's workspace, or a new one from torch's allocator."""
         if given is None:
@@ -340,6 +347,7 @@ class Context:
     def rope_cache_kv8(self, qkv, ldq, requests, rows, hq, positions, counts, inv_freq, cache, q_out, ldqo, stream=None):
         """mt_rope_cache_kv8: rotate q and k, quantise k and v into the cache."""
         self._enough(cache, requests)
+        self._places(requests, positions, counts)
         st = lib().mt_rope_cache_kv8(self._ctx, self._device_stream() if stream is None else stream, qkv.data_ptr(), ldq,
                                      requests, rows, hq, positions.data_ptr(),
                                      None if counts is None else counts.data_ptr(), inv_freq.data_ptr(), cache.ref,
@@ -350,6 +358,7 @@ class Context:
     def kv8_read(self, cache, requests, rows, positions, counts, k, v, out_capacity, stream=None):
         """mt_kv8_read: a range of positions back into fp32."""
         self._enough(cache, requests)
+        self._places(requests, positions, counts)
         st = lib().mt_kv8_read(self._ctx, self._device_stream() if stream is None else stream, cache.ref, requests, rows,
                                positions.data_ptr(), None if counts is None else counts.data_ptr(), ptr(k), ptr(v),
                                out_capacity)
@@ -361,6 +370,7 @@ class Context:
         """mt_attention_kv8: causal attention over the cache. Without a workspace (a CUDA tensor), one comes
         from torch's allocator on the current stream: give one when `stream` is another."""
         self._enough(cache, requests)
+        self._places(requests, positions, counts)
         need = lib().mt_attention_kv8_workspace(self._ctx, cache.ref, requests, rows, hq, window)
         keep, wp, wn = self._workspace(need, workspace) if need else (None, None, 0)
         st = lib().mt_attention_kv8(self._ctx, self._device_stream() if stream is None else stream, q.data_ptr(), ldq,
@@ -377,6 +387,7 @@ class Context:
         self._enough(cache, requests)
         if prefix is not None:
             self._enough(prefix, 1)
+        self._places(requests, positions, counts)
         need = lib().mt_attention_prefix_kv8_workspace(self._ctx, prefix_len, cache.ref, requests, rows, hq)
         keep, wp, wn = self._workspace(need, workspace) if need else (None, None, 0)
         st = lib().mt_attention_prefix_kv8(self._ctx, self._device_stream() if stream is None else stream, q.data_ptr(),

@@ -133,6 +133,23 @@ def test_calls_refuse_caches_of_fewer_requests_or_another_device(mt):
                                  None, 896)
 
 
+def test_calls_refuse_positions_of_another_type(mt):
+    import torch
+    from types import SimpleNamespace
+    ctx = object.__new__(mt.Context)
+    ctx.device = 0
+    cache = SimpleNamespace(requests=2, index=0, device="cuda:0")
+    good = torch.zeros(2, dtype=torch.int32)
+    for pos, counts in ((good.long(), None), (good[:1], None), (torch.zeros(4, dtype=torch.int32)[::2], None), (good, good.long()),
+                        (good, good[:1])):
+        for call in (lambda: ctx.rope_cache_kv8(None, 1152, 2, 1, 14, pos, counts, None, cache, None, 896),
+                     lambda: ctx.kv8_read(cache, 2, 1, pos, counts, None, None, 1),
+                     lambda: ctx.attention_kv8(None, 896, 2, 1, 14, pos, counts, 0, cache, None, 896),
+                     lambda: ctx.attention_prefix_kv8(None, 896, 2, 1, 14, pos, counts, cache, 3, cache, None, 896)):
+            with pytest.raises(TypeError):
+                call()
+
+
 # ------------------------------------------------------------------------------------------------
 # The plain implementation, 64 bits
 # ------------------------------------------------------------------------------------------------
