@@ -102,10 +102,12 @@ struct UnitRows {
         keys.capacity = a.c.capacity;
         keys.row = (size_t)request * a.c.request_stride + (size_t)kvh * a.c.capacity;
         shift = 0;
-        if (!prefix) {
-            span = kv8_span(a.rows, request);
-            first = max(a.rows.base, span.pos + span.count - a.c.capacity);
-        }
+    }
+    // Reads the request's span: the rest needs it.
+    __device__ __forceinline__ void locate() {
+        if (a.prefix_len > 0) return;
+        span = kv8_span(a.rows, request);
+        first = max(a.rows.base, span.pos + span.count - a.c.capacity);
     }
     // (row, head) pairs of the unit.
     __device__ __forceinline__ int size() const {

@@ -198,6 +198,7 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
     int row_block = a.row_blocks - 1 - block / (a.splits * unit_blocks);
     long long part0 = a.part0;
     if constexpr (SHARE) {
+        pass_begin(a.beside);
         const int kvh = block % a.hkv;
         row_block = block / a.hkv % a.row_blocks;
         const int slot = block / (a.hkv * a.row_blocks);
@@ -218,6 +219,8 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
     const int phase = warp % a.key_warps;
     const int tile = row_block * (WARPS / a.key_warps) + group % a.unit_tiles;
     UnitRows rows(a, min(unit, a.units - 1));
+    if constexpr (!SHARE) pass_begin(a.beside);  // the indices above are computed while the kernel before ends
+    rows.locate();
     const int e0 = tile * ROWS;
     const bool any_row = unit < a.units && group < a.pack * a.unit_tiles && e0 < rows.size();
     if (any_row) rows.tile(e0, ROWS);
@@ -263,6 +266,25 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
     if (at < end) {
         const bool l1 = a.key_warps == 1;  // the block's warps read the same keys
         const uint8_t* const ring = reinterpret_cast<const uint8_t*>(smem) + SUM_BYTES + warp * RING * TILE_BYTES;
+        // The queries' loads go first: they are back when the first key tiles are.
+        float x[16];
+        if (row_of >= 0) {
+            const int row = row_of / a.hq, head = row_of - row * a.hq;
+            const float* src = a.q + (size_t)row * a.ldq + (size_t)head * 64 + 16 * t;
+            if (a.qvec) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float4 f = reinterpret_cast<const float4*>(src)[j];
+                    x[4 * j] = f.x; x[4 * j + 1] = f.y; x[4 * j + 2] = f.z; x[4 * j + 3] = f.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; j++) x[j] = src[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) x[j] = 0.f;
+        }
         const KeyCopy copy(a.c, r, smem_u32(ring), lane, l1);
 #pragma unroll
         for (int i = 0; i < RING - 1; i++) {
@@ -273,25 +295,7 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
         uint32_t qa[4][4];
         float q_scale;
         {
-            float x[16];
             float top = 0.f;
-            if (row_of >= 0) {
-                const int row = row_of / a.hq, head = row_of - row * a.hq;
-                const float* src = a.q + (size_t)row * a.ldq + (size_t)head * 64 + 16 * t;
-                if (a.qvec) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float4 f = reinterpret_cast<const float4*>(src)[j];
-                        x[4 * j] = f.x; x[4 * j + 1] = f.y; x[4 * j + 2] = f.z; x[4 * j + 3] = f.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 16; j++) x[j] = src[j];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 16; j++) x[j] = 0.f;
-            }
 #pragma unroll
             for (int j = 0; j < 16; j++) top = fmaxf(top, fabsf(x[j]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -366,8 +370,9 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
                 return fmaxf(fmaxf(fabsf(w[0]), fabsf(w[1])), fmaxf(fabsf(w[2]), fabsf(w[3]))) <= KV8_PRODUCT_MAX &&
                        add <= KV8_WEIGHT_MAX;
             };
-            const bool fine = whole ? weigh(std::false_type{}) : weigh(std::true_type{});
-            if (fresh || __any_sync(0xffffffffu, !fine)) {  // rare: a row's unit is set, or moves
+            bool fine = false;
+            if (!fresh) fine = whole ? weigh(std::false_type{}) : weigh(std::true_type{});
+            if (__any_sync(0xffffffffu, !fine)) {  // rare: a row's unit is set, or moves
                 float z[4], v[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -431,17 +436,28 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
         const int row = e >> 4, d4 = e & 15, target = owner[row];
         if (target < 0) continue;
         const int base = row / ROWS * a.key_warps * ROWS + row % ROWS;
+        float4 m[WARPS], v[WARPS];  // all loads before the first use
         float top = KV8_REF_NONE, l = 0.f;
-        for (int k = 0; k < a.key_warps; k++) top = fmaxf(top, ml[base + k * ROWS].x);
-        for (int k = 0; k < a.key_warps; k++) l += ex2(ml[base + k * ROWS].x - top) * ml[base + k * ROWS].y;
+#pragma unroll
+        for (int k = 0; k < WARPS; k++) {
+            const bool on = k < a.key_warps;
+            m[k] = on ? ml[base + k * ROWS] : make_float4(KV8_REF_NONE, 0.f, 0.f, 0.f);
+            v[k] = on ? reinterpret_cast<const float4*>(smem + (base + k * ROWS) * 64)[d4] : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < WARPS; k++) top = fmaxf(top, m[k].x);
+#pragma unroll
+        for (int k = 0; k < WARPS; k++) {
+            m[k].y *= ex2(m[k].x - top);
+            l += m[k].y;
+        }
         const float over = rcp(l);
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < a.key_warps; k++) {
-            const float4 m = ml[base + k * ROWS];
-            const float f = ex2(m.x - top) * m.y * over;
-            const float4 v = reinterpret_cast<const float4*>(smem + (base + k * ROWS) * 64)[d4];
-            y.x += f * (v.x * m.z * m.w); y.y += f * (v.y * m.z * m.w);
-            y.z += f * (v.z * m.z * m.w); y.w += f * (v.w * m.z * m.w);
+#pragma unroll
+        for (int k = 0; k < WARPS; k++) {
+            const float f = m[k].y * over;
+            y.x += f * (v[k].x * m[k].z * m[k].w); y.y += f * (v[k].y * m[k].z * m[k].w);
+            y.z += f * (v[k].z * m[k].z * m[k].w); y.w += f * (v[k].w * m[k].z * m[k].w);
         }
         if (!a.parted) {
             const int qrow = target / a.hq, head = target - qrow * a.hq;
@@ -461,7 +477,6 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
 
 template <int KIND, bool SHARE>
 __global__ void __launch_bounds__(WARPS * 32, 2) kv8_pass_kernel(const PassArgs a) {
-    pass_begin(a.beside);
     pass_block<KIND, SHARE>(a, blockIdx.x);
     if (a.beside) pdl_wait();
 }
@@ -469,7 +484,6 @@ __global__ void __launch_bounds__(WARPS * 32, 2) kv8_pass_kernel(const PassArgs 
 // The two passes of a call behind a prefix in one launch.
 template <int PREFIX_KIND, int KIND>
 __global__ void __launch_bounds__(WARPS * 32, 2) kv8_passes_kernel(const PassArgs prefix, const PassArgs own, int prefix_blocks) {
-    pass_begin(false);
     const int block = blockIdx.x;
     if (block < prefix_blocks) pass_block<PREFIX_KIND, false>(prefix, block);
     else pass_block<KIND, false>(own, block - prefix_blocks);

@@ -293,6 +293,8 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
     const int unit = (blockIdx.x / a.splits) % a.units;
     const int row_block = a.row_blocks - 1 - blockIdx.x / (a.splits * a.units);
     UnitRows rows(a, unit);
+    pass_begin(a.beside);
+    rows.locate();
     const int e0 = row_block * KV8_WIDE_ROWS, left = rows.size() - e0;
     if (left <= 0) return;
     rows.tile(e0, KV8_WIDE_ROWS);
@@ -624,7 +626,6 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
 
 template <int KIND>
 __global__ void __launch_bounds__(WD_THREADS, 1) kv8_wide_kernel(const PassArgs a, int chunk, unsigned int* status) {
-    pass_begin(a.beside);
     wide_block<KIND>(a, chunk, status);
     if (a.beside) pdl_wait();
 }
