@@ -246,10 +246,10 @@ struct ReadArgs {
 // of a thread (four rows of keys, four of values) are issued before the first is used.
 template <int KIND>
 __global__ void __launch_bounds__(RD_THREADS) kv8_read_kernel(ReadArgs a) {
-    pdl_wait();
-    pdl_launch();
     const int tile = blockIdx.x % a.tiles, unit = blockIdx.x / a.tiles;
     const int head = unit % a.hkv, request = unit / a.hkv;
+    pdl_wait();
+    pdl_launch();
     const Kv8Span s = kv8_span(a.rows, request);
     const int lane = threadIdx.x & 15;
     const size_t from = (size_t)request * a.request_stride + (size_t)head * a.capacity;

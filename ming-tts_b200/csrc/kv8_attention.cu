@@ -507,10 +507,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const JoinArgs a
     __shared__ float2 weight[2 * MOST_SPLITS];  // (reference, sum), then (weight, -)
     __shared__ float warp_top[JOIN_THREADS / 32], warp_sum[JOIN_THREADS / 32];
     __shared__ float4 partial[JOIN_THREADS / 32][16];
-    pdl_wait();
-    pdl_launch();
     const int group = threadIdx.x >> 4, d4 = threadIdx.x & 15, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = blockIdx.x / a.hq, request = row / a.rows.rows;
+    pdl_wait();
+    pdl_launch();
     if (row - request * a.rows.rows >= kv8_span(a.rows, request).count) return;
     const int2 own = a.shares ? a.shares[request] : make_int2(request * a.splits, a.splits);
     const int parts = a.prefix_splits + own.y;
@@ -578,11 +578,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_kernel(const JoinArgs a
 // The same for at most JOIN_GROUPS parts: a group of 16 lanes a (row, head), every lane all weights. The
 // reductions over a block above take 0.5 us longer.
 __global__ void __launch_bounds__(JOIN_THREADS) kv8_join_few_kernel(const JoinArgs a, int pairs) {
+    const int pair = blockIdx.x * JOIN_GROUPS + (threadIdx.x >> 4), d4 = threadIdx.x & 15;
+    const int row = pair / a.hq, request = row / a.rows.rows;
     pdl_wait();
     pdl_launch();
-    const int pair = blockIdx.x * JOIN_GROUPS + (threadIdx.x >> 4), d4 = threadIdx.x & 15;
     if (pair >= pairs) return;
-    const int row = pair / a.hq, request = row / a.rows.rows;
     if (row - request * a.rows.rows >= kv8_span(a.rows, request).count) return;
     const long long prefix_at = (long long)pair * a.prefix_splits, own_at = a.own0 + (long long)pair * a.splits - a.prefix_splits;
     const int parts = a.prefix_splits + a.splits;
