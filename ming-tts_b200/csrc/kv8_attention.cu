@@ -118,7 +118,7 @@ constexpr int FOLD = 8;               // key tiles summed in the matrix unit's a
 // The slots of a kv head (and row block) are shared out so that the longest walk is the shortest: requests
 // get ceil(rounds / q) each, with the smallest q that the slots allow, a round being a key tile for each of
 // the block's warps. Every block computes the same from all positions. With an equal number of slots each,
-// 8 requests of 4000 to 32768 keys took 23.1 us, nearly as long as 8 of 32000; so they take 19.4.
+// 8 requests of 4000 to 32768 keys took 23.1 us, nearly as long as 8 of 32000; so they took 19.4.
 constexpr int SHARE_LANES = 5;  // requests per lane at most
 struct Share {
     int request, first, parts;  // parts 0: no request's slot
@@ -637,10 +637,12 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
     PassPlan p{};
     if (units < 1) return p;
     // Which kernel: by their estimated times, in ns. The warp kernel takes 5 ps a (row, head) pair and key that
-    // it sees, once the GPU is full; a wide block takes 14 us to start and finish and 2.2 us for 64 keys, and a
-    // later one on the same SM another 8 us. Measured in us, wide against warp kernel (14 heads on 2 unless
-    // said): one request of 16 rows over 300 keys 12.6 / 6.4, 512 over themselves 21.5 / 20.1, 37 over 4000 keys
-    // 19.1 / 15.7, 64 over 4000 19.2 / 23.5; 8 requests of 64 rows over 1000 23.8 / 40.0; 64 requests of 8 rows
+    // it sees, once the GPU is full; a wide block takes 14 us to start and finish, 2.2 us for 64 keys (1.4 us
+    // with up to 128 rows), and a later one on the same SM another 8 us. Measured in us, wide against warp
+    // kernel (14 heads on 2 unless said): one request of 16 rows over 300 keys 12.6 / 6.4, 16 over 4000
+    // 15.1 / 11.6, 512 over themselves 21.5 / 20.1, 37 over 4000 keys
+    // 19.1 / 15.7, 64 over 4000 19.2 / 23.5; 8 requests of 8 rows over 4000 22.1 / 26.4,
+    // of 64 rows over 1000 23.8 / 40.0; 64 requests of 8 rows
     // over 400 keys 19.1 / 19.9, of 16 rows 19.4 / 34.6; 11 requests of 113 rows over 350, 16 heads on 16,
     // 42.2 / 53.9; a prefix of 9000 for 32 requests 21.5 / 24.1, for 414 rows 64.8 / 291. Its keys are split over
     // the SMs that its blocks leave free, two tiles a part or more (four: 64 rows over 4000 keys 24.0).
@@ -652,7 +654,8 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
         if (s < 1) s = 1;
         const long long chunk = (tiles + s - 1) / s, waves = (blocks * s + sm_count - 1) / sm_count;
         const long long each = blocks * tiles / sm_count;
-        const double wide = 14e3 + 8e3 * (double)(waves - 1) + 2.2e3 * (double)(each > chunk ? each : chunk);
+        const double tile = qrows <= KV8_WIDE_ROWS / 2 ? 1.4e3 : 2.2e3;
+        const double wide = 14e3 + 8e3 * (double)(waves - 1) + tile * (double)(each > chunk ? each : chunk);
         const double warp = 6e3 + 5e-3 * (double)units * (double)qrows * ((double)keys - 0.5 * unseen);
         if (wide < warp) {
             p.wide = true;
