@@ -908,11 +908,12 @@ def test_steps_in_the_same_buffers(ctx, mt, kind, n, plen, cap):
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
-def test_captured_steps_replay(ctx, mt, kind):
+@pytest.mark.parametrize("n,plen", [(3, 700), (64, 4000)])
+def test_captured_steps_replay(ctx, mt, kind, n, plen):
     """A captured step (append, attention behind a prefix) replayed as positions advance on the device; two
     graphs replayed at once on two streams; results equal the eager ones bit for bit."""
     import torch
-    hq, hkv, n, plen, steps = 14, 2, 3, 700, 5
+    hq, hkv, steps = 14, 2, 5
     g = torch.Generator(device="cuda").manual_seed(6)
     inv = torch.from_numpy(INV_FREQ).cuda()
     prefix = Cache(mt, kind, hkv, plen, [(0, plen)], 1).kv
