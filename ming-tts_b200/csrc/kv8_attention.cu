@@ -692,7 +692,7 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
     // takes 0.8 us for 8 requests, 1.5 us for 64.
     const long long slots = 2ll * sm_count * requests / blocks;
     if (p.splits > 1 && p.pack == 1 && requests > 1 && requests <= 32 * SHARE_LANES && slots > requests &&
-        slots - requests < MOST_SPLITS && keys <= 1 << 24 && key_tiles >= 10ll * p.key_warps * p.splits)
+        slots <= MOST_SPLITS && keys <= 1 << 24 && key_tiles >= 10ll * p.key_warps * p.splits)
         p.slots = (int)(slots < most * requests ? slots : most * requests);
     return p;
 }
