@@ -146,7 +146,7 @@ struct UnitRows {
     }
 };
 
-constexpr float KV8_REF_NONE = -1.7e38f;  // reference of a row that has seen no key
+constexpr float KV8_REF_NONE = -3.4028235e38f;  // reference of a row that has seen no key: no score is below it
 
 // The kernel for many rows (kv8_attention_wide.cu): blocks of KV8_WIDE_ROWS rows, `splits` parts of
 // `chunk` tiles of KV8_WIDE_KEYS keys each.
@@ -202,7 +202,7 @@ __device__ __forceinline__ float power_to(float x, int target) {
 // set: the two planes hold 22 bits of products down to 2^-3 of it, 2^-25 of it below, and have room for
 // 2^15 above. A row moves its unit only when a product leaves that room (or a weight fp32's): keeping
 // the products near 2^8 instead moved it ten times as often, and cost 10% of the wide kernel's time.
-constexpr float KV8_UNSET = 1000.f;           // the lift of a row that has no unit yet (its off is 0)
+constexpr float KV8_UNSET = 1000.f;           // the lift of a row that has no unit yet
 constexpr float KV8_PRODUCT_MAX = 32768.f;    // fp16 ends at 65504
 constexpr float KV8_WEIGHT_MAX = 0x1p100f;    // what a sum of four weights may be
 

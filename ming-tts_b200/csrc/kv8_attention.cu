@@ -232,7 +232,9 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
     // that its 24 do not hold (it does not round them), so a long chain of products drifts towards
     // zero: 256 key tiles in one chain were 4e-6 off. Every FOLD tiles the registers are added here.
     float4* const acc = reinterpret_cast<float4*>(smem + (warp * ROWS + g) * 64 + 16 * t);
-    float off = 0.f, at_off = 0.f, lift = KV8_UNSET, sum = 0.f, v_unit = 0.f;  // see kv8_unit; v_unit divides the value scales
+    // A row's first unit is above this one, so that its factor for what was there (nothing) is 0, whatever its scores.
+    float off = KV8_REF_NONE, at_off = KV8_REF_NONE, lift = KV8_UNSET, sum = 0.f;
+    float v_unit = 0.f;  // divides the value scales; the rest: see kv8_unit
     bool fresh = true;
     float o[8][4];
     auto clear = [&]() {

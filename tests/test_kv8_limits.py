@@ -1,0 +1,126 @@
+"""The 8-bit cache attention at the limits of its inputs, against the plain implementation in 64 bits of
+test_kv8.py and within the bound derived there.
+
+Caches are laid out by hand: `Keys` has the codes and scales of [requests, kv_heads, n, 64] for keys and values.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+import test_kv8 as base
+
+gpu = base.gpu
+KINDS = base.KINDS
+
+
+class Keys:
+    """Random codes, and the scales given (broadcast to [requests, heads, n])."""
+
+    def __init__(self, kind, requests, heads, n, k_scale, v_scale, seed=0):
+        import torch
+        g = torch.Generator().manual_seed(seed)
+        self.codes = []
+        for _ in range(2):
+            if kind == "int8":
+                c = torch.randint(-127, 128, (requests, heads, n, 64), generator=g, dtype=torch.int8)
+            else:
+                c = (torch.randn(requests, heads, n, 64, generator=g) * 110).clamp(-448, 448).to(torch.float8_e4m3fn)
+            self.codes.append(c)
+        self.scales = [torch.as_tensor(s, dtype=torch.float32).expand(requests, heads, n).clone() for s in (k_scale, v_scale)]
+
+    def values(self, which, r):
+        return self.codes[which][r].double() * self.scales[which][r].double()[..., None]
+
+    def cache(self, mt, start=0):
+        return mt.KV8Cache(*(t.cuda() for t in (*self.codes, *self.scales)), base=start)
+
+
+def attend(ctx, mt, keys, q, positions, window=0, prefix=None):
+    """One call (rows from q [requests, rows, hq, 64]): the output, the plain one and its bound, per request."""
+    import torch
+    n, rows, hq, _ = q.shape
+    plen = prefix.codes[0].shape[2] if prefix else 0
+    qd = q.reshape(n * rows, hq * 64).float().cuda()
+    out = torch.full_like(qd, 7.0)
+    pos = torch.tensor([plen + p for p in positions], dtype=torch.int32, device="cuda")
+    cache = keys.cache(mt, plen)
+    if prefix:
+        ctx.attention_prefix_kv8(qd, hq * 64, n, rows, hq, pos, None, prefix.cache(mt), plen, cache, out, hq * 64)
+    else:
+        ctx.attention_kv8(qd, hq * 64, n, rows, hq, pos, None, window, cache, out, hq * 64)
+    ctx.check()
+    out = out.cpu().double().view(n, rows, hq, 64)
+    results = []
+    for r, p in enumerate(positions):
+        at, mine = torch.arange(p + rows), torch.arange(p, p + rows)
+        sees = at <= mine[:, None]
+        if window:
+            sees &= at > mine[:, None] - window
+        k, v = (keys.values(w, r)[:, :p + rows] for w in range(2))
+        if prefix:
+            k, v = torch.cat([prefix.values(0, 0), k], 1), torch.cat([prefix.values(1, 0), v], 1)
+            sees = torch.cat([torch.ones(rows, plen, dtype=torch.bool), sees], 1)
+        want, bound = base.attend_reference(q[r].float().double(), k, v, sees)
+        results.append((out[r], want, bound))
+    return results
+
+
+def check(results):
+    import torch
+    for r, (got, want, bound) in enumerate(results):
+        assert torch.isfinite(got).all(), f"request {r}: {int((~torch.isfinite(got)).sum())} outputs are not finite"
+        err = (got - want).abs().amax(-1)
+        assert torch.all(err <= bound), (f"request {r}: worst error {float((err / bound).max()):.3g} of the bound at "
+                                         f"{np.unravel_index(int((err / bound).argmax()), err.shape)}")
+
+
+# ------------------------------------------------------------------------------------------------
+# Scores far below zero
+# ------------------------------------------------------------------------------------------------
+def against(kind, requests, heads, n, score, seed=0):
+    """Keys whose codes are the largest against a query of ones: scores of about `score` ([n]) each."""
+    import torch
+    limit = base.LIMIT[kind]
+    keys = Keys(kind, requests, heads, n, -torch.as_tensor(score, dtype=torch.float32) / (8 * limit), 2.0 / limit, seed)
+    keys.codes[0] = torch.full_like(keys.codes[0].float(), -limit).to(base.torch_kind(kind))
+    return keys
+
+
+def ones(requests, rows, hq, seed=0):
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    return 1.0 + 0.05 * torch.rand(requests, rows, hq, 64, generator=g)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("low", [-85.0, -95.0, -300.0, -4e4])
+def test_first_scores_far_below_zero(ctx, mt, kind, low):
+    """Every key that a warp meets first scores below the range of 2^-x: one key, one tile, windows, many rows."""
+    import torch
+    spread = low + 3 * torch.rand(4096, generator=torch.Generator().manual_seed(1)) - 3
+    check(attend(ctx, mt, against(kind, 1, 2, 1, spread[:1]), ones(1, 1, 14), [0]))
+    check(attend(ctx, mt, against(kind, 2, 2, 300, spread[:300]), ones(2, 1, 14), [11, 299]))
+    rising = torch.cat([spread[:70], spread[70:700] * 0.5])  # the largest scores come later
+    check(attend(ctx, mt, against(kind, 1, 2, 700, rising), ones(1, 1, 14), [699]))
+    check(attend(ctx, mt, against(kind, 1, 2, 700, rising), ones(1, 9, 6), [650]))
+    check(attend(ctx, mt, against(kind, 1, 2, 64, spread[:64]), ones(1, 20, 4), [40], window=1))
+    check(attend(ctx, mt, against(kind, 1, 2, 700, spread[:700]), ones(1, 40, 4), [600], window=200))
+    check(attend(ctx, mt, against(kind, 1, 1, 4000, spread[:4000]), ones(1, 1, 7), [3999]))
+    check(attend(ctx, mt, against(kind, 1, 2, 1024, spread[:1024]), ones(1, 500, 14), [500]))
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("plen", [40, 1500])
+def test_own_scores_far_below_zero_behind_a_prefix(ctx, mt, kind, plen):
+    """A request's own keys score far below the prefix's, and far above them."""
+    low, fair = against(kind, 3, 2, 20, [-300.0 - i for i in range(20)]), Keys(kind, 1, 2, plen, 0.5 / base.LIMIT[kind], 1.0, seed=2)
+    check(attend(ctx, mt, low, ones(3, 1, 14), [0, 5, 19], prefix=fair))
+    check(attend(ctx, mt, low, ones(3, 4, 14), [0, 5, 16], prefix=fair))
+    deep = against(kind, 1, 2, plen, [-300.0 - i % 7 for i in range(plen)], seed=3)
+    own = Keys(kind, 3, 2, 20, 0.5 / base.LIMIT[kind], 1.0, seed=4)
+    check(attend(ctx, mt, own, ones(3, 1, 14), [0, 5, 19], prefix=deep))
