@@ -197,18 +197,27 @@ __device__ __forceinline__ float power_to(float x, int target) {
     return __uint_as_float((uint32_t)(min(126, max(-126, target - e)) + 127) << 23);
 }
 
-// The unit of a row's weights. They are 2^(score - off), off = reference - lift: the reference is near a
-// score that was the row's largest, the lift brings the largest weight times value scale to 1 when it is
-// set: the two planes hold 22 bits of products down to 2^-3 of it, 2^-25 of it below, and have room for
-// 2^15 above. A row moves its unit only when a product leaves that room (or a weight fp32's): keeping
-// the products near 2^8 instead moved it ten times as often, and cost 10% of the wide kernel's time.
-constexpr float KV8_UNSET = 1000.f;           // the lift of a row that has no unit yet
+// The units of a row. Weights are 2^(score - off), off = reference - lift: the reference is near a score that was the
+// row's largest. Products of a weight and its value scale go into the planes times `extra`, a power of two: lift and
+// extra, 2^total together, bring the largest product to 1 when they are set. The two planes hold 22 bits of
+// products down to 2^-3 of it, 2^-25 of it below, and have room for 2^15 above. How much of the total is lift is a
+// kernel's own choice: a lift rounds the exponents of the largest weights to its own size, an extra that is a row's
+// own takes a multiplication. A row moves its units only when a product leaves their room (or a weight fp32's):
+// keeping the products near 2^8 instead moved it ten times as often, and cost 10% of the wide kernel's time.
+constexpr float KV8_UNSET = 1000.f;           // the total of a row that has no units yet
 constexpr float KV8_PRODUCT_MAX = 32768.f;    // fp16 ends at 65504
 constexpr float KV8_WEIGHT_MAX = 0x1p100f;    // what a sum of four weights may be
 
-// (off, lift) of a row after four of a lane's keys (scores z in powers of two, -infinity where not seen,
-// value scales v): all four lanes of the row get the same.
-__device__ __forceinline__ float2 kv8_unit(const float (&z)[4], const float (&v)[4], float off, float lift) {
+__device__ __forceinline__ float kv8_power(float n) { return __uint_as_float((uint32_t)((int)n + 127) << 23); }  // 2^n, |n| <= 126
+
+// Sets off and total of a row after four of a lane's keys (scores z in powers of two, -infinity where not seen,
+// value scales v), to the same in all four lanes of the row; lift(total) is the lift. Returns what the row's sum of
+// weights and its outputs so far have to be multiplied by: neither grows, but for sums of a row without units.
+struct Kv8Move {
+    float sums, outputs;
+};
+template <typename Lift>
+__device__ __forceinline__ Kv8Move kv8_move(const float (&z)[4], const float (&v)[4], float& off, float& total, Lift&& lift) {
     auto row_max = [](float x) {
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
         return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
@@ -219,15 +228,20 @@ __device__ __forceinline__ float2 kv8_unit(const float (&z)[4], const float (&v)
         for (int j = 0; j < 4; j++) x = fmaxf(x, ex2(z[j] - from) * v[j]);
         return row_max(x);
     };
+    const bool unset = total == KV8_UNSET;
     const float most = row_max(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
-    const bool unset = lift == KV8_UNSET;
-    const float now = product(off);
+    const float old_lift = unset ? 0.f : lift(total), old_extra = unset ? 0.f : total - old_lift;  // of 2
+    const float now = product(off) * kv8_power(old_extra);
     const bool move = most > -INFINITY && (unset || most - off > 90.f || now > KV8_PRODUCT_MAX);
-    const float ref = unset ? most : fmaxf(off + lift, most);
+    const float ref = unset ? most : fmaxf(off + old_lift, most);
     const float then = product(ref);
-    if (!move) return make_float2(off, lift);
-    lift = then > 0.f ? fminf(80.f, fmaxf(-100.f, (float)(127 - (int)(__float_as_uint(then) >> 23)))) : 0.f;
-    return make_float2(ref - lift, lift);
+    if (!move) return Kv8Move{1.f, 1.f};
+    float to = then > 0.f ? fminf(126.f, fmaxf(-126.f, (float)(127 - (int)(__float_as_uint(then) >> 23)))) : unset ? 0.f : total;
+    if (!unset) to = fminf(to, total + floorf(ref - (off + old_lift)));  // what is there may be the larger part
+    const float sums = ex2(off - (ref - lift(to)));
+    off = ref - lift(to);
+    total = to;
+    return Kv8Move{sums, unset ? 0.f : sums * kv8_power(to - lift(to)) * kv8_power(-old_extra)};
 }
 
 // A row's sum of weights, in units of 2^off, as (reference, sum) with sum in [1, 2): whatever its units,
@@ -239,13 +253,13 @@ __device__ __forceinline__ float2 kv8_total(float off, float sum) {
     return make_float2(off + (float)(127 - (int)(__float_as_uint(p) >> 23)), sum * p);
 }
 
-// Outputs (in units of `unit`, a power of two) divided by the sum of weights: unit and the sum's power of two
+// Outputs (times `extra`, a power of two) divided by the sum of weights: extra and the sum's power of two
 // in two halves, the rest of the sum, in [1, 2), with the first. No product leaves fp32 where the result does not.
 struct OverSum {
     float first, second;
-    __device__ __forceinline__ OverSum(float unit, float sum) {
+    __device__ __forceinline__ OverSum(float extra, float sum) {
         const float p = power_to(sum, 0);
-        const int e = (int)(__float_as_uint(unit) >> 23) + (int)(__float_as_uint(p) >> 23) - 2 * 127, half = e >> 1;
+        const int e = (int)(__float_as_uint(p) >> 23) - (int)(__float_as_uint(extra) >> 23), half = e >> 1;
         first = sum == 0.f ? 0.f : __uint_as_float((uint32_t)(half + 127) << 23) * rcp(sum * p);
         second = __uint_as_float((uint32_t)(e - half + 127) << 23);
     }

@@ -8,8 +8,8 @@
 // weight (times its value row's scale) are carried as two fp16 planes, x = hi + lo with
 // |x - hi - lo| <= 2^-22 |x|, so two 16-bit matrix products with fp32 sums give both contractions at
 // fp32 accuracy: q.k_j = scale_j (hi.c_j + lo.c_j), and the same for the values. Queries are scaled by
-// a power of two per row, weights by one per row that follows the largest weight times scale, so that
-// the planes use fp16's range whatever the units.
+// a power of two per row, products of weights and value scales by one per row that follows the largest, so
+// that the planes use fp16's range whatever the units (kv8_move).
 //
 // A warp owns a tile of 8 query rows (rows x grouped heads, flattened) and walks its keys 16 at a time, copied
 // ahead into a ring in shared memory. The rows' hi planes are rows 0-7 and their lo planes rows 8-15 of the
@@ -102,16 +102,8 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Power of two that brings the largest of a tile's value scales near 1 (all zero: 1).
-__device__ __forceinline__ float value_unit(const float (&vs)[4]) {
-    float x = fmaxf(fmaxf(fabsf(vs[0]), fabsf(vs[1])), fmaxf(fabsf(vs[2]), fabsf(vs[3])));
-    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-    return x > 0.f ? power_to(x, 0) : 1.f;
-}
-
 constexpr int ROWS = 8, WARPS = 8;  // rows of a warp, warps of a block (two blocks an SM)
-constexpr int SUM_BYTES = WARPS * ROWS * (64 + 4 + 1) * 4;  // sums, references and units, owners
+constexpr int SUM_BYTES = WARPS * ROWS * (64 + 4 + 1) * 4;  // sums, references and factors, owners
 constexpr int SMEM = SUM_BYTES + WARPS * RING * TILE_BYTES;
 constexpr int FOLD = 8;               // key tiles summed in the matrix unit's accumulators at a time
 
@@ -228,14 +220,14 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
     int hi, lo;  // keys of the lane's row, g
     const int row_of = any_row ? rows.pair(e0 + g, lo, hi) : -1;
 
-    // Sums of the rows in shared memory, in units of 2^at_off: the matrix unit drops the bits of a sum
+    // Sums of the rows in shared memory: the matrix unit drops the bits of a sum
     // that its 24 do not hold (it does not round them), so a long chain of products drifts towards
     // zero: 256 key tiles in one chain were 4e-6 off. Every FOLD tiles the registers are added here.
     float4* const acc = reinterpret_cast<float4*>(smem + (warp * ROWS + g) * 64 + 16 * t);
-    // A row's first unit is above this one, so that its factor for what was there (nothing) is 0, whatever its scores.
-    float off = KV8_REF_NONE, at_off = KV8_REF_NONE, lift = KV8_UNSET, sum = 0.f;
-    float v_unit = 0.f;  // divides the value scales; the rest: see kv8_unit
-    bool fresh = true;
+    // See kv8_move; no lift, and extra is the factor of the value scales. A row's first off is above this one, so that
+    // the factor for what was there (nothing) is 0.
+    float off = KV8_REF_NONE, extra = 0.f, sum = 0.f;  // extra 0: the row has no units yet
+    bool set = false;                                  // all rows of the warp have
     float o[8][4];
     auto clear = [&]() {
 #pragma unroll
@@ -245,15 +237,13 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
     };
     clear();
     auto fold = [&](bool first) {
-        const float f = first ? 0.f : ex2(at_off - off);
-        at_off = off;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             float4 y = first ? make_float4(0.f, 0.f, 0.f, 0.f) : acc[j];
             auto add = [&](float& x, int d) {
                 const float* const from = o[4 * (j & 1) + d] + (j >> 1);
                 const float v = from[0] + from[2];  // the planes
-                x = first ? v : fmaf(x, f, v);
+                x = first ? v : x + v;
             };
             add(y.x, 0); add(y.y, 1); add(y.z, 2); add(y.w, 3);
             acc[j] = y;
@@ -348,20 +338,19 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
                 s[2 * j + 1] = c[1] + c[3];
             }
             const bool whole = u0 >= r.in_lo && u0 + 15 <= r.in_hi;
-            if (v_unit == 0.f) v_unit = value_unit(vs);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                vs[k] *= v_unit;
+                vs[k] *= extra;  // may be infinite: the product with a weight is then too, or NaN
                 s[k] *= ks[k];
             }
             // Weights 2^(score - off), times the value rows' scales.
             float w[4], add;
-            auto weigh = [&](auto masked) {
+            auto weigh = [&](auto masked, float after) {
                 float p[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     p[k] = ex2(fmaf(s[k], q_scale, -off));
-                    w[k] = p[k] * vs[k];
+                    w[k] = p[k] * vs[k] * after;
                     if (masked) {
                         const bool on = u0 + 4 * t + k >= lo && u0 + 4 * t + k <= hi;
                         p[k] = on ? p[k] : 0.f;
@@ -369,32 +358,39 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
                     }
                 }
                 add = (p[0] + p[1]) + (p[2] + p[3]);
-                return fmaxf(fmaxf(fabsf(w[0]), fabsf(w[1])), fmaxf(fabsf(w[2]), fabsf(w[3]))) <= KV8_PRODUCT_MAX &&
-                       add <= KV8_WEIGHT_MAX;
+                return (fabsf(w[0]) + fabsf(w[1])) + (fabsf(w[2]) + fabsf(w[3])) <= KV8_PRODUCT_MAX && add <= KV8_WEIGHT_MAX;
             };
             bool fine = false;
-            if (!fresh) fine = whole ? weigh(std::false_type{}) : weigh(std::true_type{});
-            if (__any_sync(0xffffffffu, !fine)) {  // rare: a row's unit is set, or moves
+            if (set) fine = whole ? weigh(std::false_type{}, 1.f) : weigh(std::true_type{}, 1.f);
+            if (__any_sync(0xffffffffu, !fine)) {  // rare: a row's units are set, or move
                 float z[4], v[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
+                    vs[k] = reinterpret_cast<const volatile float*>(x + 2112 + 16 * t)[k];  // as they are (read again: registers)
                     const bool on = whole || (u0 + 4 * t + k >= lo && u0 + 4 * t + k <= hi);
                     z[k] = on ? s[k] * q_scale : -INFINITY;
                     v[k] = on ? fabsf(vs[k]) : 0.f;
                 }
-                const float2 to = kv8_unit(z, v, off, lift);
-                if (to.x != off) {
-                    const float f = ex2(off - to.x);
-                    sum *= f;
+                float total = extra == 0.f ? KV8_UNSET : (float)((int)(__float_as_uint(extra) >> 23) - 127);
+                const Kv8Move move = kv8_move(z, v, off, total, [](float) { return 0.f; });
+                extra = total == KV8_UNSET ? 0.f : kv8_power(total);
+                if (move.sums != 1.f || move.outputs != 1.f) {
+                    const float f = move.outputs;
+                    sum *= move.sums;
 #pragma unroll
                     for (int n = 0; n < 8; n++) {
                         o[n][0] *= f; o[n][1] *= f; o[n][2] *= f; o[n][3] *= f;
                     }
+                    if (folded) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const float4 y = acc[j];
+                            acc[j] = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+                        }
+                    }
                 }
-                off = to.x;
-                lift = to.y;
-                fresh = __any_sync(0xffffffffu, lift == KV8_UNSET);
-                weigh(std::true_type{});
+                set = __all_sync(0xffffffffu, extra != 0.f);
+                weigh(std::true_type{}, extra);
             }
             uint32_t pa[4];
             sum += add;
@@ -422,14 +418,14 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
 
     // Merge the key_warps warps of each row tile.
     fold(!folded);
-    float4* const ml = reinterpret_cast<float4*>(smem + WARPS * ROWS * 64);  // reference, sum; halves of the unit
+    float4* const ml = reinterpret_cast<float4*>(smem + WARPS * ROWS * 64);  // reference, sum; see OverSum
     int* const owner = reinterpret_cast<int*>(ml + WARPS * ROWS);
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     if (t == 0) {
-        const float2 total = kv8_total(off, sum);
-        const OverSum out(v_unit > 0.f ? 1.f / v_unit : 1.f, sum);
-        ml[warp * ROWS + g] = make_float4(total.x, total.y, out.first, out.second);
+        const float2 all = kv8_total(off, sum);
+        const OverSum out(extra == 0.f ? 1.f : extra, sum);
+        ml[warp * ROWS + g] = make_float4(all.x, all.y, out.first, out.second);
         if (phase == 0) owner[group * ROWS + g] = row_of;
     }
     __syncthreads();

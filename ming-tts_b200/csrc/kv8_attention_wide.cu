@@ -121,26 +121,36 @@ constexpr uint32_t IDESC_S = 1u << 4 | (WD_KEYS / 8) << 17 | (128 / 16) << 24;
 constexpr uint32_t IDESC_O = 1u << 4 | 1u << 16 | (64 / 8) << 17 | (128 / 16) << 24;  // B with N along its rows
 
 struct Shared {
-    alignas(16) float ks[WD_STAGES][WD_KEYS], vs[WD_STAGES][WD_KEYS];  // scales of the stages' keys (values': / unit)
+    alignas(16) float ks[WD_STAGES][WD_KEYS], vs[2][WD_STAGES][WD_KEYS];  // scales of the stages' keys; values': times 2^unit, and as they are
     float first[WD_CONVERT_WARPS];
-    float unit;                                                        // power of two near the first value scales
+    float unit;                                                        // brings the first value scales near 1
     uint64_t k_full[WD_STAGES], k_free[WD_STAGES], v_full[WD_STAGES], v_free[WD_STAGES];
     uint64_t q_ready[2], s_ready[2][2], p_ready[2][2], o_ready[2][2];     // by row tile (and key tile parity)
     uint32_t tmem;
     int abort;
 };
 
-// The state of a lane's two rows. Sums and outputs are in units of 2^off (see kv8_unit); a sum is the lane's
-// own part of the row.
+// Units of rows (see kv8_move). The factor 2^unit is in the value scales already, for all rows of a block; a row's lift
+// does the rest up to 2^16 either way, at the price of the exponents' rounding to 2^-20, and the fast path knows no
+// other. Rows whose first values are further from the first of the block go the slow way, with an extra of their own.
+constexpr float WD_LIFT = 16.f, WD_LARGEST = 0x1p127f;
+__device__ __forceinline__ float row_lift(float total, float unit) { return fminf(WD_LIFT, fmaxf(-WD_LIFT, total - unit)); }
+__device__ __forceinline__ float row_extra(float total, float unit) {
+    return total == KV8_UNSET ? 1.f : kv8_power(total - row_lift(total, unit));
+}
+__device__ __forceinline__ bool row_usual(float total, float unit) { return fabsf(total - unit) <= WD_LIFT; }
+
+// The state of a lane's two rows; off and total: see kv8_move. A sum is the lane's own part of the row.
 struct RowState {
-    float off[2], lift[2], rs[2];  // rs: scores in powers of two are TMEM value x key scale x rs
+    float off[2], total[2], rs[2];  // rs: scores in powers of two are TMEM value x key scale x rs
     int lo[2], hi[2];              // keys that the row sees
     float sum[2];
     float o[4][8];  // 16 columns each, as tmem_ld_tile
-    bool fresh;     // the unit of one of the warp's rows is not set yet
+    bool usual;     // all rows of the warp are: see row_usual
 
-    __device__ __forceinline__ void scale(int slot, float f) {
-        sum[slot] *= f;
+    __device__ __forceinline__ void scale(int slot, const Kv8Move& move) {
+        const float f = move.outputs;
+        sum[slot] *= move.sums;
 #pragma unroll
         for (int c = 0; c < 4; c++)
 #pragma unroll
@@ -156,6 +166,9 @@ struct RowState {
 struct TileKeys {
     const float *ks, *vs;
     int u;
+    const float* at_unit;
+    __device__ __forceinline__ float unit() const { return *reinterpret_cast<const volatile float*>(at_unit); }
+    __device__ __forceinline__ const float* raw() const { return vs + WD_STAGES * WD_KEYS; }  // the values' as they are
 };
 
 // The planes of `chunks` times 16 keys, scaled by the rows' factors.
@@ -180,32 +193,34 @@ __device__ __forceinline__ void row_rescale(uint32_t tm, int chunks, float f0, f
 }
 
 // Weights of 16 keys (s: scores, k and v: the keys' scales): 2^(score - off), their sums, and times the
-// value scales as planes. Returns the largest product.
-template <bool MASK>
+// value scales and the rows' extra (unless 2^unit does for all of them: see row_usual) as planes. Returns the largest product.
+template <bool SLOW>
 __device__ __forceinline__ float row_products(const TileKeys& t, const RowState& row, int c, const float (&s)[8], uint32_t (&planes)[8],
                                               float (&add)[2]) {
     const float2 k[2] = {*reinterpret_cast<const float2*>(t.ks + 16 * c), *reinterpret_cast<const float2*>(t.ks + 16 * c + 8)};
-    const float2 v[2] = {*reinterpret_cast<const float2*>(t.vs + 16 * c), *reinterpret_cast<const float2*>(t.vs + 16 * c + 8)};
+    const float* const vs = (SLOW && !row.usual ? t.raw() : t.vs) + 16 * c;
+    const float2 v[2] = {*reinterpret_cast<const float2*>(vs), *reinterpret_cast<const float2*>(vs + 8)};
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         float sum[2];
+        const float extra = SLOW && !row.usual ? row_extra(row.total[i], t.unit()) : 1.f;
 #pragma unroll
         for (int n = 0; n < 2; n++) {
             const int u = t.u + 16 * c + 8 * n;
-            const bool on0 = !MASK || (u >= row.lo[i] && u <= row.hi[i]), on1 = !MASK || (u + 1 >= row.lo[i] && u + 1 <= row.hi[i]);
+            const bool on0 = !SLOW || (u >= row.lo[i] && u <= row.hi[i]), on1 = !SLOW || (u + 1 >= row.lo[i] && u + 1 <= row.hi[i]);
             float p0 = ex2(fmaf(s[4 * n + 2 * i] * k[n].x, row.rs[i], -row.off[i]));
             float p1 = ex2(fmaf(s[4 * n + 2 * i + 1] * k[n].y, row.rs[i], -row.off[i]));
-            if (MASK) {
+            if (SLOW) {
                 p0 = on0 ? p0 : 0.f;
                 p1 = on1 ? p1 : 0.f;
             }
             sum[n] = p0 + p1;
             p0 *= v[n].x;
             p1 *= v[n].y;
-            if (MASK) {  // a scale of a key that this row does not see may be NaN
-                p0 = on0 ? p0 : 0.f;
-                p1 = on1 ? p1 : 0.f;
+            if (SLOW) {  // a scale of a key that this row does not see may be NaN
+                p0 = on0 ? p0 * extra : 0.f;
+                p1 = on1 ? p1 * extra : 0.f;
             }
             top = fmaxf(top, fmaxf(fabsf(p0), fabsf(p1)));
             split_half2(p0, p1, planes[2 * n + i], planes[4 + 2 * n + i]);
@@ -215,7 +230,7 @@ __device__ __forceinline__ float row_products(const TileKeys& t, const RowState&
     return top;
 }
 
-// A tile whose keys all rows see and whose products stay in range: nothing here changes a row's unit,
+// A tile whose keys all rows see and whose products stay in range: nothing here changes a row's units,
 // which is what keeps the loop at 9.4 instructions a weight (with that code in it, 12). Returns the first
 // 16 keys whose products do not stay in range, or 4.
 __device__ __forceinline__ int row_weights(uint32_t tm, const TileKeys& t, RowState& row) {
@@ -235,8 +250,8 @@ __device__ __forceinline__ int row_weights(uint32_t tm, const TileKeys& t, RowSt
     return c;
 }
 
-// The rest of a tile from `c` on, whatever its rows see: sets the units of rows that have none, and moves
-// them where products leave the range. `settle` adds the outputs that are still in TMEM, which are in the
+// The rest of a tile from `c` on, whatever its rows see and their units are: sets those of rows that have none, and
+// moves them where products leave the range. `settle` adds the outputs that are still in TMEM, which are in the
 // units before.
 template <typename F>
 __device__ __forceinline__ void row_weights_slowly(uint32_t tm, const TileKeys& t, RowState& row, int c, F&& settle) {
@@ -249,7 +264,8 @@ __device__ __forceinline__ void row_weights_slowly(uint32_t tm, const TileKeys& 
 #pragma unroll 1
         for (int tries = 0; tries < 2; tries++) {
             const float top = row_products<true>(t, row, c, s, planes, add);
-            if (!row.fresh && !__any_sync(0xffffffffu, !(top <= KV8_PRODUCT_MAX && add[0] <= KV8_WEIGHT_MAX && add[1] <= KV8_WEIGHT_MAX))) break;
+            if (!__any_sync(0xffffffffu, !(top <= KV8_PRODUCT_MAX && add[0] <= KV8_WEIGHT_MAX && add[1] <= KV8_WEIGHT_MAX &&
+                                           row.total[0] != KV8_UNSET && row.total[1] != KV8_UNSET))) break;
             settle(1);
             float f[2];
 #pragma unroll
@@ -260,16 +276,13 @@ __device__ __forceinline__ void row_weights_slowly(uint32_t tm, const TileKeys& 
                     const int key = 16 * c + 8 * (j >> 1) + (j & 1);
                     const bool on = t.u + key >= row.lo[i] && t.u + key <= row.hi[i];
                     z[j] = on ? s[4 * (j >> 1) + 2 * i + (j & 1)] * t.ks[key] * row.rs[i] : -INFINITY;
-                    v[j] = on ? fabsf(t.vs[key]) : 0.f;
+                    v[j] = on ? fabsf(t.raw()[key]) : 0.f;
                 }
-                const float2 to = kv8_unit(z, v, row.off[i], row.lift[i]);
-                const float off = to.x, lift = to.y;
-                f[i] = row.lift[i] == KV8_UNSET ? 1.f : ex2(row.off[i] - off);
-                if (off != row.off[i]) row.scale(i, f[i]);
-                row.off[i] = off;
-                row.lift[i] = lift;
+                const Kv8Move move = kv8_move(z, v, row.off[i], row.total[i], [&](float total) { return row_lift(total, t.unit()); });
+                if (move.sums != 1.f || move.outputs != 1.f) row.scale(i, move);
+                f[i] = move.outputs;
             }
-            row.fresh = __any_sync(0xffffffffu, row.lift[0] == KV8_UNSET || row.lift[1] == KV8_UNSET);
+            row.usual = __all_sync(0xffffffffu, row_usual(row.total[0], t.unit()) && row_usual(row.total[1], t.unit()));
             row_rescale(tm, c, f[0], f[1]);
         }
         row.sum[0] += add[0];
@@ -398,11 +411,11 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
                 for (int i = 0; i < 2; i++) {
                     // up is a power of two within 2^+-126: so is its reciprocal
                     row.rs[i] = 0.125f * 1.4426950408889634f * __uint_as_float(0x7F000000u - __float_as_uint(up[i]));
-                    row.off[i] = 0.f;
-                    row.lift[i] = KV8_UNSET;
+                    row.off[i] = KV8_REF_NONE;
+                    row.total[i] = KV8_UNSET;
                     row.sum[i] = 0.f;
                 }
-                row.fresh = true;
+                row.usual = false;
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -438,11 +451,11 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
                      mbar_wait(&sh.s_ready[tile][n & 1], (n >> 1) & 1, status, 20, abort);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 tmem_acquire();
-                const TileKeys keys{sh.ks[st] + col, sh.vs[st] + col, u0 + col};
+                const TileKeys keys{sh.ks[st] + col, sh.vs[0][st] + col, u0 + col, &sh.unit};
                 const uint32_t tp = tm + (n & 1) * WD_KEYS;
                 settle(2);
                 int c = 0;
-                if (!row.fresh && u0 >= r.in_lo && u0 + WD_KEYS - 1 <= r.in_hi) c = row_weights(tp, keys, row);
+                if (row.usual && u0 >= r.in_lo && u0 + WD_KEYS - 1 <= r.in_hi) c = row_weights(tp, keys, row);
                 if (c < 4) row_weights_slowly(tp, keys, row, c, settle);
                 tmem_publish();
                 __syncwarp();
@@ -456,7 +469,7 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
                     s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
                     s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
                     if (target[i] < 0) continue;
-                    const OverSum out(sh.unit, s0);
+                    const OverSum out(row_extra(row.total[i], sh.unit), s0);
                     float* dst;
                     bool vec = true;
                     if (!a.parted) {
@@ -529,15 +542,16 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
         load(u_first);
-        // The value scales' unit, from the first tile: a power of two, divided out of all of them.
+        // The value scales' unit, from the first tile (all zero: none).
         float most = 0.f;
 #pragma unroll
         for (int j = 0; j < TURNS; j++) most = fmaxf(most, fabsf(vs[j]));
         most = warp_max(most);
         if (lane == 0) sh.first[w] = most;
         asm volatile("bar.sync 1, 96;" ::: "memory");
-        const float per_unit = power_to(fmaxf(sh.first[0], fmaxf(sh.first[1], sh.first[2])), 0);
-        if (w == 0 && lane == 0) sh.unit = 1.f / per_unit;
+        most = fmaxf(sh.first[0], fmaxf(sh.first[1], sh.first[2]));
+        const float per_unit = most > 0.f ? power_to(most, 0) : 1.f;
+        if (w == 0 && lane == 0) sh.unit = (float)((int)(__float_as_uint(per_unit) >> 23) - 127);
         for (int n = 0; n < tiles; n++) {
             if (n > 0) load(u_first + n * WD_KEYS);
             const int st = n & (WD_STAGES - 1);
@@ -554,7 +568,11 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
                     const int key = key_of(j);
                     if (key >= WD_KEYS) break;
                     sh.ks[st][key] = ks[j];
-                    sh.vs[st][key] = vs[j] * per_unit;
+                    // Not infinite, so that a weight of 0 does not make it NaN. A usual row's largest weight is 2^-16 or
+                    // more, and one of 2^-112 times this is a product that goes the slow way.
+                    const float near1 = vs[j] * per_unit;
+                    sh.vs[0][st][key] = near1 > WD_LARGEST ? WD_LARGEST : near1;
+                    sh.vs[1][st][key] = vs[j];
                 }
             }
             __syncwarp();

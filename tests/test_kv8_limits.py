@@ -124,3 +124,62 @@ def test_own_scores_far_below_zero_behind_a_prefix(ctx, mt, kind, plen):
     deep = against(kind, 1, 2, plen, [-300.0 - i % 7 for i in range(plen)], seed=3)
     own = Keys(kind, 3, 2, 20, 0.5 / base.LIMIT[kind], 1.0, seed=4)
     check(attend(ctx, mt, own, ones(3, 1, 14), [0, 5, 19], prefix=deep))
+
+
+# ------------------------------------------------------------------------------------------------
+# Value scales of different sizes
+# ------------------------------------------------------------------------------------------------
+def value_scale_calls(ctx, mt, kind, scales, q_size=0.01, key_scale=None):
+    """Calls of every layout over keys whose value scales are `scales(n)`. Queries are small, so that the
+    scores' part of the bound is, and weights nearly equal."""
+    import torch
+    ks = 2.0 / base.LIMIT[kind] if key_scale is None else key_scale
+
+    def q(*shape, seed=0):
+        return q_size * torch.randn(*shape, 64, generator=torch.Generator().manual_seed(seed))
+
+    def keys(requests, heads, n, seed=0):
+        return Keys(kind, requests, heads, n, ks, scales(n), seed)
+
+    check(attend(ctx, mt, keys(2, 2, 300), q(2, 1, 14), [40, 299]))
+    check(attend(ctx, mt, keys(1, 2, 300), q(1, 9, 6), [291]))
+    check(attend(ctx, mt, keys(1, 2, 4000), q(1, 1, 14), [3999]))
+    check(attend(ctx, mt, keys(2, 2, 4000), q(2, 1, 14), [3999, 1000]))
+    check(attend(ctx, mt, keys(1, 2, 1024), q(1, 500, 14), [524]))
+    check(attend(ctx, mt, keys(1, 2, 700), q(1, 700, 14), [0]))
+    fair = Keys(kind, 64, 2, 20, ks, float(scales(4000)[-1]), seed=5)
+    check(attend(ctx, mt, fair, q(64, 1, 14), [i % 20 for i in range(64)], prefix=keys(1, 2, 4000)))
+    check(attend(ctx, mt, Keys(kind, 3, 2, 20, ks, float(scales(174)[-1]), seed=5), q(3, 1, 14), [0, 7, 19], prefix=keys(1, 2, 174)))
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("zeros", [1, 16, 64, 200])
+@pytest.mark.parametrize("size", [4.0, 1e-2])
+def test_zero_values_first(ctx, mt, kind, zeros, size):
+    """The first value rows are zero (scale 0, as they are written), the rest of one size: errors are relative to it."""
+    import torch
+
+    def scales(n):
+        s = size * (0.5 + torch.rand(n, generator=torch.Generator().manual_seed(7)))
+        s[:zeros] = 0.0
+        return s
+
+    value_scale_calls(ctx, mt, kind, scales)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("first,small,large", [(16, -126, 0), (64, -126, 0), (64, -126, 110), (130, -100, 20), (300, -20, 100),
+                                               (20, 105, -100), (300, 30, -126)])
+def test_value_scales_of_any_ratio(ctx, mt, kind, first, small, large):
+    """The first value scales 2^small, the others 2^large: each row is exact to the largest value that it sees itself."""
+    import torch
+
+    def scales(n):
+        s = 1 + torch.rand(n, generator=torch.Generator().manual_seed(8), dtype=torch.float64)
+        s[:first] *= 2.0 ** small
+        s[first:] *= 2.0 ** large
+        return s.float()
+
+    value_scale_calls(ctx, mt, kind, scales)
