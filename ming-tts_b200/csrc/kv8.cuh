@@ -204,7 +204,7 @@ __device__ __forceinline__ float power_to(float x, int target) {
 // kernel's own choice: a lift rounds the exponents of the largest weights to its own size, an extra that is a row's
 // own takes a multiplication. A row moves its units only when a product leaves their room (or a weight fp32's):
 // keeping the products near 2^8 instead moved it ten times as often, and cost 10% of the wide kernel's time.
-constexpr float KV8_UNSET = 1000.f;           // the total of a row that has no units yet
+constexpr float KV8_UNSET = 1000.f;           // the total of a row that has seen no value but zeros
 constexpr float KV8_PRODUCT_MAX = 32768.f;    // fp16 ends at 65504
 constexpr float KV8_WEIGHT_MAX = 0x1p100f;    // what a sum of four weights may be
 
@@ -233,15 +233,17 @@ __device__ __forceinline__ Kv8Move kv8_move(const float (&z)[4], const float (&v
     const float old_lift = unset ? 0.f : lift(total), old_extra = unset ? 0.f : total - old_lift;  // of 2
     const float now = product(off) * kv8_power(old_extra);
     const bool move = most > -INFINITY && (unset || most - off > 90.f || now > KV8_PRODUCT_MAX);
-    const float ref = unset ? most : fmaxf(off + old_lift, most);
+    const float ref = fmaxf(off + old_lift, most);
     const float then = product(ref);
     if (!move) return Kv8Move{1.f, 1.f};
-    float to = then > 0.f ? fminf(126.f, fmaxf(-126.f, (float)(127 - (int)(__float_as_uint(then) >> 23)))) : unset ? 0.f : total;
+    // No product but zeros yet: the weights have their unit, the products wait for theirs.
+    const bool none = unset && then == 0.f;
+    float to = then > 0.f ? fminf(126.f, fmaxf(-126.f, (float)(127 - (int)(__float_as_uint(then) >> 23)))) : total;
     if (!unset) to = fminf(to, total + floorf(ref - (off + old_lift)));  // what is there may be the larger part
-    const float sums = ex2(off - (ref - lift(to)));
-    off = ref - lift(to);
+    const float new_lift = none ? 0.f : lift(to), sums = ex2(off - (ref - new_lift));
+    off = ref - new_lift;
     total = to;
-    return Kv8Move{sums, unset ? 0.f : sums * kv8_power(to - lift(to)) * kv8_power(-old_extra)};
+    return Kv8Move{sums, unset ? 0.f : sums * kv8_power(to - new_lift) * kv8_power(-old_extra)};
 }
 
 // A row's sum of weights, in units of 2^off, as (reference, sum) with sum in [1, 2): whatever its units,

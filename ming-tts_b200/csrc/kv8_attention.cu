@@ -226,7 +226,7 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
     float4* const acc = reinterpret_cast<float4*>(smem + (warp * ROWS + g) * 64 + 16 * t);
     // See kv8_move; no lift, and extra is the factor of the value scales. A row's first off is above this one, so that
     // the factor for what was there (nothing) is 0.
-    float off = KV8_REF_NONE, extra = 0.f, sum = 0.f;  // extra 0: the row has no units yet
+    float off = KV8_REF_NONE, extra = 0.f, sum = 0.f;  // extra 0: KV8_UNSET
     bool set = false;                                  // all rows of the warp have
     float o[8][4];
     auto clear = [&]() {

@@ -155,7 +155,7 @@ def value_scale_calls(ctx, mt, kind, scales, q_size=0.01, key_scale=None):
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("zeros", [1, 16, 64, 200])
-@pytest.mark.parametrize("size", [4.0, 1e-2])
+@pytest.mark.parametrize("size", [4.0, 1e-2, 1e-4, 1e-6, 1e-30])
 def test_zero_values_first(ctx, mt, kind, zeros, size):
     """The first value rows are zero (scale 0, as they are written), the rest of one size: errors are relative to it."""
     import torch
