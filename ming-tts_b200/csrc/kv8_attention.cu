@@ -318,10 +318,12 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
             __syncwarp();
             const uint8_t* const x = ring + stage * TILE_BYTES;
             const float4 ks4 = *reinterpret_cast<const float4*>(x + 2048 + 16 * t), vs4 = *reinterpret_cast<const float4*>(x + 2112 + 16 * t);
-            const float ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w};
+            // The scales of key and query first: their product is of a score's size, while a sum of codes
+            // times a large key scale may be infinite.
+            const float ks[4] = {ks4.x * q_scale, ks4.y * q_scale, ks4.z * q_scale, ks4.w * q_scale};
             float vs[4] = {vs4.x, vs4.y, vs4.z, vs4.w};
 
-            // Scores (before scaling): 4 keys of the lane's row.
+            // Scores before scaling: 4 keys of the lane's row.
             float s[4];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
@@ -339,17 +341,14 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
             }
             const bool whole = u0 >= r.in_lo && u0 + 15 <= r.in_hi;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                vs[k] *= extra;  // may be infinite: the product with a weight is then too, or NaN
-                s[k] *= ks[k];
-            }
+            for (int k = 0; k < 4; k++) vs[k] *= extra;  // may be infinite: the product with a weight is then too, or NaN
             // Weights 2^(score - off), times the value rows' scales.
             float w[4], add;
             auto weigh = [&](auto masked, float after) {
                 float p[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    p[k] = ex2(fmaf(s[k], q_scale, -off));
+                    p[k] = ex2(fmaf(s[k], ks[k], -off));
                     w[k] = p[k] * vs[k] * after;
                     if (masked) {
                         const bool on = u0 + 4 * t + k >= lo && u0 + 4 * t + k <= hi;
@@ -368,7 +367,7 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
                 for (int k = 0; k < 4; k++) {
                     vs[k] = reinterpret_cast<const volatile float*>(x + 2112 + 16 * t)[k];  // as they are (read again: registers)
                     const bool on = whole || (u0 + 4 * t + k >= lo && u0 + 4 * t + k <= hi);
-                    z[k] = on ? s[k] * q_scale : -INFINITY;
+                    z[k] = on ? s[k] * ks[k] : -INFINITY;
                     v[k] = on ? fabsf(vs[k]) : 0.f;
                 }
                 float total = extra == 0.f ? KV8_UNSET : (float)((int)(__float_as_uint(extra) >> 23) - 127);

@@ -209,8 +209,9 @@ __device__ __forceinline__ float row_products(const TileKeys& t, const RowState&
         for (int n = 0; n < 2; n++) {
             const int u = t.u + 16 * c + 8 * n;
             const bool on0 = !SLOW || (u >= row.lo[i] && u <= row.hi[i]), on1 = !SLOW || (u + 1 >= row.lo[i] && u + 1 <= row.hi[i]);
-            float p0 = ex2(fmaf(s[4 * n + 2 * i] * k[n].x, row.rs[i], -row.off[i]));
-            float p1 = ex2(fmaf(s[4 * n + 2 * i + 1] * k[n].y, row.rs[i], -row.off[i]));
+            // key scale and rs first: see kv8_attention.cu
+            float p0 = ex2(fmaf(s[4 * n + 2 * i], k[n].x * row.rs[i], -row.off[i]));
+            float p1 = ex2(fmaf(s[4 * n + 2 * i + 1], k[n].y * row.rs[i], -row.off[i]));
             if (SLOW) {
                 p0 = on0 ? p0 : 0.f;
                 p1 = on1 ? p1 : 0.f;
@@ -275,7 +276,7 @@ __device__ __forceinline__ void row_weights_slowly(uint32_t tm, const TileKeys& 
                 for (int j = 0; j < 4; j++) {
                     const int key = 16 * c + 8 * (j >> 1) + (j & 1);
                     const bool on = t.u + key >= row.lo[i] && t.u + key <= row.hi[i];
-                    z[j] = on ? s[4 * (j >> 1) + 2 * i + (j & 1)] * t.ks[key] * row.rs[i] : -INFINITY;
+                    z[j] = on ? s[4 * (j >> 1) + 2 * i + (j & 1)] * (t.ks[key] * row.rs[i]) : -INFINITY;
                     v[j] = on ? fabsf(t.raw()[key]) : 0.f;
                 }
                 const Kv8Move move = kv8_move(z, v, row.off[i], row.total[i], [&](float total) { return row_lift(total, t.unit()); });

@@ -183,3 +183,15 @@ def test_value_scales_of_any_ratio(ctx, mt, kind, first, small, large):
         return s.float()
 
     value_scale_calls(ctx, mt, kind, scales)
+
+
+# ------------------------------------------------------------------------------------------------
+# Key scales near the largest and the smallest number
+# ------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("power", [90, 112, 116, -100, -126])
+def test_key_scales_of_any_size(ctx, mt, kind, power):
+    """Scores of ordinary size from keys near either end of fp32 and queries near the other."""
+    import torch
+    value_scale_calls(ctx, mt, kind, lambda n: torch.full((n,), 0.01), q_size=2.0 ** (-power - 4), key_scale=2.0 ** power)
