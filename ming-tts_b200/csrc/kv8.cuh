@@ -205,14 +205,20 @@ __device__ __forceinline__ float power_to(float x, int target) {
 // own takes a multiplication. A row moves its units only when a product leaves their room (or a weight fp32's):
 // keeping the products near 2^8 instead moved it ten times as often, and cost 10% of the wide kernel's time.
 constexpr float KV8_UNSET = 1000.f;           // the total of a row that has seen no value but zeros
+constexpr float KV8_FAR = 400.f;              // in a total (between 200 and 600 then): the row has no lift, see kv8_move
 constexpr float KV8_PRODUCT_MAX = 32768.f;    // fp16 ends at 65504
 constexpr float KV8_WEIGHT_MAX = 0x1p100f;    // what a sum of four weights may be
 
 __device__ __forceinline__ float kv8_power(float n) { return __uint_as_float((uint32_t)((int)n + 127) << 23); }  // 2^n, |n| <= 126
 
+// A score in powers of two, rounded. off is taken from scores so rounded, and so are the weights of the keys that it
+// is taken from: at 10^9 one multiply-add gives another score by up to 2^6, which is 2^64 in a weight.
+__device__ __forceinline__ float kv8_score(float sum, float scale) { return __fmul_rn(sum, scale); }
+
 // Sets off and total of a row after four of a lane's keys (scores z in powers of two, -infinity where not seen,
 // value scales v), to the same in all four lanes of the row; lift(total) is the lift. Returns what the row's sum of
 // weights and its outputs so far have to be multiplied by: neither grows, but for sums of a row without units.
+// Where fp32 has no fraction at the reference (from 2^24 on) a lift would be rounded: extra takes all of the total.
 struct Kv8Move {
     float sums, outputs;
 };
@@ -230,7 +236,9 @@ __device__ __forceinline__ Kv8Move kv8_move(const float (&z)[4], const float (&v
     };
     const bool unset = total == KV8_UNSET;
     const float most = row_max(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
-    const float old_lift = unset ? 0.f : lift(total), old_extra = unset ? 0.f : total - old_lift;  // of 2
+    const bool was_far = !unset && total > 0.5f * KV8_FAR;
+    const float old = was_far ? total - KV8_FAR : total;
+    const float old_lift = unset || was_far ? 0.f : lift(old), old_extra = unset ? 0.f : old - old_lift;  // of 2
     const float now = product(off) * kv8_power(old_extra);
     const bool move = most > -INFINITY && (unset || most - off > 90.f || now > KV8_PRODUCT_MAX);
     const float ref = fmaxf(off + old_lift, most);
@@ -238,11 +246,14 @@ __device__ __forceinline__ Kv8Move kv8_move(const float (&z)[4], const float (&v
     if (!move) return Kv8Move{1.f, 1.f};
     // No product but zeros yet: the weights have their unit, the products wait for theirs.
     const bool none = unset && then == 0.f;
-    float to = then > 0.f ? fminf(126.f, fmaxf(-126.f, (float)(127 - (int)(__float_as_uint(then) >> 23)))) : total;
-    if (!unset) to = fminf(to, total + floorf(ref - (off + old_lift)));  // what is there may be the larger part
-    const float new_lift = none ? 0.f : lift(to), sums = ex2(off - (ref - new_lift));
+    float to = then > 0.f ? fminf(126.f, fmaxf(-126.f, (float)(127 - (int)(__float_as_uint(then) >> 23)))) : old;
+    if (!unset) to = fminf(to, old + floorf(ref - (off + old_lift)));  // what is there may be the larger part
+    float new_lift = none ? 0.f : lift(to);
+    const bool far = fabsf(ref) >= 0x1p24f && new_lift != 0.f;
+    if (far) new_lift = 0.f;
+    const float sums = ex2(off - (ref - new_lift));
     off = ref - new_lift;
-    total = to;
+    total = far ? to + KV8_FAR : to;
     return Kv8Move{sums, unset ? 0.f : sums * kv8_power(to - new_lift) * kv8_power(-old_extra)};
 }
 

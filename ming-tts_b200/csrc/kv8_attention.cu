@@ -344,11 +344,11 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
             for (int k = 0; k < 4; k++) vs[k] *= extra;  // may be infinite: the product with a weight is then too, or NaN
             // Weights 2^(score - off), times the value rows' scales.
             float w[4], add;
-            auto weigh = [&](auto masked, float after) {
+            auto weigh = [&](auto masked, auto slow, float after) {
                 float p[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    p[k] = ex2(fmaf(s[k], ks[k], -off));
+                    p[k] = ex2(slow ? kv8_score(s[k], ks[k]) - off : fmaf(s[k], ks[k], -off));
                     w[k] = p[k] * vs[k] * after;
                     if (masked) {
                         const bool on = u0 + 4 * t + k >= lo && u0 + 4 * t + k <= hi;
@@ -360,14 +360,14 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
                 return (fabsf(w[0]) + fabsf(w[1])) + (fabsf(w[2]) + fabsf(w[3])) <= KV8_PRODUCT_MAX && add <= KV8_WEIGHT_MAX;
             };
             bool fine = false;
-            if (set) fine = whole ? weigh(std::false_type{}, 1.f) : weigh(std::true_type{}, 1.f);
+            if (set) fine = whole ? weigh(std::false_type{}, std::false_type{}, 1.f) : weigh(std::true_type{}, std::false_type{}, 1.f);
             if (__any_sync(0xffffffffu, !fine)) {  // rare: a row's units are set, or move
                 float z[4], v[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     vs[k] = reinterpret_cast<const volatile float*>(x + 2112 + 16 * t)[k];  // as they are (read again: registers)
                     const bool on = whole || (u0 + 4 * t + k >= lo && u0 + 4 * t + k <= hi);
-                    z[k] = on ? s[k] * ks[k] : -INFINITY;
+                    z[k] = on ? kv8_score(s[k], ks[k]) : -INFINITY;
                     v[k] = on ? fabsf(vs[k]) : 0.f;
                 }
                 float total = extra == 0.f ? KV8_UNSET : (float)((int)(__float_as_uint(extra) >> 23) - 127);
@@ -389,7 +389,7 @@ __device__ __forceinline__ void pass_block(const PassArgs& a, int block) {
                     }
                 }
                 set = __all_sync(0xffffffffu, extra != 0.f);
-                weigh(std::true_type{}, extra);
+                weigh(std::true_type{}, std::true_type{}, extra);
             }
             uint32_t pa[4];
             sum += add;

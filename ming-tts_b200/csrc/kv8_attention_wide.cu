@@ -136,7 +136,8 @@ struct Shared {
 constexpr float WD_LIFT = 16.f, WD_LARGEST = 0x1p127f;
 __device__ __forceinline__ float row_lift(float total, float unit) { return fminf(WD_LIFT, fmaxf(-WD_LIFT, total - unit)); }
 __device__ __forceinline__ float row_extra(float total, float unit) {
-    return total == KV8_UNSET ? 1.f : kv8_power(total - row_lift(total, unit));
+    if (total == KV8_UNSET) return 1.f;
+    return kv8_power(total > 0.5f * KV8_FAR ? total - KV8_FAR : total - row_lift(total, unit));
 }
 __device__ __forceinline__ bool row_usual(float total, float unit) { return fabsf(total - unit) <= WD_LIFT; }
 
@@ -210,8 +211,9 @@ __device__ __forceinline__ float row_products(const TileKeys& t, const RowState&
             const int u = t.u + 16 * c + 8 * n;
             const bool on0 = !SLOW || (u >= row.lo[i] && u <= row.hi[i]), on1 = !SLOW || (u + 1 >= row.lo[i] && u + 1 <= row.hi[i]);
             // key scale and rs first: see kv8_attention.cu
-            float p0 = ex2(fmaf(s[4 * n + 2 * i], k[n].x * row.rs[i], -row.off[i]));
-            float p1 = ex2(fmaf(s[4 * n + 2 * i + 1], k[n].y * row.rs[i], -row.off[i]));
+            const float k0 = k[n].x * row.rs[i], k1 = k[n].y * row.rs[i], s0 = s[4 * n + 2 * i], s1 = s[4 * n + 2 * i + 1];
+            float p0 = ex2(SLOW ? kv8_score(s0, k0) - row.off[i] : fmaf(s0, k0, -row.off[i]));
+            float p1 = ex2(SLOW ? kv8_score(s1, k1) - row.off[i] : fmaf(s1, k1, -row.off[i]));
             if (SLOW) {
                 p0 = on0 ? p0 : 0.f;
                 p1 = on1 ? p1 : 0.f;
@@ -276,7 +278,7 @@ __device__ __forceinline__ void row_weights_slowly(uint32_t tm, const TileKeys& 
                 for (int j = 0; j < 4; j++) {
                     const int key = 16 * c + 8 * (j >> 1) + (j & 1);
                     const bool on = t.u + key >= row.lo[i] && t.u + key <= row.hi[i];
-                    z[j] = on ? s[4 * (j >> 1) + 2 * i + (j & 1)] * (t.ks[key] * row.rs[i]) : -INFINITY;
+                    z[j] = on ? kv8_score(s[4 * (j >> 1) + 2 * i + (j & 1)], t.ks[key] * row.rs[i]) : -INFINITY;
                     v[j] = on ? fabsf(t.raw()[key]) : 0.f;
                 }
                 const Kv8Move move = kv8_move(z, v, row.off[i], row.total[i], [&](float total) { return row_lift(total, t.unit()); });

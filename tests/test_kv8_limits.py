@@ -195,3 +195,51 @@ def test_key_scales_of_any_size(ctx, mt, kind, power):
     """Scores of ordinary size from keys near either end of fp32 and queries near the other."""
     import torch
     value_scale_calls(ctx, mt, kind, lambda n: torch.full((n,), 0.01), q_size=2.0 ** (-power - 4), key_scale=2.0 ** power)
+
+
+# ------------------------------------------------------------------------------------------------
+# Scores of any size
+# ------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [1e5, 3e7, 1e9, 1e12, 1e20, 1e30])
+@pytest.mark.parametrize("v_power", [-6, -40, 40])
+def test_scores_of_any_size(ctx, mt, kind, size, v_power):
+    """Scores so large that fp32 holds no fraction of them: where one key is ahead by more than twice what the
+    scores may be off, all others weigh nothing (e^-30 and less), and the output is its value."""
+    import torch
+    root = math.sqrt(size / 8)
+    spread = torch.exp2(torch.randint(0, 12, (4000,), generator=torch.Generator().manual_seed(3)).float())
+    seen = 0
+
+    def run(requests, heads, n, rows, hq, positions, plen=0):
+        nonlocal seen
+        g = torch.Generator().manual_seed(n)
+        q = root * torch.randn(requests, rows, hq, 64, generator=g)
+        keys = Keys(kind, requests, heads, n, 2 * root / base.LIMIT[kind], 2.0 ** v_power * spread[:n], seed=n)
+        prefix = Keys(kind, 1, heads, plen, 2 * root / base.LIMIT[kind], 2.0 ** v_power * spread[:plen], seed=n + 1) if plen else None
+        results = attend(ctx, mt, keys, q, positions, prefix=prefix)
+        check(results)
+        for r, (got, want, _) in enumerate(results):
+            p = positions[r]
+            k, v = (torch.cat([prefix.values(w, 0), keys.values(w, r)], 1) if plen else keys.values(w, r) for w in range(2))
+            for h in range(hq):
+                kv = h // (hq // heads)
+                s = q[r, :, h].double() @ k[kv].T / 8
+                s = s.masked_fill(torch.arange(k.shape[1]) - plen > torch.arange(p, p + rows)[:, None], -math.inf)
+                a = (q[r, :, h].double().abs() @ k[kv].abs().T / 8).amax(-1)
+                top = s.topk(min(2, s.shape[1]), -1)
+                ahead = top.values[:, 0] - top.values[:, -1] > 4 * 136 * 2.0 ** -24 * a + 30 if s.shape[1] > 1 else torch.ones(rows, dtype=torch.bool)
+                value = v[kv][top.indices[:, 0]]
+                err = (got[:, h] - value).abs().amax(-1)
+                assert torch.all((err <= 2.0 ** -18 * value.abs().amax(-1)) | ~ahead), f"request {r} head {h}"
+                seen += int(ahead.sum())
+
+    run(2, 2, 300, 1, 14, [40, 299])
+    run(1, 2, 60, 20, 6, [30])
+    run(1, 2, 4000, 1, 14, [3999])
+    run(1, 2, 1024, 500, 14, [524])
+    run(1, 1, 1, 1, 3, [0])
+    run(40, 2, 20, 1, 14, [i % 20 for i in range(40)], plen=3000)
+    run(3, 2, 20, 1, 14, [0, 7, 19], plen=174)
+    assert seen > 0
