@@ -356,7 +356,7 @@ mt_status mt_kv8_read(mt_ctx* ctx, void* stream, const mt_kv8_cache* cache, int 
 mt_status mt_attention_kv8(mt_ctx* ctx, void* stream, const float* q, int ldq, int requests, int rows, int hq,
                            const int32_t* positions, const int32_t* counts, int window, const mt_kv8_cache* cache,
                            float* out, int ldo, void* workspace, size_t workspace_bytes);
-/* Bytes of workspace that mt_attention_kv8 needs for these arguments on ctx (0: none). */
+/* Bytes of workspace that mt_attention_kv8 needs for these arguments on ctx (0: none, or arguments that it refuses). */
 size_t mt_attention_kv8_workspace(const mt_ctx* ctx, const mt_kv8_cache* cache, int requests, int rows, int hq, int window);
 
 /* Attention of a batch whose requests share a prefix (a voice prompt, a system prompt): every row sees

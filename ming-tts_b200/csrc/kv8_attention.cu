@@ -700,9 +700,16 @@ struct Plan {
     size_t o_bytes, ml_bytes, bytes;
 };
 
+// The sizes that make_plan is for, and that attention() accepts.
+bool plannable(int prefix_len, const mt_kv8_cache* cache, int requests, int rows, int hq, int window) {
+    return cache && prefix_len >= 0 && prefix_len <= 1 << 30 && requests > 0 && rows > 0 && hq > 0 && hq <= 1024 && cache->kv_heads > 0 &&
+           hq % cache->kv_heads == 0 && cache->capacity > 0 && cache->capacity <= 1 << 30 && window >= 0 && rows <= cache->capacity &&
+           (window == 0 || (long long)window + rows - 1 <= cache->capacity) && (long long)requests * rows <= 0x7FFFFF00ll / hq;
+}
+
 Plan make_plan(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int requests, int rows, int hq, int window) {
     Plan p{};
-    const int hkv = cache->kv_heads > 0 ? cache->kv_heads : 1;
+    const int hkv = cache->kv_heads;
     const long long group = hq / hkv;
     const long long seen = window > 0 ? (long long)window + rows - 1 : cache->capacity;
     const long long size = (long long)rows * hq;
@@ -710,7 +717,7 @@ Plan make_plan(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int
     p.own = plan_pass(ctx->sm_count, (long long)requests * hkv, requests, rows * group, keys, window > 0 ? 0 : rows - 1);
     if (prefix_len > 0) {
         p.prefix = plan_pass(ctx->sm_count, hkv, 1, (long long)requests * rows * group, prefix_len, 0);
-        p.own0 = p.prefix.splits * requests * size;
+        p.own0 = (long long)p.prefix.splits * requests * size;
     }
     if (prefix_len > 0 || p.own.splits > 1 || p.own.slots > 0) {
         p.parts = p.own0 + (p.own.slots > 0 ? p.own.slots : (long long)requests * p.own.splits) * size;
@@ -831,13 +838,12 @@ using namespace mt;
 extern "C" {
 
 size_t mt_attention_kv8_workspace(const mt_ctx* ctx, const mt_kv8_cache* cache, int requests, int rows, int hq, int window) {
-    return ctx && cache && requests > 0 && rows > 0 && hq > 0 ? make_plan(ctx, 0, cache, requests, rows, hq, window).bytes : 0;
+    return ctx && plannable(0, cache, requests, rows, hq, window) ? make_plan(ctx, 0, cache, requests, rows, hq, window).bytes : 0;
 }
 
 size_t mt_attention_prefix_kv8_workspace(const mt_ctx* ctx, int prefix_len, const mt_kv8_cache* cache, int requests,
                                          int rows, int hq) {
-    return ctx && cache && requests > 0 && rows > 0 && hq > 0 ? make_plan(ctx, prefix_len, cache, requests, rows, hq, 0).bytes
-                                                             : 0;
+    return ctx && plannable(prefix_len, cache, requests, rows, hq, 0) ? make_plan(ctx, prefix_len, cache, requests, rows, hq, 0).bytes : 0;
 }
 
 mt_status mt_attention_kv8(mt_ctx* ctx, void* stream, const float* q, int ldq, int requests, int rows, int hq,

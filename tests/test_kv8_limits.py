@@ -243,3 +243,61 @@ def test_scores_of_any_size(ctx, mt, kind, size, v_power):
     run(40, 2, 20, 1, 14, [i % 20 for i in range(40)], plen=3000)
     run(3, 2, 20, 1, 14, [0, 7, 19], plen=174)
     assert seen > 0
+
+
+# ------------------------------------------------------------------------------------------------
+# Workspace queries (on the CPU: of a context they read the number of SMs only)
+# ------------------------------------------------------------------------------------------------
+QUERIES = '''
+import ctypes, sys
+sys.path.insert(0, "tests")
+import conftest
+mt = conftest.load_package()
+context = (ctypes.c_int * 1024)(*[148] * 1024)  # whatever a context's layout, its numbers of SMs is 148
+ctx = ctypes.cast(context, ctypes.c_void_p)
+
+
+def sizes(requests, rows, hq, window=0, prefix_len=16, kv_heads=2, capacity=512, base=0):
+    c = mt.KV8CacheStruct(0, kv_heads, capacity, base, max(kv_heads * capacity, 0), None, None, None, None)
+    return (mt.lib().mt_attention_kv8_workspace(ctx, ctypes.byref(c), requests, rows, hq, window),
+            mt.lib().mt_attention_prefix_kv8_workspace(ctx, prefix_len, ctypes.byref(c), requests, rows, hq))
+
+
+big = 2 ** 31 - 1
+good = sizes(1, 1, 14, capacity=20000)
+assert good[0] > 0 and good[1] > good[0], good
+for bad in (dict(hq=1), dict(hq=3), dict(hq=0), dict(hq=-2), dict(hq=1026), dict(hq=2, kv_heads=0), dict(hq=2, kv_heads=-1),
+            dict(hq=2, kv_heads=big), dict(requests=big, rows=big, capacity=1 << 30), dict(requests=-1), dict(rows=-1), dict(requests=0),
+            dict(rows=0), dict(capacity=0), dict(capacity=-5), dict(capacity=big), dict(rows=513), dict(requests=big // 14 + 1)):
+    got = sizes(**{**dict(requests=1, rows=1, hq=14), **bad})
+    assert got == (0, 0), (bad, got)
+assert sizes(1, 1, 14, window=-1)[0] == 0 and sizes(1, 1, 14, window=513)[0] == 0 and sizes(1, 1, 14, window=big)[0] == 0
+assert sizes(1, 1, 14, prefix_len=-1)[1] == 0 and sizes(1, 1, 14, prefix_len=(1 << 30) + 1)[1] == 0
+most = sizes(requests=1, rows=1 << 21, hq=1023, kv_heads=1, capacity=1 << 30, prefix_len=1 << 30)
+assert most[1] >= (1 << 21) * 1023 * 66 * 4 * 2, most
+print("sizes fine")
+'''
+
+
+def test_workspace_queries_refuse_in_a_process_of_their_own():
+    """Sizes that the calls refuse need nothing; none of them ends the process."""
+    import os
+    import subprocess
+    import sys
+    got = subprocess.run([sys.executable, "-c", QUERIES], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                         capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and "sizes fine" in got.stdout, (got.returncode, got.stdout, got.stderr[-800:])
+
+
+@gpu
+def test_attention_refuses_head_counts(ctx, mt):
+    """A head count that does not go with the cache is an error of the call, with and without a prefix."""
+    import torch
+    cache, prefix = mt.KV8Cache.allocate(1, 2, 64, base=16), mt.KV8Cache.allocate(1, 2, 16)
+    q, pos = torch.zeros(1, 1024, device="cuda"), torch.full((1,), 20, dtype=torch.int32, device="cuda")
+    for hq in (1, 3, 0, -2):
+        for call in (lambda: ctx.attention_kv8(q, 1024, 1, 1, hq, pos, None, 0, cache, q.clone(), 1024),
+                     lambda: ctx.attention_prefix_kv8(q, 1024, 1, 1, hq, pos, None, prefix, 16, cache, q.clone(), 1024)):
+            with pytest.raises(mt.MingError) as e:
+                call()
+            assert e.value.status == mt.MT_ERR_SHAPE
