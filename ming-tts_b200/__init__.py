@@ -212,6 +212,15 @@ PROTOTYPES = {
 }
 
 _lib = None
+_torch = None
+
+
+def _load_torch():
+    """torch, imported with the first call that takes tensors: this module does not need it otherwise."""
+    global _torch
+    import torch
+    _torch = torch
+    return torch
 
 
 def lib() -> ctypes.CDLL:
@@ -318,11 +327,11 @@ class Context:
         self.call("attention", q, ldq, m, hq, hkv, pos0, window, kc, vc, cap, out, ldo)
 
     # 8-bit caches: `cache` and `prefix` are KV8Cache objects, the other tensors CUDA tensors, the rest as
-    # in mingcuda.h. The default stream is the current one of the context's device. A decode step is a
-    # few microseconds of GPU time, so these wrappers do little else than the call.
+    # in mingcuda.h. Tensors of another type or device, or too small for the call, are refused. The default stream
+    # is the current one of the context's device. A decode step is a few microseconds of GPU time, so these wrappers do
+    # little else than that and the call.
     def _device_stream(self) -> int:
-        import torch
-        return torch._C._cuda_getCurrentRawStream(self.device)
+        return (_torch or _load_torch())._C._cuda_getCurrentRawStream(self.device)
 
     def _enough(self, cache, requests: int):
         if cache.requests < requests:
@@ -331,37 +340,60 @@ class Context:
             raise MingError(MT_ERR_ARG, f"a cache on {cache.device}, but a context of cuda:{self.device}")
 
     def _places(self, requests: int, positions, counts):
-        import torch
-        for t in (positions, counts):
-            if t is not None and (t.dtype != torch.int32 or t.numel() < requests or not t.is_contiguous()):
+        """The addresses of positions and counts (None: none)."""
+        int32 = (_torch or _load_torch()).int32
+        for t in (positions,) if counts is None else (positions, counts):
+            if t.dtype is not int32 or t.numel() < requests or not t.is_contiguous():
                 raise TypeError(f"positions and counts are dense torch.int32 of {requests} requests, got {t.dtype} "
                                 f"{tuple(t.shape)}")
+        if positions.get_device() != self.device or counts is not None and counts.get_device() != self.device:
+            raise MingError(MT_ERR_ARG, f"positions or counts on another device than the context's cuda:{self.device}")
+        return positions.data_ptr(), None if counts is None else counts.data_ptr()
 
-    def _workspace(self, nbytes: int, given):
+    def _floats(self, name: str, t, need: int, strided: bool = False):
+        """The address of `t`: `need` fp32 values on the context's device, dense, or (strided) dense rows some way apart."""
+        if t.dtype is not (_torch or _load_torch()).float32:
+            raise TypeError(f"{name}: torch.float32, got {t.dtype}")
+        held = t.numel()
+        if not t.is_contiguous() and held:  # from the first value to the last
+            held = 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())) if strided and t.stride(-1) == 1 else 0
+        if held < need:
+            raise MingError(MT_ERR_SHAPE, f"{name}: {need} values, got {tuple(t.shape)} with strides {t.stride()}")
+        if t.get_device() != self.device:
+            raise MingError(MT_ERR_ARG, f"{name} on {t.device}, but a context of cuda:{self.device}")
+        return t.data_ptr()
+
+    def _workspace(self, nbytes: int, given, device):
         """(tensor, pointer, bytes): the caller's workspace, or a new one from torch's allocator."""
         if given is None:
-            import torch
-            given = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", self.device))
+            torch = _torch or _load_torch()
+            given = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            return given, given.data_ptr(), nbytes
+        if given.get_device() != self.device or not given.is_contiguous():
+            raise MingError(MT_ERR_ARG, f"a workspace is dense, on cuda:{self.device}, got {given.device}, strides {given.stride()}")
         return given, given.data_ptr(), given.numel() * given.element_size()
 
     def rope_cache_kv8(self, qkv, ldq, requests, rows, hq, positions, counts, inv_freq, cache, q_out, ldqo, stream=None):
         """mt_rope_cache_kv8: rotate q and k, quantise k and v into the cache."""
         self._enough(cache, requests)
-        self._places(requests, positions, counts)
-        st = lib().mt_rope_cache_kv8(self._ctx, self._device_stream() if stream is None else stream, qkv.data_ptr(), ldq,
-                                     requests, rows, hq, positions.data_ptr(),
-                                     None if counts is None else counts.data_ptr(), inv_freq.data_ptr(), cache.ref,
-                                     q_out.data_ptr(), ldqo)
+        pos, cnt = self._places(requests, positions, counts)
+        last = requests * rows - 1
+        x = self._floats("qkv", qkv, last * ldq + (hq + 2 * cache.kv_heads) * 64 if last >= 0 else 0, True)
+        y = self._floats("q_out", q_out, last * ldqo + hq * 64 if last >= 0 else 0, True)
+        inv = self._floats("inv_freq", inv_freq, 32)
+        st = lib().mt_rope_cache_kv8(self._ctx, self._device_stream() if stream is None else stream, x, ldq, requests, rows, hq,
+                                     pos, cnt, inv, cache.ref, y, ldqo)
         if st != MT_OK:
             self._check(st, "mt_rope_cache_kv8")
 
     def kv8_read(self, cache, requests, rows, positions, counts, k, v, out_capacity, stream=None):
         """mt_kv8_read: a range of positions back into fp32."""
         self._enough(cache, requests)
-        self._places(requests, positions, counts)
+        pos, cnt = self._places(requests, positions, counts)
+        need = ((requests * cache.kv_heads - 1) * out_capacity + rows) * 64 if requests > 0 and rows > 0 else 0
+        kp, vp = None if k is None else self._floats("k", k, need), None if v is None else self._floats("v", v, need)
         st = lib().mt_kv8_read(self._ctx, self._device_stream() if stream is None else stream, cache.ref, requests, rows,
-                               positions.data_ptr(), None if counts is None else counts.data_ptr(), ptr(k), ptr(v),
-                               out_capacity)
+                               pos, cnt, kp, vp, out_capacity)
         if st != MT_OK:
             self._check(st, "mt_kv8_read")
 
@@ -370,13 +402,14 @@ class Context:
         """mt_attention_kv8: causal attention over the cache. Without a workspace (a CUDA tensor), one comes
         from torch's allocator on the current stream: give one when `stream` is another."""
         self._enough(cache, requests)
-        self._places(requests, positions, counts)
+        pos, cnt = self._places(requests, positions, counts)
+        last = requests * rows - 1
+        x = self._floats("q", q, last * ldq + hq * 64 if last >= 0 else 0, True)
+        y = self._floats("out", out, last * ldo + hq * 64 if last >= 0 else 0, True)
         need = lib().mt_attention_kv8_workspace(self._ctx, cache.ref, requests, rows, hq, window)
-        keep, wp, wn = self._workspace(need, workspace) if need else (None, None, 0)
-        st = lib().mt_attention_kv8(self._ctx, self._device_stream() if stream is None else stream, q.data_ptr(), ldq,
-                                    requests, rows, hq, positions.data_ptr(),
-                                    None if counts is None else counts.data_ptr(), window, cache.ref, out.data_ptr(), ldo,
-                                    wp, wn)
+        keep, wp, wn = self._workspace(need, workspace, cache.device) if need else (None, None, 0)
+        st = lib().mt_attention_kv8(self._ctx, self._device_stream() if stream is None else stream, x, ldq, requests, rows, hq,
+                                    pos, cnt, window, cache.ref, y, ldo, wp, wn)
         if st != MT_OK:
             self._check(st, "mt_attention_kv8")
 
@@ -387,14 +420,15 @@ class Context:
         self._enough(cache, requests)
         if prefix is not None:
             self._enough(prefix, 1)
-        self._places(requests, positions, counts)
+        pos, cnt = self._places(requests, positions, counts)
+        last = requests * rows - 1
+        x = self._floats("q", q, last * ldq + hq * 64 if last >= 0 else 0, True)
+        y = self._floats("out", out, last * ldo + hq * 64 if last >= 0 else 0, True)
         need = lib().mt_attention_prefix_kv8_workspace(self._ctx, prefix_len, cache.ref, requests, rows, hq)
-        keep, wp, wn = self._workspace(need, workspace) if need else (None, None, 0)
-        st = lib().mt_attention_prefix_kv8(self._ctx, self._device_stream() if stream is None else stream, q.data_ptr(),
-                                           ldq, requests, rows, hq, positions.data_ptr(),
-                                           None if counts is None else counts.data_ptr(),
-                                           None if prefix is None else prefix.ref, prefix_len, cache.ref, out.data_ptr(),
-                                           ldo, wp, wn)
+        keep, wp, wn = self._workspace(need, workspace, cache.device) if need else (None, None, 0)
+        st = lib().mt_attention_prefix_kv8(self._ctx, self._device_stream() if stream is None else stream, x, ldq, requests, rows,
+                                           hq, pos, cnt, None if prefix is None else prefix.ref, prefix_len, cache.ref, y, ldo,
+                                           wp, wn)
         if st != MT_OK:
             self._check(st, "mt_attention_prefix_kv8")
 
@@ -430,7 +464,7 @@ class KV8Cache:
                 raise ValueError(f"KV8Cache: strides {t.stride()} of a tensor [{requests}, {heads}, {capacity}, ...]")
         self.tensors = (k, v, k_scale, v_scale)  # kept alive
         self.k, self.v, self.k_scale, self.v_scale = self.tensors
-        self.requests, self.base, self.device, self.index = requests, base, k.device, k.device.index
+        self.requests, self.kv_heads, self.base, self.device, self.index = requests, heads, base, k.device, k.device.index
         self.struct = KV8CacheStruct(kinds[k.dtype], heads, capacity, base, stride, *(t.data_ptr() for t in self.tensors))
         self.ref = ctypes.byref(self.struct)
 

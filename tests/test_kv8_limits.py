@@ -301,3 +301,91 @@ def test_attention_refuses_head_counts(ctx, mt):
             with pytest.raises(mt.MingError) as e:
                 call()
             assert e.value.status == mt.MT_ERR_SHAPE
+
+
+# ------------------------------------------------------------------------------------------------
+# Tensors of the Python calls (on the CPU: refused before anything reads them)
+# ------------------------------------------------------------------------------------------------
+def tensor_calls(mt, on="cpu"):
+    """Per call of Context: its tensors by name (2 requests of 3 rows, 4 heads on 2), and the call itself with some replaced."""
+    import torch
+    from types import SimpleNamespace
+    ctx = object.__new__(mt.Context)
+    ctx.device = 0
+    cache = SimpleNamespace(requests=2, kv_heads=2, index=0, device="cuda:0", ref=None)
+    qkv, q, pos = torch.zeros(6, 512, device=on), torch.zeros(6, 256, device=on), torch.zeros(2, dtype=torch.int32, device=on)
+    append = dict(qkv=qkv, positions=pos, counts=pos, inv_freq=torch.zeros(32, device=on), q_out=q)
+    read = dict(positions=pos, counts=pos, k=torch.zeros(2, 2, 5, 64, device=on), v=torch.zeros(2, 2, 5, 64, device=on))
+    attend = dict(q=q, positions=pos, counts=pos, out=q.clone())
+    return [
+        (append, lambda a: ctx.rope_cache_kv8(a["qkv"], 512, 2, 3, 4, a["positions"], a["counts"], a["inv_freq"], cache, a["q_out"], 256)),
+        (read, lambda a: ctx.kv8_read(cache, 2, 3, a["positions"], a["counts"], a["k"], a["v"], 5)),
+        (attend, lambda a: ctx.attention_kv8(a["q"], 256, 2, 3, 4, a["positions"], a["counts"], 0, cache, a["out"], 256)),
+        (attend, lambda a: ctx.attention_prefix_kv8(a["q"], 256, 2, 3, 4, a["positions"], a["counts"], cache, 3, cache, a["out"], 256)),
+    ]
+
+
+def test_calls_refuse_tensors_of_the_host(mt, monkeypatch):
+    """None of them reaches the library, with everything else in order."""
+    import torch
+    monkeypatch.setattr(mt, "lib", lambda: pytest.fail("the library was called"))
+    real = torch.Tensor.get_device
+    for args, call in tensor_calls(mt):
+        for host in args:
+            others = [id(t) for name, t in args.items() if name != host and t is not args[host]]
+            monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0 if id(t) in others else real(t))
+            with pytest.raises(mt.MingError) as e:
+                call(args)
+            assert e.value.status == mt.MT_ERR_ARG, host
+
+
+def test_calls_refuse_tensors_of_another_type_or_size(mt, monkeypatch):
+    import torch
+    monkeypatch.setattr(mt, "lib", lambda: pytest.fail("the library was called"))
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    for args, call in tensor_calls(mt):
+        for name in args:
+            if name in ("positions", "counts"):
+                continue
+            for dtype in (torch.bfloat16, torch.float16, torch.float64, torch.int32):
+                with pytest.raises(TypeError):
+                    call({**args, name: args[name].to(dtype)})
+            short = args[name].flatten()
+            gap = 128 if name in ("k", "v") else 0  # rows 3 and 4 of the last head are not part of the call
+            spread = torch.zeros(4, 512)[:, ::2] if name != "inv_freq" else torch.zeros(20)[::2]
+            for bad in (short[:len(short) - gap - 1], args[name][:1], spread[:0]) + ((spread,) if name in ("q", "out", "q_out") else ()) + (
+                    (torch.zeros(2, 2, 5, 128)[..., :64],) if name in ("k", "v") else ()):
+                with pytest.raises(mt.MingError) as e:
+                    call({**args, name: bad})
+                assert e.value.status == mt.MT_ERR_SHAPE, name
+
+
+def test_workspaces_of_the_host_or_with_gaps_are_refused(mt):
+    import torch
+    ctx = object.__new__(mt.Context)
+    ctx.device = 0
+    with pytest.raises(mt.MingError) as e:
+        ctx._workspace(64, torch.zeros(64, dtype=torch.uint8), None)
+    assert e.value.status == mt.MT_ERR_ARG
+
+
+@gpu
+def test_calls_take_views(ctx, mt):
+    """q as the first columns of qkv and rows of a larger buffer, as before."""
+    import torch
+    hq, hkv = 4, 2
+    g = torch.Generator(device="cuda").manual_seed(3)
+    qkv = torch.randn(6, (hq + 2 * hkv) * 64, device="cuda", generator=g)
+    pos, inv = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.from_numpy(base.INV_FREQ).cuda()
+    outs = []
+    for view in (False, True):
+        cache = mt.KV8Cache.allocate(2, hkv, 8)
+        x, out = qkv.clone(), torch.zeros(9, hq * 64 + 8, device="cuda")
+        q = x[:, :hq * 64] if view else torch.empty(6, hq * 64, device="cuda")
+        ld = x.shape[1] if view else hq * 64
+        ctx.rope_cache_kv8(x, x.shape[1], 2, 3, hq, pos, None, inv, cache, q, ld)
+        ctx.attention_kv8(q, ld, 2, 3, hq, pos, None, 0, cache, out[2:8, 8:], hq * 64 + 8)
+        ctx.check()
+        assert torch.all(out[:2] == 0) and torch.all(out[8:] == 0) and torch.all(out[:, :8] == 0)
+        outs.append(out)
+    assert torch.equal(outs[0], outs[1])
