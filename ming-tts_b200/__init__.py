@@ -363,11 +363,16 @@ class Context:
             raise MingError(MT_ERR_ARG, f"{name} on {t.device}, but a context of cuda:{self.device}")
         return t.data_ptr()
 
-    def _workspace(self, nbytes: int, given, device):
-        """(tensor, pointer, bytes): the caller's workspace, or a new one from torch's allocator."""
+    def _workspace(self, nbytes: int, given, device, stream):
+        """(tensor, pointer, bytes): the caller's workspace, or a new one from torch's allocator, which gives its
+        memory to later calls on the stream that it was allocated on: the call's."""
         if given is None:
             torch = _torch or _load_torch()
-            given = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            if stream is None:
+                given = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            else:
+                with torch.cuda.stream(torch.cuda.ExternalStream(stream, device)):
+                    given = torch.empty(nbytes, dtype=torch.uint8, device=device)
             return given, given.data_ptr(), nbytes
         if given.get_device() != self.device or not given.is_contiguous():
             raise MingError(MT_ERR_ARG, f"a workspace is dense, on cuda:{self.device}, got {given.device}, strides {given.stride()}")
@@ -400,14 +405,14 @@ class Context:
     def attention_kv8(self, q, ldq, requests, rows, hq, positions, counts, window, cache, out, ldo, workspace=None,
                       stream=None):
         """mt_attention_kv8: causal attention over the cache. Without a workspace (a CUDA tensor), one comes
-        from torch's allocator on the current stream: give one when `stream` is another."""
+        from torch's allocator on the call's stream."""
         self._enough(cache, requests)
         pos, cnt = self._places(requests, positions, counts)
         last = requests * rows - 1
         x = self._floats("q", q, last * ldq + hq * 64 if last >= 0 else 0, True)
         y = self._floats("out", out, last * ldo + hq * 64 if last >= 0 else 0, True)
         need = lib().mt_attention_kv8_workspace(self._ctx, cache.ref, requests, rows, hq, window)
-        keep, wp, wn = self._workspace(need, workspace, cache.device) if need else (None, None, 0)
+        keep, wp, wn = self._workspace(need, workspace, cache.device, stream) if need else (None, None, 0)
         st = lib().mt_attention_kv8(self._ctx, self._device_stream() if stream is None else stream, x, ldq, requests, rows, hq,
                                     pos, cnt, window, cache.ref, y, ldo, wp, wn)
         if st != MT_OK:
@@ -425,7 +430,7 @@ class Context:
         x = self._floats("q", q, last * ldq + hq * 64 if last >= 0 else 0, True)
         y = self._floats("out", out, last * ldo + hq * 64 if last >= 0 else 0, True)
         need = lib().mt_attention_prefix_kv8_workspace(self._ctx, prefix_len, cache.ref, requests, rows, hq)
-        keep, wp, wn = self._workspace(need, workspace, cache.device) if need else (None, None, 0)
+        keep, wp, wn = self._workspace(need, workspace, cache.device, stream) if need else (None, None, 0)
         st = lib().mt_attention_prefix_kv8(self._ctx, self._device_stream() if stream is None else stream, x, ldq, requests, rows,
                                            hq, pos, cnt, None if prefix is None else prefix.ref, prefix_len, cache.ref, y, ldo,
                                            wp, wn)

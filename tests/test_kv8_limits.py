@@ -365,7 +365,7 @@ def test_workspaces_of_the_host_or_with_gaps_are_refused(mt):
     ctx = object.__new__(mt.Context)
     ctx.device = 0
     with pytest.raises(mt.MingError) as e:
-        ctx._workspace(64, torch.zeros(64, dtype=torch.uint8), None)
+        ctx._workspace(64, torch.zeros(64, dtype=torch.uint8), None, None)
     assert e.value.status == mt.MT_ERR_ARG
 
 
@@ -389,3 +389,47 @@ def test_calls_take_views(ctx, mt):
         assert torch.all(out[:2] == 0) and torch.all(out[8:] == 0) and torch.all(out[:, :8] == 0)
         outs.append(out)
     assert torch.equal(outs[0], outs[1])
+
+
+@gpu
+@pytest.mark.parametrize("behind", [False, True])
+def test_default_workspace_on_another_stream(ctx, mt, behind):
+    """A call on a stream given by its handle, without a workspace: memory that the current stream allocates after
+    the call does not share with the workspace that the call is still to use."""
+    import torch
+    hq, hkv, n, plen = 14, 2, 20000, 4000
+    g = torch.Generator(device="cuda").manual_seed(5)
+    full = Keys("int8", 1, hkv, n, 2.0 / 127, 2.0 / 127).cache(mt, plen if behind else 0)
+    prefix = Keys("int8", 1, hkv, plen, 2.0 / 127, 2.0 / 127, seed=1).cache(mt)
+    q = torch.randn(1, hq * 64, device="cuda", generator=g)
+    pos = torch.tensor([n - 1 + (plen if behind else 0)], dtype=torch.int32, device="cuda")
+
+    def call(out, **k):
+        if behind:
+            ctx.attention_prefix_kv8(q, hq * 64, 1, 1, hq, pos, None, prefix, plen, full, out, hq * 64, **k)
+        else:
+            ctx.attention_kv8(q, hq * 64, 1, 1, hq, pos, None, 0, full, out, hq * 64, **k)
+
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    call(want)
+    need = (mt.lib().mt_attention_prefix_kv8_workspace(ctx.handle, plen, full.ref, 1, 1, hq) if behind else
+            mt.lib().mt_attention_kv8_workspace(ctx.handle, full.ref, 1, 1, hq, 0))
+    assert need > 0
+    call(out, stream=torch.cuda.default_stream().cuda_stream)
+    assert torch.equal(out, want)
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    for _ in range(5):
+        with torch.cuda.stream(other):
+            torch.cuda._sleep(4_000_000)  # some ms in which the call waits
+        call(out, stream=other.cuda_stream)
+        mine = [torch.full((need,), 255, dtype=torch.uint8, device="cuda") for _ in range(3)]  # NaN, as fp32
+        while not other.query():  # for as long as the call may read and write
+            for t in mine:
+                t.fill_(255)
+            torch.cuda.current_stream().synchronize()
+        torch.cuda.synchronize()
+        assert all(bool((t == 255).all()) for t in mine)
+        assert torch.equal(out, want)
+        del mine
