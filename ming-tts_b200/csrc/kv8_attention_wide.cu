@@ -126,8 +126,9 @@ struct Shared {
     float unit;                                                        // brings the first value scales near 1
     uint64_t k_full[WD_STAGES], k_free[WD_STAGES], v_full[WD_STAGES], v_free[WD_STAGES];
     uint64_t q_ready[2], s_ready[2][2], p_ready[2][2], o_ready[2][2];     // by row tile (and key tile parity)
+    uint64_t idle;                                                        // all matrix instructions are done
     uint32_t tmem;
-    int abort;
+    int abort, never;  // never stays 0: for the wait that goes on after an abort
 };
 
 // Units of rows (see kv8_move). The factor 2^unit is in the value scales already, for all rows of a block; a row's lift
@@ -345,7 +346,8 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
             mbar_init(&sh.o_ready[i][0], 1);
             mbar_init(&sh.o_ready[i][1], 1);
         }
-        sh.abort = 0;
+        mbar_init(&sh.idle, 1);
+        sh.abort = sh.never = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == WD_ROW_WARPS + WD_CONVERT_WARPS) {
@@ -559,11 +561,12 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
             if (n > 0) load(u_first + n * WD_KEYS);
             const int st = n & (WD_STAGES - 1);
             const uint32_t reuse = ((n / WD_STAGES) & 1) ^ 1;
-            if (n >= WD_STAGES && !mbar_wait(&sh.k_free[st], reuse, status, 23, abort)) break;
+            // A wait that gives up ends the loop for the whole warp: its lanes meet again below.
+            if (n >= WD_STAGES && !__all_sync(0xffffffffu, mbar_wait(&sh.k_free[st], reuse, status, 23, abort))) break;
             store(stages + st * WD_STAGE, k);
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.k_full[st]);
-            if (n >= WD_STAGES && !mbar_wait(&sh.v_free[st], reuse, status, 24, abort)) break;
+            if (n >= WD_STAGES && !__all_sync(0xffffffffu, mbar_wait(&sh.v_free[st], reuse, status, 24, abort))) break;
             store(stages + (WD_STAGES + st) * WD_STAGE, v);
             if (part == 0) {
 #pragma unroll
@@ -634,6 +637,9 @@ __device__ __forceinline__ void wide_block(const PassArgs& a, int chunk, unsigne
             }
             if (ok) mma_done(&sh.v_free[n & (WD_STAGES - 1)]);
         }
+        // Also after a wait that gave up: shared memory and TMEM stay until nothing uses them.
+        mma_done(&sh.idle);
+        mbar_wait(&sh.idle, 0, status, 29, &sh.never);
         }
     }
     __syncwarp();
