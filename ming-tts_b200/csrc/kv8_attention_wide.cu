@@ -133,14 +133,19 @@ struct Shared {
 
 // Units of rows (see kv8_move). The factor 2^unit is in the value scales already, for all rows of a block; a row's lift
 // does the rest up to 2^16 either way, at the price of the exponents' rounding to 2^-20, and the fast path knows no
-// other. Rows whose first values are further from the first of the block go the slow way, with an extra of their own.
+// other. Rows whose first values are further from the first of the block, or whose scores have no fraction in fp32
+// (see kv8_score), go the slow way, with an extra of their own.
 constexpr float WD_LIFT = 16.f, WD_LARGEST = 0x1p127f;
 __device__ __forceinline__ float row_lift(float total, float unit) { return fminf(WD_LIFT, fmaxf(-WD_LIFT, total - unit)); }
 __device__ __forceinline__ float row_extra(float total, float unit) {
     if (total == KV8_UNSET) return 1.f;
     return kv8_power(total > 0.5f * KV8_FAR ? total - KV8_FAR : total - row_lift(total, unit));
 }
-__device__ __forceinline__ bool row_usual(float total, float unit) { return fabsf(total - unit) <= WD_LIFT; }
+__device__ __forceinline__ bool row_usual(float off, float total, float unit) { return fabsf(total - unit) <= WD_LIFT && fabsf(off) < 0x1p24f; }
+// Not that far, but without products that count (yet).
+__device__ __forceinline__ bool row_plain(float off, float total, float unit) {
+    return (total == KV8_UNSET || fabsf(total - unit) <= WD_LIFT) && (off == KV8_REF_NONE || fabsf(off) < 0x1p24f);
+}
 
 // The state of a lane's two rows; off and total: see kv8_move. A sum is the lane's own part of the row.
 struct RowState {
@@ -195,36 +200,40 @@ __device__ __forceinline__ void row_rescale(uint32_t tm, int chunks, float f0, f
 }
 
 // Weights of 16 keys (s: scores, k and v: the keys' scales): 2^(score - off), their sums, and times the
-// value scales and the rows' extra (unless 2^unit does for all of them: see row_usual) as planes. Returns the largest product.
-template <bool SLOW>
+// value scales as planes. MASK: rows see some of the keys; OWN: units are the rows' own. Returns the largest product.
+template <bool MASK, bool OWN>
 __device__ __forceinline__ float row_products(const TileKeys& t, const RowState& row, int c, const float (&s)[8], uint32_t (&planes)[8],
                                               float (&add)[2]) {
     const float2 k[2] = {*reinterpret_cast<const float2*>(t.ks + 16 * c), *reinterpret_cast<const float2*>(t.ks + 16 * c + 8)};
-    const float* const vs = (SLOW && !row.usual ? t.raw() : t.vs) + 16 * c;
+    const float* const vs = (OWN ? t.raw() : t.vs) + 16 * c;
     const float2 v[2] = {*reinterpret_cast<const float2*>(vs), *reinterpret_cast<const float2*>(vs + 8)};
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         float sum[2];
-        const float extra = SLOW && !row.usual ? row_extra(row.total[i], t.unit()) : 1.f;
+        const float extra = OWN ? row_extra(row.total[i], t.unit()) : 1.f;
 #pragma unroll
         for (int n = 0; n < 2; n++) {
             const int u = t.u + 16 * c + 8 * n;
-            const bool on0 = !SLOW || (u >= row.lo[i] && u <= row.hi[i]), on1 = !SLOW || (u + 1 >= row.lo[i] && u + 1 <= row.hi[i]);
+            const bool on0 = !MASK || (u >= row.lo[i] && u <= row.hi[i]), on1 = !MASK || (u + 1 >= row.lo[i] && u + 1 <= row.hi[i]);
             // key scale and rs first: see kv8_attention.cu
             const float k0 = k[n].x * row.rs[i], k1 = k[n].y * row.rs[i], s0 = s[4 * n + 2 * i], s1 = s[4 * n + 2 * i + 1];
-            float p0 = ex2(SLOW ? kv8_score(s0, k0) - row.off[i] : fmaf(s0, k0, -row.off[i]));
-            float p1 = ex2(SLOW ? kv8_score(s1, k1) - row.off[i] : fmaf(s1, k1, -row.off[i]));
-            if (SLOW) {
+            float p0 = ex2(OWN ? kv8_score(s0, k0) - row.off[i] : fmaf(s0, k0, -row.off[i]));
+            float p1 = ex2(OWN ? kv8_score(s1, k1) - row.off[i] : fmaf(s1, k1, -row.off[i]));
+            if (MASK) {
                 p0 = on0 ? p0 : 0.f;
                 p1 = on1 ? p1 : 0.f;
             }
             sum[n] = p0 + p1;
             p0 *= v[n].x;
             p1 *= v[n].y;
-            if (SLOW) {  // a scale of a key that this row does not see may be NaN
-                p0 = on0 ? p0 * extra : 0.f;
-                p1 = on1 ? p1 * extra : 0.f;
+            if (OWN) {
+                p0 *= extra;
+                p1 *= extra;
+            }
+            if (MASK) {  // a scale of a key that this row does not see may be NaN
+                p0 = on0 ? p0 : 0.f;
+                p1 = on1 ? p1 : 0.f;
             }
             top = fmaxf(top, fmaxf(fabsf(p0), fabsf(p1)));
             split_half2(p0, p1, planes[2 * n + i], planes[4 + 2 * n + i]);
@@ -245,7 +254,7 @@ __device__ __forceinline__ int row_weights(uint32_t tm, const TileKeys& t, RowSt
         uint32_t planes[8];
         tmem_ld_tile(tm + 16 * c, s);
         tmem_ld_wait(s);
-        const float top = row_products<false>(t, row, c, s, planes, add);
+        const float top = row_products<false, false>(t, row, c, s, planes, add);
         if (__any_sync(0xffffffffu, !(top <= KV8_PRODUCT_MAX && add[0] <= KV8_WEIGHT_MAX && add[1] <= KV8_WEIGHT_MAX))) break;
         row.sum[0] += add[0];
         row.sum[1] += add[1];
@@ -266,28 +275,33 @@ __device__ __forceinline__ void row_weights_slowly(uint32_t tm, const TileKeys& 
         tmem_ld_tile(tm + 16 * c, s);
         tmem_ld_wait(s);
 #pragma unroll 1
-        for (int tries = 0; tries < 2; tries++) {
-            const float top = row_products<true>(t, row, c, s, planes, add);
-            if (!__any_sync(0xffffffffu, !(top <= KV8_PRODUCT_MAX && add[0] <= KV8_WEIGHT_MAX && add[1] <= KV8_WEIGHT_MAX &&
-                                           row.total[0] != KV8_UNSET && row.total[1] != KV8_UNSET))) break;
-            settle(1);
-            float f[2];
+        for (bool move = __any_sync(0xffffffffu, row.total[0] == KV8_UNSET || row.total[1] == KV8_UNSET);; move = true) {
+            if (move) {
+                settle(1);
+                float f[2];
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                float z[4], v[4];
+                for (int i = 0; i < 2; i++) {
+                    float z[4], v[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int key = 16 * c + 8 * (j >> 1) + (j & 1);
-                    const bool on = t.u + key >= row.lo[i] && t.u + key <= row.hi[i];
-                    z[j] = on ? kv8_score(s[4 * (j >> 1) + 2 * i + (j & 1)], t.ks[key] * row.rs[i]) : -INFINITY;
-                    v[j] = on ? fabsf(t.raw()[key]) : 0.f;
+                    for (int j = 0; j < 4; j++) {
+                        const int key = 16 * c + 8 * (j >> 1) + (j & 1);
+                        const bool on = t.u + key >= row.lo[i] && t.u + key <= row.hi[i];
+                        z[j] = on ? kv8_score(s[4 * (j >> 1) + 2 * i + (j & 1)], t.ks[key] * row.rs[i]) : -INFINITY;
+                        v[j] = on ? fabsf(t.raw()[key]) : 0.f;
+                    }
+                    const Kv8Move by = kv8_move(z, v, row.off[i], row.total[i], [&](float total) { return row_lift(total, t.unit()); });
+                    if (by.sums != 1.f || by.outputs != 1.f) row.scale(i, by);
+                    f[i] = by.outputs;
                 }
-                const Kv8Move move = kv8_move(z, v, row.off[i], row.total[i], [&](float total) { return row_lift(total, t.unit()); });
-                if (move.sums != 1.f || move.outputs != 1.f) row.scale(i, move);
-                f[i] = move.outputs;
+                row.usual = __all_sync(0xffffffffu, row_usual(row.off[0], row.total[0], t.unit()) && row_usual(row.off[1], row.total[1], t.unit()));
+                row_rescale(tm, c, f[0], f[1]);
             }
-            row.usual = __all_sync(0xffffffffu, row_usual(row.total[0], t.unit()) && row_usual(row.total[1], t.unit()));
-            row_rescale(tm, c, f[0], f[1]);
+            float top;
+            if (__all_sync(0xffffffffu, row_plain(row.off[0], row.total[0], t.unit()) && row_plain(row.off[1], row.total[1], t.unit())))
+                top = row_products<true, false>(t, row, c, s, planes, add);
+            else
+                top = row_products<true, true>(t, row, c, s, planes, add);
+            if (move || !__any_sync(0xffffffffu, !(top <= KV8_PRODUCT_MAX && add[0] <= KV8_WEIGHT_MAX && add[1] <= KV8_WEIGHT_MAX))) break;
         }
         row.sum[0] += add[0];
         row.sum[1] += add[1];
