@@ -108,10 +108,11 @@ __device__ __forceinline__ uint32_t encode4(float4 x4, float scale, float rcp) {
 // stores of a head are whole 128-byte lines and a code row is 16 words. The angles are made in 64 bits,
 // one thread each (a position of 10^5 leaves an fp32 angle with 2 digits less, and a code is the same for
 // every caller only if the rotated key is: rounding it once from 64 bits makes it so), while the loads of
-// the group's first heads are under way. Queries are turned in 32 bits.
-// A decode step is bounded by its launch (2.5 us for 1 to 64 requests of 14 + 2 + 2 heads), prompts by issue and
-// latency: 4128 rows in 9.6 us, 3.6 TB/s; 1764 instructions a row before angles, divisions and conversions were
-// shared out as here, 1000 now.
+// the group's first heads are under way. Queries are not quantised, and are turned in 32 bits with cosines and sines
+// rounded once from 64: 3.6e-8 off in the mean instead of one rounding's 2.5e-8, a tenth of what attention adds.
+// A decode step is bounded by its launch (2.7 us for 1 to 64 requests of 14 + 2 + 2 heads), prompts by latency (memory
+// and 64-bit angles, 49% of the issue slots used): 4128 rows in 8.6 us, 4.0 TB/s; 1764 instructions a row before
+// angles, divisions and conversions were shared out as here, 1000 now.
 template <int KIND>
 __global__ void __launch_bounds__(AP_THREADS, 3) rope_cache_kv8_kernel(const AppendArgs a) {
     __shared__ __align__(16) double turn[AP_MAX_ROWS][2][32];  // cos, sin

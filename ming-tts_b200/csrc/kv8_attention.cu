@@ -21,9 +21,11 @@
 //     scores, column g of half j is key 4 (g / 2) + 2 j + g % 2, so lane t's scores are keys 4t .. 4t+3
 //     values, contraction index 2t, 2t+1, 2t+8, 2t+9 is key 4t .. 4t+3; column g of block i is dimension
 //     8 g + i, so lane t's outputs are dimensions 16 t .. 16 t + 15.
-// Bounded by instruction issue: 332 a tile of 16 keys, of which 16 are matrix instructions and some 90 the
-// conversion of codes, 57% of the issue slots used at 16 warps an SM; 64 requests of 8000 keys run at half of
-// the copy bandwidth. Tiles of 16 and 32 rows (the planes as operands of their own, each code converted once
+// Bounded by latency: a warp is one chain of dependent steps a key tile (codes, conversion, scores, exponentials,
+// planes, products), and registers leave 4 warps a scheduler. 64 requests of 8000 keys take 43 us, half of the copy
+// bandwidth: 336 instructions a tile of 16 keys (16 matrix instructions, some 90 to convert codes) use 56% of the issue
+// slots, and a warp waits 1.7 cycles an instruction for the fixed latency of the one before, 0.6 each for the matrix
+// unit and shared memory. Tiles of 16 and 32 rows (the planes as operands of their own, each code converted once
 // for all of them) were no faster at any size: 974 instructions a tile of 32, but registers for 8 warps an
 // SM, which used 40% of the slots, and 16 rows over 300 keys took 9.1 and 13.6 us instead of 6.3. Many rows
 // against many keys go to kv8_attention_wide.cu.
