@@ -239,7 +239,7 @@ __device__ __forceinline__ Kv8Move kv8_move(const float (&z)[4], const float (&v
     const bool was_far = !unset && total > 0.5f * KV8_FAR;
     const float old = was_far ? total - KV8_FAR : total;
     const float old_lift = unset || was_far ? 0.f : lift(old), old_extra = unset ? 0.f : old - old_lift;  // of 2
-    const float now = product(off) * kv8_power(old_extra);
+    const float now = __any_sync(0xffffffffu, !unset) ? product(off) * kv8_power(old_extra) : 0.f;
     const bool move = most > -INFINITY && (unset || most - off > 90.f || now > KV8_PRODUCT_MAX);
     const float ref = fmaxf(off + old_lift, most);
     const float then = product(ref);

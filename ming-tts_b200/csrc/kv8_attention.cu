@@ -638,12 +638,13 @@ PassPlan plan_pass(int sm_count, long long units, int requests, long long qrows,
     // Which kernel: by their estimated times, in ns. The warp kernel takes 5 ps a (row, head) pair and key that
     // it sees, once the GPU is full; a wide block takes 14 us to start and finish, 2.2 us for 64 keys (1.4 us
     // with up to 128 rows), and a later one on the same SM another 8 us. Measured in us, wide against warp
-    // kernel (14 heads on 2 unless said): one request of 16 rows over 300 keys 12.6 / 6.4, 16 over 4000
-    // 15.1 / 11.6, 512 over themselves 21.5 / 20.1, 37 over 4000 keys
-    // 19.1 / 15.7, 64 over 4000 19.2 / 23.5; 8 requests of 8 rows over 4000 22.1 / 26.4,
-    // of 64 rows over 1000 23.8 / 40.0; 64 requests of 8 rows
-    // over 400 keys 19.1 / 19.9, of 16 rows 19.4 / 34.6; 11 requests of 113 rows over 350, 16 heads on 16,
-    // 42.2 / 53.9; a prefix of 9000 for 32 requests 21.5 / 24.1, for 414 rows 64.8 / 291. Its keys are split over
+    // kernel, one call behind the other in a graph (int8, 14 heads on 2 unless said): one request of 16 rows over
+    // 300 keys 12.7 / 5.2, 16 over 4000 17.7 / 11.2, 512 over themselves 22.3 / 19.8, 37 over 4000 22.5 / 14.3,
+    // 64 over 4000 22.7 / 22.0; 8 requests of 8 rows over 4000 24.2 / 25.8, of 64 rows over 1000 24.3 / 36.8;
+    // 64 requests of 8 rows over 400 keys 21.4 / 18.6, of 16 rows 22.8 / 33.4; 11 requests of 113 rows over 350,
+    // 16 heads on 16, 39.2 / 42.1; a prefix of 9000 for 32 requests 24.0 / 21.9, for 414 rows 73.7 / 289. With a
+    // window the estimate counts keys that rows do not see: 700 rows over 1 18.1 / 8.9, 400 over 65 20.1 / 8.6,
+    // 4096 over 512 71.8 / 141, all of them wide. Its keys are split over
     // the SMs that its blocks leave free, two tiles a part or more (four: 64 rows over 4000 keys 24.0).
     {
         const long long row_blocks = (qrows + KV8_WIDE_ROWS - 1) / KV8_WIDE_ROWS, blocks = units * row_blocks;

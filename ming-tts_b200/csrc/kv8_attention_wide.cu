@@ -29,9 +29,9 @@
 //
 // Bounded by the row warps: 22 instructions a score, two thirds of the SM's issue slots, the rest their waits for TMEM
 // and for one another; 16 bytes a thread of the 96 registers spill, beside the loops. 2.2 us for 64 keys of 256 rows in
-// the steady state, 14 us more for a block's start and end. 4096 rows over themselves, 14 heads on 2, e4m3: 131 us,
-// 462 TFLOP/s of matrix work in two planes; the warp kernel took 304. The same with int8, 5 instructions for 4 codes
-// instead of 2, takes 160 us.
+// the steady state, 14 us more for a block's start and end. 4096 rows over themselves, 14 heads on 2, e4m3: 130 us,
+// 464 TFLOP/s of matrix work in two planes; the warp kernel took 304. The same with int8, 5 instructions for 4 codes
+// instead of 2, takes 157 us.
 #include <math.h>
 
 #include "kv8.cuh"
@@ -277,7 +277,7 @@ __device__ __forceinline__ void row_weights_slowly(uint32_t tm, const TileKeys& 
         tmem_ld_tile(tm + 16 * c, s);
         tmem_ld_wait(s);
 #pragma unroll 1
-        for (bool move = __any_sync(0xffffffffu, row.total[0] == KV8_UNSET || row.total[1] == KV8_UNSET);; move = true) {
+        for (bool move = !row.usual && __any_sync(0xffffffffu, row.total[0] == KV8_UNSET || row.total[1] == KV8_UNSET);; move = true) {
             if (move) {
                 settle(1);
                 float f[2];
@@ -299,7 +299,7 @@ __device__ __forceinline__ void row_weights_slowly(uint32_t tm, const TileKeys& 
                 row_rescale(tm, c, f[0], f[1]);
             }
             float top;
-            if (__all_sync(0xffffffffu, row_plain(row.off[0], row.total[0], t.unit()) && row_plain(row.off[1], row.total[1], t.unit())))
+            if (row.usual || __all_sync(0xffffffffu, row_plain(row.off[0], row.total[0], t.unit()) && row_plain(row.off[1], row.total[1], t.unit())))
                 top = row_products<true, false>(t, row, c, s, planes, add);
             else
                 top = row_products<true, true>(t, row, c, s, planes, add);
