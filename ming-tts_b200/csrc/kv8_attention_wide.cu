@@ -27,7 +27,7 @@
 // and g + 8 (its slots 0 and 1). Four such warps a scheduler hide one another's latencies: with 8 warps of
 // 32 rows a key tile took 3400 cycles, of which 2200 were these warps' own.
 //
-// Bounded by the row warps: 22 instructions a score, two thirds of the SM's issue slots, the rest their waits for TMEM
+// Bounded by the row warps: 21 instructions a score, two thirds of the SM's issue slots, the rest their waits for TMEM
 // and for one another; 16 bytes a thread of the 96 registers spill, beside the loops. 2.2 us for 64 keys of 256 rows in
 // the steady state, 14 us more for a block's start and end. 4096 rows over themselves, 14 heads on 2, e4m3: 130 us,
 // 464 TFLOP/s of matrix work in two planes; the warp kernel took 304. The same with int8, 5 instructions for 4 codes
